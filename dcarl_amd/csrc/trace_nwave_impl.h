@@ -262,7 +262,6 @@ __global__ __launch_bounds__((NW * nwv_max_slices<NA, NW>() * WAVE)) void trace_
                                                            // does not kill the HIP context either: the wave raises the library's fault
                                                            // word (dcarl_trace_status reports it) and ends; its partners, waiting
                                                            // for ITS hand-overs, follow the same way.  The launch's outputs are void then.
-        const int one = 1;
 #ifndef DCARL_SPIN_SLEEP
 #define DCARL_SPIN_SLEEP 1                                 // s_sleep argument between two polls (64 clocks each); -1: no sleep at all
 #endif
@@ -283,12 +282,14 @@ __global__ __launch_bounds__((NW * nwv_max_slices<NA, NW>() * WAVE)) void trace_
 #endif
             "s_branch 1b\n\t"
             "3:\n\t"
-            "s_store_dword %5, %4, 0x0 glc\n\t"
-            "s_waitcnt lgkmcnt(0)\n\t"
-            "s_dcache_wb\n\t"
+            "s_waitcnt lgkmcnt(0)\n\t"           // given up: the wave ends here, so its two registers carry the vector store of the fault word
+            "v_mov_b32 %0, 0\n\t"
+            "v_mov_b32 %2, 1\n\t"
+            "global_store_dword %0, %2, %4 sc0 sc1\n\t"
+            "s_waitcnt vmcnt(0)\n\t"
             "s_endpgm\n\t"
             "2:"
-            : "+v"(seen), "+s"(budget) : "v"(addr), "s"(need), "s"(fault), "s"(one) : "vcc", "scc", "memory");
+            : "+v"(seen), "+s"(budget) : "v"(addr), "s"(need), "s"(fault) : "vcc", "scc", "memory");
         if constexpr (FENCED) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
     };
     auto publish = [&](int* counter, int value) __attribute__((always_inline)) {
