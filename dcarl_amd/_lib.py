@@ -49,6 +49,20 @@ class CFrenetLimits(C.Structure):
                 ("check_radius", C.c_double), ("move_gap", C.c_double), ("n_predict", C.c_int32)]
 
 
+class CRecurrence(C.Structure):
+    _fields_ = [("N", C.c_int64), ("D", C.c_int64), ("E", C.c_int64), ("ep_off", C.c_void_p), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("gate", C.c_void_p), ("ldg", C.c_int64), ("h0", C.c_void_p), ("ldh0", C.c_int64), ("gate_value", C.c_double),
+                ("gate_kind", C.c_int32), ("reverse", C.c_int32), ("type", C.c_int32), ("reserved", C.c_int32)]
+
+
+class CScores(C.Structure):
+    _fields_ = [("scores", C.c_void_p), ("B", C.c_int64), ("V", C.c_int64), ("ld_scores", C.c_int64), ("taken", C.c_void_p),
+                ("taken_off", C.c_void_p), ("n_taken", C.c_int64), ("given", C.c_void_p), ("repetition", C.c_void_p),
+                ("frequency", C.c_void_p), ("presence", C.c_void_p), ("bias", C.c_void_p), ("ld_bias", C.c_int64),
+                ("allowed", C.c_void_p), ("ld_allowed", C.c_int64), ("repetition_value", C.c_float), ("frequency_value", C.c_float),
+                ("presence_value", C.c_float), ("type", C.c_int32), ("id_bytes", C.c_int32), ("reserved", C.c_int32)]
+
+
 class CDeviceInfo(C.Structure):
     _fields_ = [("arch", C.c_char * 32), ("compute_units", C.c_int32), ("wavefront", C.c_int32),
                 ("hbm_bytes", C.c_int64)]
@@ -138,6 +152,14 @@ SIGNATURES = {
     "dcarl_rls_neighbour_stats_f64": (_i32, [_vp, _vp, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
     "dcarl_rls_gate_train": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),
     "dcarl_rls_decide": (_i32, [_vp, _vp, _vp, _i32, _i32, C.POINTER(CRlsParams), _vp, _vp]),
+    "dcarl_recurrence_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),
+    "dcarl_recurrence_states_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),
+    "dcarl_recurrence_forward": (_i32, [C.POINTER(CRecurrence), _vp, _vp, _vp, _vp, _vp]),
+    "dcarl_recurrence_backward": (_i32, [C.POINTER(CRecurrence), _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "dcarl_rows_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
+    "dcarl_rows_gather": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64, _f64, _vp, _vp]),
+    "dcarl_rows_gradient": (_i32, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _f64, _vp, _vp, _vp]),
+    "dcarl_adjust_scores": (_i32, [C.POINTER(CScores), _vp, _i64, _vp]),
 }
 
 _libs = {}                      # variant -> typed library ("" = the product library)

@@ -1,0 +1,79 @@
+"""What the sequence operators share (``episodes.gated_recurrence``, ``tables.lookup``, ``candidates.adjust``): storage types, the
+checks of ids and offsets, the device a call runs on."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from . import _lib
+
+TYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}          # DCARL_F64 ... of include/dcarl.h
+
+
+def type_code(name: str, t: torch.Tensor, allowed=TYPES) -> int:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
+    if t.dtype not in allowed:
+        raise TypeError(f"{name} is {t.dtype}: " + ", ".join(str(k).replace("torch.", "") for k in allowed) + " are supported")
+    return TYPES[t.dtype]
+
+
+def on_device(*named) -> torch.device:
+    """The one GPU that all of the (name, tensor or None) live on; raises where one lives elsewhere (there is no CPU path)."""
+    dev = None
+    for name, t in named:
+        if t is None:
+            continue
+        if t.device.type != "cuda":
+            raise _lib.DcarlError(f"{name} is on {t.device}: the operator has no CPU path")
+        if dev is not None and t.device != dev[1].device:
+            raise ValueError(f"{name} is on {t.device}, {dev[0]} on {dev[1].device}")
+        dev = dev or (name, t)
+    return dev[1].device
+
+
+@contextlib.contextmanager
+def running_on(device: torch.device):
+    """Everything inside — allocations, the current stream, the launches — on `device`, whatever the current device is."""
+    if torch.cuda.current_device() == device.index:
+        yield
+    else:
+        with torch.cuda.device(device):
+            yield
+
+
+def rows_of(t: torch.Tensor):
+    """(tensor, elements between its rows) of a 2-D operand whose channels are contiguous; a copy where they are not.  Rows may lie
+    anywhere at a non-negative distance (slices, one row expanded to many)."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < 0:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def capturing() -> bool:
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+
+
+def whole_numbers(name: str, t) -> torch.Tensor:
+    t = torch.as_tensor(t)
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
+    return t
+
+
+def offsets(name: str, off, n: int, segments, validate: bool) -> torch.Tensor:
+    """The offsets of ragged segments over `n` entries as a contiguous int64 tensor, checked: they rise from 0 to at most `n`.  Offsets on the
+    GPU are checked through a copy to the host that waits for them; ``validate=False`` leaves that out, and is what a captured call needs."""
+    off = whole_numbers(name, off)
+    if off.dim() != 1 or off.numel() < 1:
+        raise ValueError(f"{name} must be one-dimensional with an entry more than there are segments")
+    if segments is not None and off.numel() != segments + 1:
+        raise ValueError(f"{name} has {off.numel()} entries for {segments} segments: {segments + 1} are needed")
+    if validate:
+        if off.device.type == "cuda" and capturing():
+            raise ValueError(f"{name} cannot be checked while a graph is captured: pass validate=False")
+        host = off.cpu().to(torch.int64)
+        if int(host[0]) != 0 or int(host[-1]) > n or bool((host[1:] < host[:-1]).any()):
+            raise ValueError(f"{name} must rise from 0 to at most {n}")
+    return off.to(torch.int64).contiguous()

@@ -1,0 +1,100 @@
+"""Candidate scores before the arg-max: penalties for what was taken already, biases, masks.
+
+``frenet.select`` and the gates of ``rls`` decide between a few trajectories; here a policy's scores over any number of candidates are adjusted
+by each observation's own history, by biases, and by which candidates are allowed (``frenet``'s feasibility bits, a grammar's next symbols)."""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib, _sequence as _seq
+
+SCORE_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def pack_allowed(allowed):
+    """(..., V) truth values -> (..., ceil(V/32)) int32 words as ``adjust`` wants them: candidate v in bit v % 32 of word v // 32."""
+    allowed = torch.as_tensor(allowed).to(torch.bool)
+    V = allowed.shape[-1]
+    bits = torch.nn.functional.pad(allowed, (0, -V % 32)).unflatten(-1, (-1, 32)).to(torch.int64) if V else allowed.new_zeros((*allowed.shape[:-1], 0, 32), dtype=torch.int64)
+    words = (bits << torch.arange(32, device=allowed.device)).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
+def _strength(name, v, B):
+    """A number, or a float32 tensor with one per row."""
+    if isinstance(v, torch.Tensor):
+        if v.dtype != torch.float32 or tuple(v.shape) != (B,):
+            raise ValueError(f"{name} must be a number or a float32 tensor ({B},), not {v.dtype} {tuple(v.shape)}")
+        return v.contiguous(), 0.0
+    v = float(v)
+    if v != v or (name == "repetition" and not v > 0.0):
+        raise ValueError(f"{name} = {v}" + (" is not positive" if name == "repetition" else ""))
+    return None, v
+
+
+def _per_row(name, t, B, width, dtype):
+    if t is None:
+        return None, 0
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError(f"{name} must be a {dtype} tensor")
+    if tuple(t.shape) == (width,):
+        return t.contiguous(), 0
+    if tuple(t.shape) != (B, width):
+        raise ValueError(f"{name} {tuple(t.shape)} is neither ({width},) nor ({B}, {width})")
+    return _seq.rows_of(t)
+
+
+def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, out=None,
+           validate: bool = False):
+    """For each of B rows of V scores:  z = score;  taken before: z = z / r if z > 0 else z * r;  z -= f * n + p where n > 0;
+    z += bias;  z = -inf where not allowed, whatever it was.  -> (B, V) of the scores' type, computed in f32, rounded once.
+
+    scores: (B, V) float32, bfloat16 or float16, rows at any distance.  taken: the rows' histories one after the other (int32 or int64 ids;
+    ids outside [0, V), such as -1, count nowhere), row b's is ``taken[taken_off[b]:taken_off[b+1]]``.  given: (B,) int32, how many
+    entries at a history's front were handed to the policy and not chosen by it: ``n`` counts the others, "taken before" looks at all.
+    repetition (> 0), frequency, presence: r, f, p, a number or a float32 tensor (B,).  bias: float32 (V,) or (B, V).
+    allowed: int32 words of ``pack_allowed``, (ceil(V/32),) or (B, ceil(V/32)); a row that allows nothing is -inf throughout.
+    out: where the result goes; ``out=scores`` adjusts in place.  validate: check taken_off's values (waits for them when they are on
+    the GPU); without it, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one are refused."""
+    if not isinstance(scores, torch.Tensor) or scores.dtype not in SCORE_TYPES:
+        raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
+    if scores.dim() != 2:
+        raise ValueError(f"scores must be (B, V), not {tuple(scores.shape)}")
+    if torch.is_grad_enabled() and scores.requires_grad:
+        raise ValueError("adjust has no gradient: detach the scores")
+    B, V = scores.shape
+    if (taken is None) != (taken_off is None):
+        raise ValueError("taken and taken_off come together")
+    off = None
+    if taken is not None:
+        taken = _seq.whole_numbers("taken", taken)
+        if taken.dim() != 1:
+            raise ValueError("taken must be one-dimensional")
+        taken = taken.contiguous()
+        off = _seq.offsets("taken_off", taken_off, taken.numel(), B, validate)
+    if given is not None and (not isinstance(given, torch.Tensor) or given.dtype != torch.int32 or tuple(given.shape) != (B,)):
+        raise ValueError(f"given must be an int32 tensor ({B},)")
+    (rep, rep0), (freq, freq0), (pres, pres0) = (_strength(n, v, B) for n, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)))
+    bias, ld_bias = _per_row("bias", bias, B, V, torch.float32)
+    allowed, ld_allowed = _per_row("allowed", allowed, B, (V + 31) // 32, torch.int32)
+    if out is not None:
+        if not isinstance(out, torch.Tensor) or out.dtype != scores.dtype or out.shape != scores.shape:
+            raise ValueError(f"out must be a {scores.dtype} tensor {tuple(scores.shape)}")
+        if V > 1 and out.stride(1) != 1 or B > 1 and out.stride(0) < V:
+            raise ValueError("out must have contiguous rows that do not overlap")
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError("out requires a gradient")
+    dev = _seq.on_device(("scores", scores), ("taken", taken), ("taken_off", off), ("given", given), ("repetition", rep), ("frequency", freq),
+                         ("presence", pres), ("bias", bias), ("allowed", allowed), ("out", out))
+    with _seq.running_on(dev):
+        s, ld = _seq.rows_of(scores)
+        z = torch.empty(B, V, dtype=s.dtype, device=dev) if out is None else out
+        given = None if given is None else given.contiguous()
+        at = lambda t: 0 if t is None else t.data_ptr()      # noqa: E731
+        a = _lib.CScores(at(s), B, V, ld, at(taken), at(off), 0 if taken is None else taken.numel(), at(given), at(rep), at(freq), at(pres), at(bias),
+                         ld_bias, at(allowed), ld_allowed, rep0 if rep is None else 1.0, freq0, pres0, _seq.TYPES[s.dtype],
+                         4 if taken is None else taken.element_size(), 0)
+        _lib.check(_lib.load().dcarl_adjust_scores(C.byref(a), _lib.ptr(z), z.stride(0), _lib.stream_ptr()), "dcarl_adjust_scores")
+    return z

@@ -88,6 +88,14 @@ int launch_true_step(const uint8_t*, const int64_t*, const int32_t*, const int32
 int launch_census_table(const double*, int, int, const DevParams&, unsigned long long*, hipStream_t);
 template <typename T>
 int launch_census_trace(const T*, const uint8_t*, const int64_t*, const int32_t*, int, int, const DevParams&, unsigned long long*, hipStream_t);
+int64_t recurrence_workspace_bytes(int64_t, int64_t, int64_t, int, int);
+int64_t recurrence_states_bytes(int64_t, int64_t, int64_t, int, int);
+void launch_recurrence_forward(const dcarl_recurrence_t&, void*, void*, void*, void*, hipStream_t);
+void launch_recurrence_backward(const dcarl_recurrence_t&, const void*, void*, const void*, int64_t, const void*, void*, void*, void*, hipStream_t);
+int64_t rows_workspace_bytes(int64_t, int64_t, int64_t);
+void launch_rows_gather(int, const void*, int64_t, int64_t, const void*, int, int64_t, int64_t, double, void*, hipStream_t);
+void launch_rows_gradient(int, const void*, int64_t, const void*, int, int64_t, int64_t, int64_t, double, void*, void*, hipStream_t);
+void launch_scores(const dcarl_scores_t&, void*, int64_t, hipStream_t);
 }  // namespace dcarl
 
 namespace {
@@ -1035,6 +1043,118 @@ int32_t dcarl_index_states_f64(const double* obs, int64_t N, int32_t D, const do
     if (!aligned16(workspace) || !aligned16(obs) || !aligned16(cells)) return fail(DCARL_EINVAL, "dcarl_index_states: obs, cells and workspace need 16-byte alignment");
     dcarl::launch_index_states(obs, N, D, cell_width, max_states, workspace, cells, ids, out, static_cast<hipStream_t>(stream));
     return after_launch("dcarl_index_states");
+}
+
+// ---- sequence operators ------------------------------------------------------------------------------------------------
+constexpr int64_t SEQ_MAX = (int64_t)1 << 31;          // steps, channels, episodes, rows, ids of one call
+constexpr int64_t SEQ_MAX_ELEMENTS = (int64_t)1 << 46; // of one operand: byte offsets stay far inside 63 bits
+
+static int check_seq(const char* who, int32_t type, int64_t n, int64_t d, int64_t e) {
+    if (type < DCARL_F64 || type > DCARL_F16) return fail(DCARL_EINVAL, "%s: type=%d is none of DCARL_F64/F32/BF16/F16", who, type);
+    if (n < 0 || d < 0 || e < 0 || n >= SEQ_MAX - 1 || d >= SEQ_MAX - 1 || e >= SEQ_MAX - 1 || (d && n > SEQ_MAX_ELEMENTS / d) || (d && e > SEQ_MAX_ELEMENTS / d))
+        return fail(DCARL_EINVAL, "%s: sizes %lld, %lld, %lld out of range", who, (long long)n, (long long)d, (long long)e);
+    return DCARL_OK;
+}
+static int check_ld(const char* who, const char* name, int64_t ld) {
+    if (ld < 0 || ld > SEQ_MAX_ELEMENTS) return fail(DCARL_EINVAL, "%s: %s=%lld out of range", who, name, (long long)ld);
+    return DCARL_OK;
+}
+static int check_recurrence(const char* who, const dcarl_recurrence_t* r) {
+    if (!r) return fail(DCARL_EINVAL, "%s: arguments are NULL", who);
+    if (int rc = check_seq(who, r->type, r->N, r->D, r->E)) return rc;
+    if (r->gate_kind < 0 || r->gate_kind > 2) return fail(DCARL_EINVAL, "%s: gate_kind=%d outside [0,2]", who, r->gate_kind);
+    if (int rc = check_ld(who, "ldx", r->ldx)) return rc;
+    if (int rc = check_ld(who, "ldg", r->ldg)) return rc;
+    if (int rc = check_ld(who, "ldh0", r->ldh0)) return rc;
+    if (r->E && !r->ep_off) return fail(DCARL_EINVAL, "%s: ep_off is NULL", who);
+    if (r->N && r->D && (!r->x || (r->gate_kind && !r->gate))) return fail(DCARL_EINVAL, "%s: x / gate is NULL", who);
+    return DCARL_OK;
+}
+
+int64_t dcarl_recurrence_workspace_bytes(int64_t N, int64_t D, int64_t E, int32_t type, int32_t gate_kind) {
+    if (check_seq("dcarl_recurrence_workspace_bytes", type, N, D, E) || gate_kind < 0 || gate_kind > 2) return 0;
+    return dcarl::recurrence_workspace_bytes(N, D, E, type, gate_kind);
+}
+int64_t dcarl_recurrence_states_bytes(int64_t N, int64_t D, int64_t E, int32_t type, int32_t gate_kind) {
+    if (check_seq("dcarl_recurrence_states_bytes", type, N, D, E) || gate_kind < 0 || gate_kind > 2) return 0;
+    return dcarl::recurrence_states_bytes(N, D, E, type, gate_kind);
+}
+
+int32_t dcarl_recurrence_forward(const dcarl_recurrence_t* r, void* states, void* workspace, void* h, void* last, void* stream) {
+    const char* who = "dcarl_recurrence_forward";
+    if (int rc = check_recurrence(who, r)) return rc;
+    if (r->D == 0 || (r->N == 0 && r->E == 0)) return DCARL_OK;
+    if (r->N && !h) return fail(DCARL_EINVAL, "%s: h is NULL", who);
+    if (!workspace && dcarl::recurrence_workspace_bytes(r->N, r->D, r->E, r->type, r->gate_kind)) return fail(DCARL_EINVAL, "%s: workspace is NULL", who);
+    if (!aligned16(workspace) || !aligned16(states)) return fail(DCARL_EINVAL, "%s: workspace and states need 16-byte alignment", who);
+    dcarl::launch_recurrence_forward(*r, states, workspace, h, last, static_cast<hipStream_t>(stream));
+    return after_launch(who);
+}
+
+int32_t dcarl_recurrence_backward(const dcarl_recurrence_t* r, const void* states, void* workspace, const void* dh, int64_t lddh, const void* dlast,
+                                  void* dx, void* dgate, void* dh0, void* stream) {
+    const char* who = "dcarl_recurrence_backward";
+    if (int rc = check_recurrence(who, r)) return rc;
+    if (int rc = check_ld(who, "lddh", lddh)) return rc;
+    if (dgate && r->gate_kind == 0) return fail(DCARL_EINVAL, "%s: a gate that is a number has no gradient", who);
+    if (r->D == 0 || (r->N == 0 && r->E == 0)) return DCARL_OK;
+    if (r->N && (!dh || !states)) return fail(DCARL_EINVAL, "%s: dh / states is NULL", who);
+    if (!workspace && dcarl::recurrence_workspace_bytes(r->N, r->D, r->E, r->type, r->gate_kind)) return fail(DCARL_EINVAL, "%s: workspace is NULL", who);
+    if (!aligned16(workspace) || !aligned16(states)) return fail(DCARL_EINVAL, "%s: workspace and states need 16-byte alignment", who);
+    dcarl::launch_recurrence_backward(*r, states, workspace, dh, lddh, dlast, dx, dgate, dh0, static_cast<hipStream_t>(stream));
+    return after_launch(who);
+}
+
+int64_t dcarl_rows_workspace_bytes(int64_t N, int64_t S, int64_t D, int32_t type) {
+    if (check_seq("dcarl_rows_workspace_bytes", type, N, D, S)) return 0;
+    return dcarl::rows_workspace_bytes(N, S, D);
+}
+
+int32_t dcarl_rows_gather(const void* table, int32_t type, int64_t ld, int64_t S, const void* ids, int32_t id_bytes, int64_t N, int64_t D,
+                          double scale, void* out, void* stream) {
+    const char* who = "dcarl_rows_gather";
+    if (int rc = check_seq(who, type, N, D, S)) return rc;
+    if (int rc = check_ld(who, "ld", ld)) return rc;
+    if (id_bytes != 4 && id_bytes != 8) return fail(DCARL_EINVAL, "%s: id_bytes=%d is neither 4 nor 8", who, id_bytes);
+    if (N == 0 || D == 0) return DCARL_OK;
+    if ((S && !table) || !ids || !out) return fail(DCARL_EINVAL, "%s: NULL argument", who);
+    dcarl::launch_rows_gather(type, table, ld, S, ids, id_bytes, N, D, scale, out, static_cast<hipStream_t>(stream));
+    return after_launch(who);
+}
+
+int32_t dcarl_rows_gradient(const void* dout, int32_t type, int64_t ldd, const void* ids, int32_t id_bytes, int64_t N, int64_t D, int64_t S,
+                            double scale, void* workspace, void* grad, void* stream) {
+    const char* who = "dcarl_rows_gradient";
+    if (int rc = check_seq(who, type, N, D, S)) return rc;
+    if (int rc = check_ld(who, "ldd", ldd)) return rc;
+    if (id_bytes != 4 && id_bytes != 8) return fail(DCARL_EINVAL, "%s: id_bytes=%d is neither 4 nor 8", who, id_bytes);
+    if (S == 0 || D == 0) return DCARL_OK;
+    if ((N && (!dout || !ids)) || !workspace || !grad) return fail(DCARL_EINVAL, "%s: NULL argument", who);
+    if (!aligned16(workspace)) return fail(DCARL_EINVAL, "%s: workspace needs 16-byte alignment", who);
+    dcarl::launch_rows_gradient(type, dout, ldd, ids, id_bytes, N, D, S, scale, workspace, grad, static_cast<hipStream_t>(stream));
+    return after_launch(who);
+}
+
+int32_t dcarl_adjust_scores(const dcarl_scores_t* s, void* out, int64_t ld_out, void* stream) {
+    const char* who = "dcarl_adjust_scores";
+    if (!s) return fail(DCARL_EINVAL, "%s: arguments are NULL", who);
+    if (int rc = check_seq(who, s->type, s->B, s->V, s->n_taken)) return rc;
+    if (s->type == DCARL_F64) return fail(DCARL_EINVAL, "%s: scores are DCARL_F32, DCARL_BF16 or DCARL_F16", who);
+    if (int rc = check_ld(who, "ld_scores", s->ld_scores)) return rc;
+    if (int rc = check_ld(who, "ld_out", ld_out)) return rc;
+    if (int rc = check_ld(who, "ld_bias", s->ld_bias)) return rc;
+    if (int rc = check_ld(who, "ld_allowed", s->ld_allowed)) return rc;
+    if (s->B == 0 || s->V == 0) return DCARL_OK;
+    if (!s->scores || !out) return fail(DCARL_EINVAL, "%s: scores / out is NULL", who);
+    if (s->B > 1 && ld_out < s->V) return fail(DCARL_EINVAL, "%s: the rows of out overlap (ld_out=%lld, V=%lld)", who, (long long)ld_out, (long long)s->V);
+    if (out == s->scores && s->B > 1 && ld_out != s->ld_scores) return fail(DCARL_EINVAL, "%s: in place needs equal strides", who);
+    if (s->taken_off && s->n_taken && !s->taken) return fail(DCARL_EINVAL, "%s: taken is NULL", who);
+    if (s->taken_off && s->id_bytes != 4 && s->id_bytes != 8) return fail(DCARL_EINVAL, "%s: id_bytes=%d is neither 4 nor 8", who, s->id_bytes);
+    uint32_t rep;                                          // > 0 and no NaN, by its bits: this unit is compiled without NaNs
+    memcpy(&rep, &s->repetition_value, sizeof(rep));
+    if (!s->repetition && (rep == 0 || rep > 0x7f800000u)) return fail(DCARL_EINVAL, "%s: repetition=%g not positive", who, (double)s->repetition_value);
+    dcarl::launch_scores(*s, out, ld_out, static_cast<hipStream_t>(stream));
+    return after_launch(who);
 }
 
 }  // extern "C"

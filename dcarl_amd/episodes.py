@@ -5,7 +5,9 @@
   plus the AveSpeed the collector logs.
 * ``nstep_backup`` — the field vehicle's ``RLS.add_data`` value stream (stable_baselines/deepq/RLS.py:185-215): a 10-deep
   trajectory buffer; a transition leaves it with its own reward, the last ten of a finished episode get the terminal
-  reward times ``gamma**k``."""
+  reward times ``gamma**k``.
+* ``gated_recurrence`` — a state carried along every episode, h[t] = gate[t] * h[t-1] + x[t], with its gradients; and
+  ``discounted_returns``, the returns of a discount, which are that recurrence reversed (neither has a counterpart in the reference)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -13,7 +15,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, _sequence as _seq
 
 COLLISION, PASSED, STUCK = 1, 2, 4          # flag bits of a step (TS:406, 413, 418)
 
@@ -68,3 +70,129 @@ def nstep_backup(rew, ep_off, ep_done, gamma: float = 0.95, horizon: int = 10):
                                           int(horizon), _lib.ptr(value), _lib.ptr(rec), _lib.stream_ptr()),
                "dcarl_nstep_backup_f64")
     return value, rec.bool()
+
+
+# ---- the recurrence along episodes --------------------------------------------------------------------------------------------
+def _recurrence_args(x, gate, ep_off, h0, gate_value, reverse):
+    kind = 0 if gate is None else 2 if gate.dim() == 2 else 1
+    x, ldx = _seq.rows_of(x)
+    ldg = 0
+    if kind == 2:
+        gate, ldg = _seq.rows_of(gate)
+    elif kind == 1:
+        gate, ldg = (gate, gate.stride(0)) if gate.stride(0) >= 0 else (gate.contiguous(), 1)
+    ldh0 = 0
+    if h0 is not None:
+        h0, ldh0 = _seq.rows_of(h0)
+    N, D = x.shape
+    a = _lib.CRecurrence(N, D, ep_off.numel() - 1, ep_off.data_ptr(), x.data_ptr(), ldx, 0 if gate is None else gate.data_ptr(), ldg,
+                         0 if h0 is None else h0.data_ptr(), ldh0, gate_value, kind, int(reverse), _seq.TYPES[x.dtype], 0)
+    return a, (x, gate, h0)                                   # the tensors: alive until the launch
+
+
+def _bytes(n, dev):
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+
+
+def _recurrence_forward(x, gate, ep_off, h0, gate_value, reverse, want_last, want_states):
+    lib, dev = _lib.load(), x.device
+    with _seq.running_on(dev):
+        a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
+        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        last = torch.empty(a.E, a.D, dtype=x.dtype, device=dev) if want_last else None
+        sizes = (a.N, a.D, a.E, a.type, a.gate_kind)
+        states = _bytes(lib.dcarl_recurrence_states_bytes(*sizes), dev) if want_states else None
+        ws = _bytes(lib.dcarl_recurrence_workspace_bytes(*sizes), dev)
+        _lib.check(lib.dcarl_recurrence_forward(C.byref(a), _lib.ptr(states), _lib.ptr(ws), _lib.ptr(h), _lib.ptr(last), _lib.stream_ptr()),
+                   "dcarl_recurrence_forward")
+    return h, last, states
+
+
+def _recurrence_backward(x, gate, ep_off, h0, gate_value, reverse, states, dh, dlast, want):
+    lib, dev = _lib.load(), x.device
+    with _seq.running_on(dev):
+        a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
+        dh, lddh = _seq.rows_of(dh)
+        dlast = None if dlast is None else dlast.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+        dgate = torch.empty(gate.shape, dtype=x.dtype, device=dev) if want[1] else None
+        dh0 = torch.empty(h0.shape, dtype=x.dtype, device=dev) if want[2] else None
+        ws = _bytes(lib.dcarl_recurrence_workspace_bytes(a.N, a.D, a.E, a.type, a.gate_kind), dev)
+        _lib.check(lib.dcarl_recurrence_backward(C.byref(a), _lib.ptr(states), _lib.ptr(ws), _lib.ptr(dh), lddh, _lib.ptr(dlast), _lib.ptr(dx),
+                                                 _lib.ptr(dgate), _lib.ptr(dh0), _lib.stream_ptr()), "dcarl_recurrence_backward")
+    return dx, dgate, dh0
+
+
+class _Recurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, h0, ep_off, gate_value, reverse, want_last):
+        h, last, states = _recurrence_forward(x, gate, ep_off, h0, gate_value, reverse, want_last, any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, gate, h0, ep_off, states)
+        ctx.rest = gate_value, reverse
+        return (h, last) if want_last else h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast=None):
+        x, gate, h0, ep_off, states = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dgate, dh0 = _recurrence_backward(x, gate, ep_off, h0, *ctx.rest, states, dh, dlast, need[:3])
+        return dx, dgate, dh0, None, None, None, None
+
+
+def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_last: bool = False, validate: bool = True):
+    """``h[t] = gate[t] * h[t-1] + x[t]`` per channel along each episode, with gradients for ``x``, ``gate`` and ``h0``.
+
+    x: (N, D) steps, or (N,) for one channel; float64, float32, bfloat16 or float16 (sums in f32; f64 for float64; each result rounded once).
+    gate: (N, D) like x, (N,) shared by the channels of a step, or a number.  ep_off: (E+1,) int offsets of the episodes as in
+    ``episode_returns``; steps behind ``ep_off[E]`` belong to none: they are not read, the results are zero there.
+    h0: (E, D) (or (E,)) states before the first steps; one step of E live episodes is N == E with every length 1.
+    reverse: mirrored, ``h[t] = gate[t] * h[t+1] + x[t]`` from the end of each episode.
+    want_last: also the (E, D) states that the episodes end with (``h0`` or zero for an empty one).
+    validate: check ep_off's values; where it lies on the GPU this waits for it.  ``validate=False`` never waits and is what a captured call
+    needs; offsets that do not rise from 0 to at most N then give unspecified results (and no access out of range).
+
+    Everything runs on the tensors' device and its current stream; nothing is kept between calls.  A backward pass that is to be captured
+    into a graph goes through ``torch.autograd.grad`` of a forward pass captured with it, with no other graph of the same leaves alive."""
+    code = _seq.type_code("x", x)
+    flat = x.dim() == 1
+    if x.dim() not in (1, 2):
+        raise ValueError(f"x must be (N, D) or (N,), not {tuple(x.shape)}")
+    N = x.shape[0]
+    value = 0.0
+    if isinstance(gate, torch.Tensor):
+        if gate.dtype != x.dtype:
+            raise TypeError(f"gate is {gate.dtype}, x {x.dtype}")
+        if tuple(gate.shape) not in (tuple(x.shape), (N,)):
+            raise ValueError(f"gate {tuple(gate.shape)} fits neither x {tuple(x.shape)} nor its {N} steps")
+    else:
+        value, gate = float(gate), None
+    E = None
+    if h0 is not None:
+        if _seq.type_code("h0", h0) != code:
+            raise TypeError(f"h0 is {h0.dtype}, x {x.dtype}")
+        if h0.dim() != x.dim() or h0.shape[1:] != x.shape[1:]:
+            raise ValueError(f"h0 {tuple(h0.shape)} does not hold a state like x {tuple(x.shape)} for every episode")
+        E = h0.shape[0]
+    off = _seq.offsets("ep_off", ep_off, N, E, validate)
+    dev = _seq.on_device(("x", x), ("gate", gate), ("h0", h0), ("ep_off", off if off.device.type == "cuda" else None))
+    if off.device != dev:
+        if _seq.capturing():
+            raise ValueError("ep_off must lie on the GPU while a graph is captured")
+        off = off.to(dev)
+    if flat:
+        x, h0 = x.unsqueeze(1), None if h0 is None else h0.unsqueeze(1)
+    if gate is not None and gate.dim() == 1 and x.shape[1] == 1:
+        gate = gate.unsqueeze(1)                              # one channel: shared or not is the same
+    out = _Recurrence.apply(x, gate, h0, off, value, bool(reverse), bool(want_last))
+    if flat:
+        out = tuple(o.squeeze(1) for o in out) if want_last else out.squeeze(1)
+    return out
+
+
+def discounted_returns(rew, ep_off, gamma: float = 0.95, *, validate: bool = True):
+    """``R[t] = rew[t] + gamma * R[t+1]`` to the end of each episode: the cumulative-reward column for a discount, where ``nstep_backup``
+    has the field recorder's ten-step rule.  rew: (N,) tensor on the GPU; float64 sums for float64 rewards."""
+    if not isinstance(rew, torch.Tensor):
+        rew = _dev64(rew, _lib.require_gpu())
+    return gated_recurrence(rew, float(gamma), ep_off, reverse=True, validate=validate)

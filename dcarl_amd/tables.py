@@ -1,0 +1,93 @@
+"""Rows of a table by dense state id, with the gradient of the table by sorted ids.
+
+A table has one row of D values per state (``state_ids`` / ``index_states`` hand out the ids, the samplers -1 for a visit they drop);
+``lookup`` reads the rows of a batch of ids, its gradient adds a batch's rows up per id, always in the same order."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib, _sequence as _seq
+
+
+def _check_ids(ids, n_rows: int, validate: bool):
+    ids = _seq.whole_numbers("ids", ids)
+    if validate and ids.numel():
+        if ids.device.type == "cuda" and _seq.capturing():
+            raise ValueError("ids cannot be checked while a graph is captured: pass validate=False")
+        lo, hi = (int(v) for v in torch.aminmax(ids))
+        if lo < -1 or hi >= n_rows:
+            raise IndexError(f"ids out of range: [{lo},{hi}] vs {n_rows} rows (-1 = no row)")
+    return ids.contiguous()
+
+
+def _gather(table, ids, scale):
+    lib = _lib.load()
+    with _seq.running_on(table.device):
+        t, ld = _seq.rows_of(table)
+        D = t.shape[1]
+        out = torch.empty(*ids.shape, D, dtype=t.dtype, device=t.device)
+        _lib.check(lib.dcarl_rows_gather(_lib.ptr(t), _seq.TYPES[t.dtype], ld, t.shape[0], _lib.ptr(ids), ids.element_size(), ids.numel(), D,
+                                         scale, _lib.ptr(out), _lib.stream_ptr()), "dcarl_rows_gather")
+    return out
+
+
+def _gradient(dout, ids, n_rows, scale):
+    lib = _lib.load()
+    with _seq.running_on(dout.device):
+        N, D = ids.numel(), dout.shape[-1]
+        d, ldd = _seq.rows_of(dout.reshape(N, D))
+        code = _seq.TYPES[d.dtype]
+        grad = torch.empty(n_rows, D, dtype=d.dtype, device=d.device)
+        ws = torch.empty(max(lib.dcarl_rows_workspace_bytes(N, n_rows, D, code), 16), dtype=torch.uint8, device=d.device)
+        _lib.check(lib.dcarl_rows_gradient(_lib.ptr(d), code, ldd, _lib.ptr(ids), ids.element_size(), N, D, n_rows, scale, _lib.ptr(ws),
+                                           _lib.ptr(grad), _lib.stream_ptr()), "dcarl_rows_gradient")
+    return grad
+
+
+class _Lookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale):
+        ctx.save_for_backward(ids)
+        ctx.rest = table.shape[0], scale
+        return _gather(table, ids, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        return _gradient(dout, ctx.saved_tensors[0], *ctx.rest), None, None
+
+
+def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
+    """``scale * table[ids]``, zeros where an id is -1; ids of any shape, the result has a dimension D behind it.
+
+    table: (S, D) float64, float32, bfloat16 or float16 on the GPU, rows at any distance; ids: int32 or int64.
+    The gradient of the table is dense, of the table's type: per id the sum over the batch in ascending order, held in f32 (f64), scaled and
+    rounded once; rows no id names are zero.  validate: raise IndexError for ids outside [-1, S), which waits for them; with
+    ``validate=False`` nothing waits (a captured call needs it) and such ids count as -1."""
+    _seq.type_code("table", table)
+    if table.dim() != 2:
+        raise ValueError(f"table must be (S, D), not {tuple(table.shape)}")
+    ids = _check_ids(ids, table.shape[0], validate)
+    dev = _seq.on_device(("table", table), ("ids", ids if ids.device.type == "cuda" else None))
+    if ids.device != dev:
+        if _seq.capturing():
+            raise ValueError("ids must lie on the GPU while a graph is captured")
+        ids = ids.to(dev)
+    return _Lookup.apply(table, ids, float(scale))
+
+
+def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: bool = True):
+    """The gradient of ``lookup``'s table by itself: (n_rows, D) with row s = scale * the sum of ``dout`` (ids' shape, D) over ids == s."""
+    _seq.type_code("dout", dout)
+    n_rows = int(n_rows)
+    if n_rows < 0:
+        raise ValueError(f"n_rows = {n_rows} is negative")
+    ids = _check_ids(ids, n_rows, validate)
+    if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"dout {tuple(dout.shape)} has no row for each of the ids {tuple(ids.shape)}")
+    dev = _seq.on_device(("dout", dout), ("ids", ids if ids.device.type == "cuda" else None))
+    if ids.device != dev:
+        if _seq.capturing():
+            raise ValueError("ids must lie on the GPU while a graph is captured")
+        ids = ids.to(dev)
+    return _gradient(dout, ids, n_rows, float(scale))

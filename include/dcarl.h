@@ -615,6 +615,77 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
                             const double* obstacles, int32_t n_obs, int64_t B, const dcarl_frenet_grid_t* grid /* [host] */,
                             const dcarl_frenet_limits_t* limits /* [host] */, int32_t* choice, uint8_t* ok, void* stream);
 
+/* ---- sequence operators: a recurrent policy over recorded episodes (no counterpart in the reference) -----------------------
+ * Storage types of these entry points.  Sums, states and products are held in f32 (f64 for DCARL_F64); a result is rounded once. */
+#define DCARL_F64 0
+#define DCARL_F32 1
+#define DCARL_BF16 2
+#define DCARL_F16 3
+/* Gated linear recurrence along ragged episodes, per channel d:   h[t] = g[t] * h[t-1] + x[t]
+ *   episode e = steps [ep_off[e], ep_off[e+1]) (device, ep_off[0] == 0, rising, ep_off[E] <= N), h before its first step = h0[e] or 0.
+ *   reverse != 0 mirrors time: h[t] = g[t] * h[t+1] + x[t], an episode starts at its last step (discounted returns: x = rewards,
+ *   g = gamma, D = 1).  x [N][D] with ldx elements between steps (channels contiguous; any alignment of the type);
+ *   gate_kind 0: g = gate_value; 1: gate [N], element stride ldg, shared by the channels; 2: gate [N][D], ldg elements between steps.
+ *   Steps behind the last episode are read by nothing; the outputs hold zeros there.
+ * dcarl_recurrence_forward: h [N][D] contiguous; last (nullable) [E][D] = the state each episode ends with, h0[e] (or 0) for an empty one;
+ *   states (nullable): dcarl_recurrence_states_bytes bytes the backward call wants (16-byte aligned).
+ * dcarl_recurrence_backward, from the same arguments, the forward call's states, dh [N][D] (lddh elements between steps) and dlast (nullable)
+ *   [E][D]:  d[t] = dh[t] + g[t+1] d[t+1] inside the episode;  dx = d;  dgate[t] = d[t] * h[t-1] (gate_kind 1: summed over the channels);
+ *   dh0[e] = g[s] d[s] (s: the first step; dlast[e] for an empty episode).  dx / dgate / dh0 nullable, contiguous; dgate must be NULL for
+ *   gate_kind 0.  No atomics: run-to-run identical.
+ * workspace: dcarl_recurrence_workspace_bytes bytes, 16-byte aligned, contents irrelevant before / after. */
+typedef struct dcarl_recurrence {
+    int64_t N, D, E;
+    const int64_t* ep_off;
+    const void* x;
+    int64_t ldx;
+    const void* gate;
+    int64_t ldg;
+    const void* h0;
+    int64_t ldh0;
+    double gate_value;
+    int32_t gate_kind, reverse, type, reserved;
+} dcarl_recurrence_t;
+int64_t dcarl_recurrence_workspace_bytes(int64_t N, int64_t D, int64_t E, int32_t type, int32_t gate_kind);
+int64_t dcarl_recurrence_states_bytes(int64_t N, int64_t D, int64_t E, int32_t type, int32_t gate_kind);
+int32_t dcarl_recurrence_forward(const dcarl_recurrence_t* r /* [host] */, void* states, void* workspace, void* h, void* last, void* stream);
+int32_t dcarl_recurrence_backward(const dcarl_recurrence_t* r /* [host] */, const void* states, void* workspace, const void* dh, int64_t lddh,
+                                  const void* dlast, void* dx, void* dgate, void* dh0, void* stream);
+/* Rows of a table by id (ids of id_bytes 4 or 8, device): out[n] = scale * table[ids[n]], [N][D] contiguous; zeros for an id outside [0, S)
+ *   (dcarl_sample_pairs hands out -1 for a visit it drops).  table [S][D], ld elements between rows.
+ * dcarl_rows_gradient: grad [S][D] contiguous, every row written: scale * the sum of dout[n] (ldd elements between rows) over ids[n] == s, in
+ *   a fixed order (the ids are sorted, stably; no atomics on values).  N, S < 2^31 - 1.
+ *   workspace: dcarl_rows_workspace_bytes bytes, 16-byte aligned. */
+int64_t dcarl_rows_workspace_bytes(int64_t N, int64_t S, int64_t D, int32_t type);
+int32_t dcarl_rows_gather(const void* table, int32_t type, int64_t ld, int64_t S, const void* ids, int32_t id_bytes, int64_t N, int64_t D,
+                          double scale, void* out, void* stream);
+int32_t dcarl_rows_gradient(const void* dout, int32_t type, int64_t ldd, const void* ids, int32_t id_bytes, int64_t N, int64_t D, int64_t S,
+                            double scale, void* workspace, void* grad, void* stream);
+/* Candidate scores adjusted by what was taken already, by biases and masks, for B rows of V candidates (no limit of DCARL_MAX_ACTIONS here):
+ *   z = scores[b][v];  where v is in the row's history: z = z > 0 ? z / r : z * r;  z -= f * n + p where n > 0;  z += bias;
+ *   z = -inf where v is not allowed (whatever z is, NaN included).  A row that allows nothing is -inf throughout.
+ *   history of row b: taken[taken_off[b] .. taken_off[b+1]) (ids of id_bytes 4 or 8; ids outside [0, V) count nowhere), its first given[b]
+ *   entries (given nullable = 0) were handed to the policy, the others are its own choices: n counts those, r looks at all.
+ *   r, f, p: [B] arrays, or where those are NULL the *_value.  bias (nullable): ld_bias elements between rows, 0 = one row for all.
+ *   allowed (nullable): bit v % 32 of word v / 32, ld_allowed words between rows, 0 = one row for all.
+ * dcarl_adjust_scores: out [B][V], ld_out elements between rows, of the scores' type; out == scores is allowed with equal strides. */
+typedef struct dcarl_scores {
+    const void* scores;
+    int64_t B, V, ld_scores;
+    const void* taken;
+    const int64_t* taken_off;
+    int64_t n_taken;
+    const int32_t* given;
+    const float *repetition, *frequency, *presence;
+    const float* bias;
+    int64_t ld_bias;
+    const uint32_t* allowed;
+    int64_t ld_allowed;
+    float repetition_value, frequency_value, presence_value;
+    int32_t type, id_bytes, reserved;
+} dcarl_scores_t;
+int32_t dcarl_adjust_scores(const dcarl_scores_t* s /* [host] */, void* out, int64_t ld_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
