@@ -8,7 +8,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["abi.hip", "trace.hip", "trace_final.hip", "diag.hip", "trace_nwave_f32.hip", "trace_nwave_f64.hip", "bounds.hip", "buckets.hip", "ingest.hip", "comm.hip", "episodes.hip", "sampler.hip", "misc.hip", "rls.hip", "frenet.hip", "recurrence.hip", "rows.hip", "scores.hip"]
+SOURCES = ["abi.hip", "trace.hip", "trace_final.hip", "diag.hip", "trace_nwave_f32.hip", "trace_nwave_f64.hip", "bounds.hip", "buckets.hip", "ingest.hip", "comm.hip", "episodes.hip", "sampler.hip", "misc.hip", "rls.hip", "frenet.hip", "recurrence.hip", "recurrence_back.hip", "rows.hip", "scores.hip"]
 LIB = os.path.join(HERE, "libdcarl_hip.so")
 # Variants of the one source tree.  "" = the product library (no environment knobs, no measurement-only kernel instances).
 # "ab" = -DDCARL_AB_BUILD: the launchers' choices can be overridden through DCARL_* environment variables and the two- / four-wave,
@@ -22,7 +22,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-u
 # 3.062 -> 3.033, 2.549 -> 2.523, 1.179 -> 1.171 ms (round 6, profiles/r06_ab_online_sched_strategy.txt); no instance spills with it.
 # The sequence operators take NaNs and infinities as ordinary inputs, and keep the packed f32 instructions out.
 _SEQ = ["-fhonor-nans", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCE_FLAGS = {"trace_nwave_f32.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"], "recurrence.hip": _SEQ, "rows.hip": _SEQ, "scores.hip": _SEQ}
+SOURCE_FLAGS = {"trace_nwave_f32.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"], "recurrence.hip": _SEQ, "recurrence_back.hip": _SEQ, "rows.hip": _SEQ, "scores.hip": _SEQ}
 
 
 def hipcc():

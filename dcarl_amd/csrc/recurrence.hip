@@ -1,140 +1,158 @@
-// Gated linear recurrence along ragged episodes: h_t = g_t * h_{t-1} + x_t per channel, restarted from h0[e] (or 0) where episode e
-// begins, and its gradients  d_t = dh_t + g_{t+1} d_{t+1},  dx = d,  dg_t = d_t h_{t-1},  dh0[e] = g_s d_s (s: the episode's first
-// step).  `reverse` mirrors time: the host passes the last row's address and negative row strides, and the kernels read the
-// offsets mirrored.
-#include "seq_common.h"
+// The recurrence along episodes: the walk's flags, the plan of a call, the launches of the forward pass (kernels: recurrence_impl.h).
+#include <type_traits>
+#include "recurrence_impl.h"
 
 namespace dcarl {
 
-struct RecArgs {
-    int64_t N, D, E;
-    const int64_t* ep_off;
-    const void *x, *gate, *h0;
-    int64_t ldx, ldg, ldh0;
-    double gate_value;
-    int gate_kind, reverse;
-};
-
-// rows [b, e) of episode `ep`, clamped into [0, N) whatever the offsets hold; in walking order for `reverse`
-__device__ __forceinline__ void rec_span(const RecArgs& a, int64_t ep, int64_t& b, int64_t& e) {
-    b = a.ep_off[ep]; e = a.ep_off[ep + 1];
-    b = b < 0 ? 0 : b > a.N ? a.N : b;
-    e = e < b ? b : e > a.N ? a.N : e;
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void rec_forward_kernel(RecArgs a, typename SeqType<T>::Acc* states, T* h, int64_t ldh, T* last) {
-    using Acc = typename SeqType<T>::Acc;
-    const int64_t d = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (d >= a.D) return;
-    for (int64_t ep = blockIdx.y; ep < a.E; ep += gridDim.y) {
-        int64_t b, e;
-        rec_span(a, ep, b, e);
-        Acc s = a.h0 ? widen(static_cast<const T*>(a.h0)[ep * a.ldh0 + d]) : Acc(0);
-        for (int64_t i = 0; i < e - b; ++i) {
-            const int64_t t = a.reverse ? e - 1 - i : b + i;
-            const Acc g = a.gate_kind == 0 ? (Acc)a.gate_value
-                          : widen(static_cast<const T*>(a.gate)[t * a.ldg + (a.gate_kind == 2 ? d : 0)]);
-            if (states) states[t * a.D + d] = s;            // the state BEFORE step t
-            s = g * s + widen(static_cast<const T*>(a.x)[t * a.ldx + d]);
-            h[t * ldh + d] = narrow<T>(s);
+// thread r < N: flags and episode of step r of the walk; threads N .. N + P: where part p begins
+__global__ __launch_bounds__(256) void rec_walk_kernel(const int64_t* off, int64_t E, int64_t N, int reverse, int P, int64_t R, uint8_t* flag,
+                                                       int32_t* ep, int64_t* part) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i > N + P) return;
+    const int64_t p = i - N;
+    if (p == 0 || p == P) { part[p] = p ? N : 0; return; }
+    const int64_t r = p > 0 ? p * R : i;
+    if (r >= N) { part[p] = N; return; }
+    const int64_t t = reverse ? N - 1 - r : r;
+    int64_t lo = 0, hi = E + 1;                            // the first offset above t
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (off[mid] <= t) lo = mid + 1; else hi = mid;
+    }
+    const bool out = lo == 0 || lo > E;
+    const int64_t e = out ? 0 : lo - 1;
+    if (p > 0) {
+        int64_t at = r;
+        if (!out) {                                        // the nearest start within a quarter of a part
+            const int64_t s0 = rec_ep_begin(off, e, reverse, N), s1 = rec_ep_end(off, e, reverse, N);
+            const int64_t b = r - s0, f = s1 - r;
+            if (b <= f && b <= R / 4) at = s0;
+            else if (f < b && f <= R / 4) at = s1;
         }
-        if (last) last[ep * a.D + d] = narrow<T>(s);
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(64) void rec_backward_kernel(RecArgs a, const typename SeqType<T>::Acc* states, const T* dh, int64_t lddh,
-                                                          const T* dlast, T* dx, T* dgate, T* dh0, typename SeqType<T>::Acc* terms) {
-    using Acc = typename SeqType<T>::Acc;
-    const int64_t d = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (d >= a.D) return;
-    for (int64_t ep = blockIdx.y; ep < a.E; ep += gridDim.y) {
-        int64_t b, e;
-        rec_span(a, ep, b, e);
-        Acc c = dlast ? widen(dlast[ep * a.D + d]) : Acc(0);
-        for (int64_t i = e - b - 1; i >= 0; --i) {
-            const int64_t t = a.reverse ? e - 1 - i : b + i;
-            const Acc g = a.gate_kind == 0 ? (Acc)a.gate_value
-                          : widen(static_cast<const T*>(a.gate)[t * a.ldg + (a.gate_kind == 2 ? d : 0)]);
-            const Acc dt = widen(dh[t * lddh + d]) + c;
-            if (dx) dx[t * a.D + d] = narrow<T>(dt);
-            const Acc term = dt * states[t * a.D + d];
-            if (terms) terms[t * a.D + d] = term;
-            else if (dgate) dgate[t * a.D + d] = narrow<T>(term);
-            c = g * dt;
+        part[p] = at;
+    } else {
+        int f = REC_OUT;
+        if (!out) {
+            const bool first = t == off[e], last = t == off[e + 1] - 1;
+            f = ((reverse ? last : first) ? REC_START : 0) | ((reverse ? first : last) ? REC_END : 0);
         }
-        if (dh0) dh0[ep * a.D + d] = narrow<T>(c);
+        flag[r] = (uint8_t)f;
+        ep[r] = (int32_t)e;
     }
 }
 
-// dgate[t] = sum over the channels of one step, for a gate that all channels share: one wavefront per step, a fixed butterfly
-template <typename T>
-__global__ __launch_bounds__(64) void rec_share_kernel(const typename SeqType<T>::Acc* terms, int64_t N, int64_t D, const int64_t* ep_off,
-                                                       int64_t E, T* dgate) {
-    using Acc = typename SeqType<T>::Acc;
-    const int64_t n = E > 0 ? ep_off[E] : 0;
-    for (int64_t t = blockIdx.x; t < N; t += gridDim.x) {
-        Acc s = 0;
-        if (t < n) for (int64_t d = threadIdx.x; d < D; d += 64) s += terms[t * D + d];
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-        if (threadIdx.x == 0) dgate[t] = narrow<T>(s);
-    }
+template <typename T> __global__ __launch_bounds__(256) void rec_share_kernel(const typename SeqType<T>::Acc* dgp, int blocks, int64_t N, int step, T* dg) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= N) return;
+    typename SeqType<T>::Acc s = 0;
+    for (int b = 0; b < blocks; ++b) s += dgp[b * N + r];
+    dg[r * step] = narrow<T>(s);
 }
 
-// rows behind the last episode: zeros in what the call makes
-template <typename T>
-__global__ __launch_bounds__(256) void rec_tail_kernel(const int64_t* ep_off, int64_t E, int64_t N, int64_t D, T* a, T* b, T* c) {
-    int64_t n = E > 0 ? ep_off[E] : 0;
-    n = n < 0 ? 0 : n;
-    const int64_t step = (int64_t)gridDim.x * 256;
-    for (int64_t i = n * D + (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * D; i += step) {
-        if (a) a[i] = narrow<T>(0.0f);
-        if (b) b[i] = narrow<T>(0.0f);
-        if (c) c[i] = narrow<T>(0.0f);
-    }
-}
+static int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 
-static RecArgs rec_args(const dcarl_recurrence_t& r) {
-    return RecArgs{r.N, r.D, r.E, r.ep_off, r.x, r.gate, r.h0, r.ldx, r.ldg, r.ldh0, r.gate_value, r.gate_kind, r.reverse};
-}
-
-int64_t recurrence_workspace_bytes(int64_t N, int64_t D, int64_t, int type, int gate_kind) {
-    return gate_kind == 1 ? N * D * (type == DCARL_F64 ? 8 : 4) : 0;
-}
-int64_t recurrence_states_bytes(int64_t N, int64_t D, int64_t, int type, int) { return N * D * (type == DCARL_F64 ? 8 : 4); }
-
-static dim3 rec_grid(const dcarl_recurrence_t& r) {
-    return dim3((unsigned)((r.D + 63) / 64), (unsigned)(r.E < 65535 ? r.E : 65535));
-}
-
-void launch_recurrence_forward(const dcarl_recurrence_t& r, void* states, void*, void* h, void* last, hipStream_t st) {
-    with_type(r.type, [&](auto t) {
+RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
+    RecPlan p{};
+    const int64_t acc = type == DCARL_F64 ? 8 : 4;
+    with_type(type, [&](auto t) {
         using T = decltype(t);
-        using Acc = typename SeqType<T>::Acc;
-        if (r.N > 0)
-            hipLaunchKernelGGL((rec_tail_kernel<T>), dim3(256), dim3(256), 0, st, r.ep_off, r.E, r.N, r.D, (T*)h, (T*)nullptr, (T*)nullptr);
-        if (r.E > 0)
-            hipLaunchKernelGGL((rec_forward_kernel<T>), rec_grid(r), dim3(64), 0, st, rec_args(r), (Acc*)states, (T*)h, r.D, (T*)last);
+        rec_with_shape<T>(D, [&](auto C, auto V) {
+            p.tile = REC_TILE<C(), T>;
+            p.blocks = (int)((D + C() * V() - 1) / (C() * V()));
+        });
+    });
+    // as many parts as give every CU a few workgroups, none under two tiles
+    int64_t want = (1024 + p.blocks - 1) / p.blocks, most = N / (2 * p.tile);
+    want = want < most ? want : most;
+    p.P = (int)(want < 1 ? 1 : want > REC_MAX_PARTS ? REC_MAX_PARTS : want);
+    p.slots = N / p.tile + p.P + 1;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t here = at; at += up16(bytes); return here; };
+    p.flag = take(N + 8); p.ep = take(4 * N); p.part = take(8 * (p.P + 1));
+    p.plan_bytes = at;
+    p.state = take(p.slots * D * acc);
+    p.states_bytes = at;
+    at = 0;
+    p.ws_plan = take(p.plan_bytes);
+    p.agg = take(p.P > 1 ? 2 * p.P * D * acc : 0);
+    p.dgp = take(gate_kind == 1 && p.blocks > 1 ? p.blocks * N * acc : 0);
+    p.ws_bytes = at;
+    return p;
+}
+int64_t recurrence_workspace_bytes(int64_t N, int64_t D, int64_t, int type, int gate_kind) { return D ? rec_plan(N, D, type, gate_kind).ws_bytes : 0; }
+int64_t recurrence_states_bytes(int64_t N, int64_t D, int64_t, int type, int gate_kind) { return D ? rec_plan(N, D, type, gate_kind).states_bytes : 0; }
+
+template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, const RecPlan& p, char* plan, char* ws) {
+    using Acc = typename SeqType<T>::Acc;
+    RecWalk<T> a{};
+    a.N = r.N; a.D = r.D; a.E = r.E; a.ep_off = r.ep_off; a.reverse = r.reverse; a.P = p.P;
+    const int64_t top = r.reverse ? r.N - 1 : 0, dir = r.reverse ? -1 : 1;
+    a.x = static_cast<const T*>(r.x) + top * r.ldx; a.sx = dir * r.ldx;
+    a.g = r.gate_kind ? static_cast<const T*>(r.gate) + top * r.ldg : nullptr; a.sg = dir * r.ldg;
+    a.h0 = static_cast<const T*>(r.h0); a.ldh0 = r.ldh0;
+    a.gval = (Acc)r.gate_value;
+    a.flag = reinterpret_cast<uint8_t*>(plan + p.flag);
+    a.ep = reinterpret_cast<int32_t*>(plan + p.ep);
+    a.part = reinterpret_cast<int64_t*>(plan + p.part);
+    a.agg = reinterpret_cast<Acc*>(ws + p.agg);
+    a.sh = dir * r.D;
+    return a;
+}
+
+template <typename T> void rec_launch_forward(const RecWalk<T>& a, int gate_kind, const RecPlan& p, hipStream_t st) {
+    rec_with_shape<T>(a.D, [&](auto C, auto V) {
+        auto go = [&](auto GK) {
+            if (p.P > 1)
+                hipLaunchKernelGGL((rec_forward_kernel<T, C(), V(), GK(), true>), dim3(p.blocks, p.P - 1), dim3(REC_THREADS), 0, st, a);
+            const unsigned empty = rec_empty_blocks(a.last, a.E);
+            hipLaunchKernelGGL((rec_forward_kernel<T, C(), V(), GK(), false>), dim3(p.blocks, p.P + empty), dim3(REC_THREADS), 0, st, a);
+        };
+        if (gate_kind == 2) go(std::integral_constant<int, 2>{});
+        else go(std::integral_constant<int, 1>{});
     });
 }
 
-void launch_recurrence_backward(const dcarl_recurrence_t& r, const void* states, void* ws, const void* dh, int64_t lddh, const void* dlast,
+static void rec_launch_walk(const dcarl_recurrence_t& r, const RecPlan& p, char* plan, hipStream_t st) {
+    const int64_t R = (r.N + p.P - 1) / p.P;
+    hipLaunchKernelGGL(rec_walk_kernel, dim3((unsigned)((r.N + p.P) / 256 + 1)), dim3(256), 0, st, r.ep_off, r.E, r.N, r.reverse, p.P, R,
+                       reinterpret_cast<uint8_t*>(plan + p.flag), reinterpret_cast<int32_t*>(plan + p.ep), reinterpret_cast<int64_t*>(plan + p.part));
+}
+
+void launch_recurrence_forward(const dcarl_recurrence_t& r, void* states, void* workspace, void* h, void* last, hipStream_t st) {
+    const RecPlan p = rec_plan(r.N, r.D, r.type, r.gate_kind);
+    char* ws = static_cast<char*>(workspace);
+    char* plan = states ? static_cast<char*>(states) : ws + p.ws_plan;
+    rec_launch_walk(r, p, plan, st);
+    with_type(r.type, [&](auto t) {
+        using T = decltype(t);
+        RecWalk<T> a = rec_walk<T>(r, p, plan, ws);
+        a.h = static_cast<T*>(h) + (r.reverse ? (r.N - 1) * r.D : 0);
+        a.last = static_cast<T*>(last);
+        if (states) a.state = reinterpret_cast<typename SeqType<T>::Acc*>(plan + p.state);
+        rec_launch_forward<T>(a, r.gate_kind, p, st);
+    });
+}
+
+void launch_recurrence_backward(const dcarl_recurrence_t& r, const void* states, void* workspace, const void* dh, int64_t lddh, const void* dlast,
                                 void* dx, void* dgate, void* dh0, hipStream_t st) {
+    const RecPlan p = rec_plan(r.N, r.D, r.type, r.gate_kind);
+    char* ws = static_cast<char*>(workspace);
+    char* plan = static_cast<char*>(const_cast<void*>(states));
     with_type(r.type, [&](auto t) {
         using T = decltype(t);
         using Acc = typename SeqType<T>::Acc;
-        Acc* terms = r.gate_kind == 1 && dgate ? (Acc*)ws : nullptr;
-        if (r.N > 0)
-            hipLaunchKernelGGL((rec_tail_kernel<T>), dim3(256), dim3(256), 0, st, r.ep_off, r.E, r.N, r.D, (T*)dx,
-                               r.gate_kind == 2 ? (T*)dgate : (T*)nullptr, (T*)nullptr);
-        if (r.E > 0)
-            hipLaunchKernelGGL((rec_backward_kernel<T>), rec_grid(r), dim3(64), 0, st, rec_args(r), (const Acc*)states, (const T*)dh, lddh,
-                               (const T*)dlast, (T*)dx, r.gate_kind == 2 ? (T*)dgate : (T*)nullptr, (T*)dh0, terms);
-        if (terms && r.N > 0)
-            hipLaunchKernelGGL((rec_share_kernel<T>), dim3((unsigned)(r.N < 16384 ? r.N : 16384)), dim3(64), 0, st, terms, r.N, r.D, r.ep_off,
-                               r.E, (T*)dgate);
+        RecWalk<T> a = rec_walk<T>(r, p, plan, ws);
+        a.state = reinterpret_cast<Acc*>(plan + p.state);
+        const int64_t top = r.reverse ? r.N - 1 : 0;
+        a.dh = static_cast<const T*>(dh) + top * lddh; a.sdh = (r.reverse ? -1 : 1) * lddh;
+        a.dlast = static_cast<const T*>(dlast);
+        a.dx = dx ? static_cast<T*>(dx) + top * r.D : nullptr;
+        a.dg = dgate ? static_cast<T*>(dgate) + top * (r.gate_kind == 2 ? r.D : 1) : nullptr;
+        a.dh0 = static_cast<T*>(dh0);
+        a.dgp = r.gate_kind == 1 && p.blocks > 1 ? reinterpret_cast<Acc*>(ws + p.dgp) : nullptr;
+        rec_launch_backward<T>(a, r.gate_kind, p, st);
+        if (a.dgp && a.dg)
+            hipLaunchKernelGGL((rec_share_kernel<T>), dim3((unsigned)((r.N + 255) / 256)), dim3(256), 0, st, a.dgp, p.blocks, r.N, r.reverse ? -1 : 1, a.dg);
     });
 }
 
