@@ -92,7 +92,7 @@ int64_t recurrence_workspace_bytes(int64_t, int64_t, int64_t, int, int);
 int64_t recurrence_states_bytes(int64_t, int64_t, int64_t, int, int);
 void launch_recurrence_forward(const dcarl_recurrence_t&, void*, void*, void*, void*, hipStream_t);
 void launch_recurrence_backward(const dcarl_recurrence_t&, const void*, void*, const void*, int64_t, const void*, void*, void*, void*, hipStream_t);
-int64_t rows_workspace_bytes(int64_t, int64_t, int64_t);
+int64_t rows_workspace_bytes(int64_t, int64_t, int64_t, int);
 void launch_rows_gather(int, const void*, int64_t, int64_t, const void*, int, int64_t, int64_t, double, void*, hipStream_t);
 void launch_rows_gradient(int, const void*, int64_t, const void*, int, int64_t, int64_t, int64_t, double, void*, void*, hipStream_t);
 void launch_scores(const dcarl_scores_t&, void*, int64_t, hipStream_t);
@@ -1107,7 +1107,7 @@ int32_t dcarl_recurrence_backward(const dcarl_recurrence_t* r, const void* state
 
 int64_t dcarl_rows_workspace_bytes(int64_t N, int64_t S, int64_t D, int32_t type) {
     if (check_seq("dcarl_rows_workspace_bytes", type, N, D, S)) return 0;
-    return dcarl::rows_workspace_bytes(N, S, D);
+    return dcarl::rows_workspace_bytes(N, S, D, type);
 }
 
 int32_t dcarl_rows_gather(const void* table, int32_t type, int64_t ld, int64_t S, const void* ids, int32_t id_bytes, int64_t N, int64_t D,

@@ -3,25 +3,60 @@
 //   gradient: grad[s] = scale * sum of dout[n] over the n with ids[n] == s, in ascending n: the ids are sorted by a stable radix sort, a row's
 //             gradient is the sum over its run -- no atomics on values, run-to-run identical
 // DS = Simulation_testing/Simulation_Data_Collection/Data_Sampling/data_sampling.py
+#include <type_traits>
 #include "seq_common.h"
 
 namespace dcarl {
 
 constexpr int RW_THREADS = 256;
+constexpr int RW_CHUNK = 128;                  // sorted places a long run is cut into; a run of more is long
+constexpr int RW_DEEP = 8;                     // rows in flight per thread of a sum
+template <typename T> constexpr int RW_VEC = 16 / sizeof(T);
 
 __device__ __forceinline__ int64_t row_id(const void* ids, int wide, int64_t n) {
     return wide ? static_cast<const int64_t*>(ids)[n] : (int64_t) static_cast<const int32_t*>(ids)[n];
 }
 
-template <typename T>
+template <typename T, int VEC> struct RowVec { T v[VEC]; };
+template <typename T, int VEC> __device__ __forceinline__ RowVec<T, VEC> row_load(const T* p) {
+    RowVec<T, VEC> r;
+    __builtin_memcpy(&r, p, sizeof(r));        // rows lie at any multiple of the type: an unaligned vector load
+    return r;
+}
+
+// A workgroup is `lanes` threads along a row (VEC channels each) times 256 / lanes rows; blockIdx.y: 256 * VEC channels each.  The last thread
+// of a row moves back to whole vectors: the same channels as its neighbour, the same values.
+struct RowLane {
+    int c, r, R;
+    int64_t cb;
+    bool live;
+};
+template <int VEC> __device__ __forceinline__ RowLane row_lane(int lanes, int64_t D) {
+    RowLane l;
+    l.R = RW_THREADS / lanes;
+    l.r = (int)threadIdx.x / lanes;
+    l.c = (int)threadIdx.x - l.r * lanes;
+    const int64_t c0 = ((int64_t)blockIdx.y * RW_THREADS + l.c) * VEC;
+    l.cb = c0 < D - VEC ? c0 : D - VEC;
+    l.live = l.r < l.R && c0 < D;
+    return l;
+}
+
+template <typename T, int VEC>
 __global__ __launch_bounds__(RW_THREADS) void rows_gather_kernel(const T* table, int64_t ld, int64_t S, const void* ids, int wide, int64_t N,
-                                                                 int64_t D, double scale, T* out) {
+                                                                 int64_t D, int lanes, double scale, T* out) {
     using Acc = typename SeqType<T>::Acc;
-    for (int64_t n = blockIdx.x; n < N; n += gridDim.x) {
+    const RowLane l = row_lane<VEC>(lanes, D);
+    if (!l.live) return;
+    const int64_t step = (int64_t)gridDim.x * l.R;
+    for (int64_t n = (int64_t)blockIdx.x * l.R + l.r; n < N; n += step) {
         const int64_t s = row_id(ids, wide, n);
+        RowVec<T, VEC> v, o;
         const bool in = s >= 0 && s < S;
-        for (int64_t d = threadIdx.x; d < D; d += RW_THREADS)
-            out[n * D + d] = narrow<T>(in ? widen(table[s * ld + d]) * (Acc)scale : Acc(0));
+        if (in) v = row_load<T, VEC>(table + s * ld + l.cb);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.v[i] = in ? narrow<T>(widen(v.v[i]) * (Acc)scale) : narrow<T>(0.0f);
+        __builtin_memcpy(out + n * D + l.cb, &o, sizeof(o));
     }
 }
 
@@ -135,27 +170,114 @@ __global__ __launch_bounds__(256) void rows_begin_kernel(const uint32_t* key, in
     begin[s] = (uint32_t)lo;
 }
 
-template <typename T>
-__global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* begin, const uint32_t* pos, const T* dout, int64_t ldd, int64_t S,
-                                                              int64_t D, double scale, T* grad) {
+// adds m rows to sum, in order: row(i) is the address of the i-th; RW_DEEP of them are in flight
+template <typename T, int VEC, typename Acc, typename Row> __device__ __forceinline__ void rows_add(Acc (&sum)[VEC], int64_t m, Row&& row) {
+    int64_t i = 0;
+    for (; i + RW_DEEP <= m; i += RW_DEEP) {
+        const T* at[RW_DEEP];
+        RowVec<T, VEC> v[RW_DEEP];
+#pragma unroll
+        for (int j = 0; j < RW_DEEP; ++j) at[j] = row(i + j);
+#pragma unroll
+        for (int j = 0; j < RW_DEEP; ++j) v[j] = row_load<T, VEC>(at[j]);
+#pragma unroll
+        for (int j = 0; j < RW_DEEP; ++j)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += widen(v[j].v[k]);
+    }
+    for (; i < m; ++i) {
+        const RowVec<T, VEC> v = row_load<T, VEC>(row(i));
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] += widen(v.v[k]);
+    }
+}
+// the sums of the workgroup's row groups, added in their order, for the threads of group 0
+template <int VEC, typename Acc> __device__ __forceinline__ void rows_join(Acc (&sum)[VEC], Acc* lds, const RowLane& l, int lanes) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) lds[threadIdx.x * VEC + k] = sum[k];
+    __syncthreads();
+    if (l.r == 0)
+        for (int r = 1; r < l.R; ++r)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += lds[(r * lanes + l.c) * VEC + k];
+}
+
+// The sums of the long runs (more than RW_CHUNK places) over one chunk of RW_CHUNK sorted places.  At most two long runs meet a chunk: the one
+// of its first place (part[chunk][0]) and the one of its last (part[chunk][1]).  The workgroup's groups take a quarter, a third ... of the places each.
+template <typename T, int VEC>
+__global__ __launch_bounds__(RW_THREADS) void rows_chunk_kernel(const uint32_t* key, const uint32_t* begin, const uint32_t* pos, const T* dout,
+                                                                int64_t ldd, int64_t N, int64_t S, int64_t D, int lanes, typename SeqType<T>::Acc* part) {
     using Acc = typename SeqType<T>::Acc;
-    for (int64_t s = blockIdx.x; s < S; s += gridDim.x) {
+    __shared__ Acc lds[RW_THREADS * VEC];
+    const RowLane l = row_lane<VEC>(lanes, D);
+    const int64_t b = (int64_t)blockIdx.x * RW_CHUNK, e = b + RW_CHUNK < N ? b + RW_CHUNK : N;
+    const uint32_t first = key[b], last = key[e - 1];
+    for (int slot = 0; slot < 2; ++slot) {
+        const uint32_t k = slot ? last : first;
+        if ((slot && last == first) || k >= S) continue;
+        const int64_t rb = begin[k], re = begin[k + 1];
+        if (re - rb <= RW_CHUNK) continue;
+        const int64_t lo = rb > b ? rb : b, hi = re < e ? re : e;
+        const int64_t each = (hi - lo + l.R - 1) / l.R, from = lo + l.r * each, to = from + each < hi ? from + each : hi;
+        Acc sum[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] = 0;
+        if (l.live && from < to) rows_add<T, VEC>(sum, to - from, [&](int64_t i) { return dout + (int64_t)pos[from + i] * ldd + l.cb; });
+        rows_join<VEC>(sum, lds, l, lanes);
+        if (l.live && l.r == 0)
+            for (int i = 0; i < VEC; ++i) part[((int64_t)blockIdx.x * 2 + slot) * D + l.cb + i] = sum[i];
+    }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* begin, const uint32_t* pos, const T* dout, int64_t ldd, int64_t S,
+                                                              int64_t D, int lanes, double scale, const typename SeqType<T>::Acc* part, T* grad) {
+    using Acc = typename SeqType<T>::Acc;
+    __shared__ Acc lds[RW_THREADS * VEC];
+    const RowLane l = row_lane<VEC>(lanes, D);
+    auto put = [&](int64_t s, const Acc(&sum)[VEC]) {
+        RowVec<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.v[i] = narrow<T>(sum[i] * (Acc)scale);
+        __builtin_memcpy(grad + s * D + l.cb, &o, sizeof(o));
+    };
+    const int64_t s0 = (int64_t)blockIdx.x * l.R;
+    const int64_t s = s0 + l.r;
+    Acc sum[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = 0;
+    bool is_long = false;
+    if (l.live && s < S) {
         const uint32_t b = begin[s], e = begin[s + 1];
-        for (int64_t d = threadIdx.x; d < D; d += RW_THREADS) {
-            Acc sum = 0;
-            for (uint32_t i = b; i < e; ++i) sum += widen(dout[(int64_t)pos[i] * ldd + d]);
-            grad[s * D + d] = narrow<T>(sum * (Acc)scale);
+        is_long = e - b > RW_CHUNK;
+        if (!is_long) {
+            rows_add<T, VEC>(sum, e - b, [&](int64_t i) { return dout + (int64_t)pos[b + i] * ldd + l.cb; });
+            put(s, sum);
         }
+    }
+    if (!__syncthreads_or(is_long)) return;
+    for (int r = 0; r < l.R && s0 + r < S; ++r) {          // the long ones, the whole workgroup at each: partial sums of their chunks
+        const int64_t b = begin[s0 + r], e = begin[s0 + r + 1];
+        if (e - b <= RW_CHUNK) continue;
+        const int64_t c0 = b / RW_CHUNK, m = (e - 1) / RW_CHUNK - c0 + 1;
+        const int64_t each = (m + l.R - 1) / l.R, from = l.r * each, to = from + each < m ? from + each : m;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] = 0;
+        if (l.live && from < to)
+            rows_add<Acc, VEC>(sum, to - from, [&](int64_t i) { return part + ((c0 + from + i) * 2 + (from + i == 0 && b % RW_CHUNK != 0)) * D + l.cb; });
+        rows_join<VEC>(sum, lds, l, lanes);
+        if (l.live && l.r == 0) put(s0 + r, sum);
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
 struct RowsPlan {
     int nblk, passes;
-    int64_t key0, key1, pos0, pos1, hist, total, begin, bytes;
+    int64_t key0, key1, pos0, pos1, hist, total, begin, part, bytes;
 };
 static int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
-static RowsPlan rows_plan(int64_t N, int64_t S, int64_t) {
+static RowsPlan rows_plan(int64_t N, int64_t S, int64_t D, int type) {
     RowsPlan p;
     p.nblk = (int)((N + RS_ITEMS - 1) / RS_ITEMS);
     int bits = 1;
@@ -165,23 +287,38 @@ static RowsPlan rows_plan(int64_t N, int64_t S, int64_t) {
     auto take = [&](int64_t words) { const int64_t here = at; at += up16(words * 4); return here; };
     p.key0 = take(N); p.key1 = take(N); p.pos0 = take(N); p.pos1 = take(N);
     p.hist = take((int64_t)RS_BINS * p.nblk); p.total = take(RS_BINS); p.begin = take(S + 1);
+    p.part = take((N + RW_CHUNK - 1) / RW_CHUNK * 2 * D * (type == DCARL_F64 ? 2 : 1));
     p.bytes = at;
     return p;
 }
-int64_t rows_workspace_bytes(int64_t N, int64_t S, int64_t D) { return rows_plan(N, S, D).bytes; }
+int64_t rows_workspace_bytes(int64_t N, int64_t S, int64_t D, int type) { return rows_plan(N, S, D, type).bytes; }
+
+// f(T{}, VEC, threads along a row, blocks along a row)
+template <typename F> static void rows_with(int type, int64_t D, F&& f) {
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        auto go = [&](auto V) {
+            const int64_t vecs = (D + V() - 1) / V();
+            f(t, V, (int)(vecs < RW_THREADS ? vecs : RW_THREADS), (unsigned)((vecs + RW_THREADS - 1) / RW_THREADS));
+        };
+        if (D >= RW_VEC<T>) go(std::integral_constant<int, RW_VEC<T>>{});
+        else go(std::integral_constant<int, 1>{});
+    });
+}
 
 void launch_rows_gather(int type, const void* table, int64_t ld, int64_t S, const void* ids, int id_bytes, int64_t N, int64_t D, double scale,
                         void* out, hipStream_t st) {
-    with_type(type, [&](auto t) {
+    rows_with(type, D, [&](auto t, auto V, int lanes, unsigned across) {
         using T = decltype(t);
-        hipLaunchKernelGGL((rows_gather_kernel<T>), dim3((unsigned)(N < 65536 ? N : 65536)), dim3(RW_THREADS), 0, st, (const T*)table, ld, S, ids,
-                           id_bytes == 8, N, D, scale, (T*)out);
+        const int64_t need = (N + RW_THREADS / lanes - 1) / (RW_THREADS / lanes);
+        hipLaunchKernelGGL((rows_gather_kernel<T, V()>), dim3((unsigned)(need < (1 << 20) ? need : 1 << 20), across), dim3(RW_THREADS), 0, st,
+                           (const T*)table, ld, S, ids, id_bytes == 8, N, D, lanes, scale, (T*)out);
     });
 }
 
 void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* ids, int id_bytes, int64_t N, int64_t D, int64_t S, double scale,
                           void* ws, void* grad, hipStream_t st) {
-    const RowsPlan p = rows_plan(N, S, D);
+    const RowsPlan p = rows_plan(N, S, D, type);
     char* w = static_cast<char*>(ws);
     auto at = [&](int64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
     uint32_t *k_in = nullptr, *p_in = nullptr, *k_out = at(p.key0), *p_out = at(p.pos0);
@@ -194,10 +331,16 @@ void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* i
         k_out = at(i % 2 ? p.key0 : p.key1); p_out = at(i % 2 ? p.pos0 : p.pos1);
     }
     hipLaunchKernelGGL(rows_begin_kernel, dim3((unsigned)((S + 256) / 256)), dim3(256), 0, st, k_in, N, S, at(p.begin));
-    with_type(type, [&](auto t) {
+    rows_with(type, D, [&](auto t, auto V, int lanes, unsigned across) {
         using T = decltype(t);
-        hipLaunchKernelGGL((rows_sum_kernel<T>), dim3((unsigned)(S < 65536 ? S : 65536)), dim3(RW_THREADS), 0, st, at(p.begin), p_in, (const T*)dout,
-                           ldd, S, D, scale, (T*)grad);
+        using Acc = typename SeqType<T>::Acc;
+        Acc* part = reinterpret_cast<Acc*>(w + p.part);
+        const int64_t R = RW_THREADS / lanes;
+        if (N > RW_CHUNK)
+            hipLaunchKernelGGL((rows_chunk_kernel<T, V()>), dim3((unsigned)((N + RW_CHUNK - 1) / RW_CHUNK), across), dim3(RW_THREADS), 0, st, k_in,
+                               at(p.begin), p_in, (const T*)dout, ldd, N, S, D, lanes, part);
+        hipLaunchKernelGGL((rows_sum_kernel<T, V()>), dim3((unsigned)((S + R - 1) / R), across), dim3(RW_THREADS), 0, st, at(p.begin), p_in,
+                           (const T*)dout, ldd, S, D, lanes, scale, part, (T*)grad);
     });
 }
 
