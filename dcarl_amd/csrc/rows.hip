@@ -11,6 +11,8 @@ namespace dcarl {
 constexpr int RW_THREADS = 256;
 constexpr int RW_CHUNK = 128;                  // sorted places a long run is cut into; a run of more is long
 constexpr int RW_DEEP = 8;                     // rows in flight per thread of a sum
+constexpr int RW_ROWS = 4;                     // ... of the gather
+constexpr int RW_SUPER = 32;                   // chunks whose partial sums are joined first where a run has more
 template <typename T> constexpr int RW_VEC = 16 / sizeof(T);
 
 __device__ __forceinline__ int64_t row_id(const void* ids, int wide, int64_t n) {
@@ -48,21 +50,36 @@ __global__ __launch_bounds__(RW_THREADS) void rows_gather_kernel(const T* table,
     using Acc = typename SeqType<T>::Acc;
     const RowLane l = row_lane<VEC>(lanes, D);
     if (!l.live) return;
-    const int64_t step = (int64_t)gridDim.x * l.R;
-    for (int64_t n = (int64_t)blockIdx.x * l.R + l.r; n < N; n += step) {
-        const int64_t s = row_id(ids, wide, n);
-        RowVec<T, VEC> v, o;
-        const bool in = s >= 0 && s < S;
-        if (in) v = row_load<T, VEC>(table + s * ld + l.cb);
+    // four consecutive groups of rows at a time, their ids and then their rows in flight together
+    const int64_t step = (int64_t)gridDim.x * l.R * RW_ROWS;
+    for (int64_t n0 = (int64_t)blockIdx.x * l.R * RW_ROWS + l.r; n0 < N; n0 += step) {
+        int64_t s[RW_ROWS];
+        RowVec<T, VEC> v[RW_ROWS];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o.v[i] = in ? narrow<T>(widen(v.v[i]) * (Acc)scale) : narrow<T>(0.0f);
-        __builtin_memcpy(out + n * D + l.cb, &o, sizeof(o));
+        for (int j = 0; j < RW_ROWS; ++j) {
+            const int64_t n = n0 + j * l.R;
+            s[j] = n < N ? row_id(ids, wide, n) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < RW_ROWS; ++j)
+            if (s[j] >= 0 && s[j] < S) v[j] = row_load<T, VEC>(table + s[j] * ld + l.cb);
+#pragma unroll
+        for (int j = 0; j < RW_ROWS; ++j) {
+            const int64_t n = n0 + j * l.R;
+            const bool in = s[j] >= 0 && s[j] < S;
+            RowVec<T, VEC> o;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o.v[i] = in ? narrow<T>(widen(v[j].v[i]) * (Acc)scale) : narrow<T>(0.0f);
+            if (n < N) __builtin_memcpy(out + n * D + l.cb, &o, sizeof(o));
+        }
     }
 }
 
-// ---- stable radix sort of (id, n): per pass a histogram per block, an exclusive scan of each digit over the blocks, a scatter ------------
-constexpr int RS_ITEMS = 4096;                 // per block: 4 wavefronts, 1024 consecutive items each, 64 at a time
+// ---- stable radix sort of (id, n): per pass a histogram per block, places by an exclusive scan over digits and blocks, a scatter -----------
+// 1024 items per block: 16384 ids make 16 blocks whose four rounds take about 2 us; 4096 per block took 17 us a pass there.
+constexpr int RS_ROUNDS = 4, RS_ITEMS = 256 * RS_ROUNDS;   // per block: 4 wavefronts of consecutive items, 64 at a time
 constexpr int RS_BITS = 8, RS_BINS = 1 << RS_BITS;
+constexpr int RS_DIRECT = 64;                  // up to so many blocks each scatter block adds the others' counts itself: a launch less
 
 // the sort key: the id, or S ("no row", behind every row) for ids outside the table
 __device__ __forceinline__ uint32_t row_key(const void* ids, int wide, const uint32_t* key, int64_t S, int64_t n) {
@@ -71,74 +88,91 @@ __device__ __forceinline__ uint32_t row_key(const void* ids, int wide, const uin
     return (uint32_t)(s >= 0 && s < S ? s : S);
 }
 
-__global__ __launch_bounds__(256) void rows_hist_kernel(const void* ids, int wide, const uint32_t* key, int64_t S, int64_t N, int shift,
-                                                        uint32_t* hist, int nblk) {
+// inclusive scan of 256 values over a workgroup of 256
+__device__ __forceinline__ uint32_t scan256(uint32_t v, uint32_t (&tot)[4]) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(v, o);
+        if (lane >= o) v += up;
+    }
+    __syncthreads();
+    if (lane == 63) tot[wv] = v;
+    __syncthreads();
+    for (int w = 0; w < wv; ++w) v += tot[w];
+    return v;
+}
+
+// hist[block][digit]
+__global__ __launch_bounds__(256) void rows_hist_kernel(const void* ids, int wide, const uint32_t* key, int64_t S, int64_t N, int shift, uint32_t* hist) {
     __shared__ uint32_t h[RS_BINS];
     h[threadIdx.x] = 0;
     __syncthreads();
-    const int64_t b = (int64_t)blockIdx.x * RS_ITEMS;
-    for (int i = threadIdx.x; i < RS_ITEMS && b + i < N; i += 256)
-        atomicAdd(&h[(row_key(ids, wide, key, S, b + i) >> shift) & (RS_BINS - 1)], 1u);
+    const int64_t b = (int64_t)blockIdx.x * RS_ITEMS + threadIdx.x;
+    uint32_t k[RS_ROUNDS];
+#pragma unroll
+    for (int i = 0; i < RS_ROUNDS; ++i)
+        if (b + i * 256 < N) k[i] = row_key(ids, wide, key, S, b + i * 256);
+#pragma unroll
+    for (int i = 0; i < RS_ROUNDS; ++i)
+        if (b + i * 256 < N) atomicAdd(&h[(k[i] >> shift) & (RS_BINS - 1)], 1u);
     __syncthreads();
-    hist[(int64_t)threadIdx.x * nblk + blockIdx.x] = h[threadIdx.x];
+    hist[(int64_t)blockIdx.x * RS_BINS + threadIdx.x] = h[threadIdx.x];
 }
 
 // block d: exclusive scan of digit d's counts over the blocks, in place; its total
 __global__ __launch_bounds__(256) void rows_scan_kernel(uint32_t* hist, int nblk, uint32_t* total) {
-    __shared__ uint32_t sm[256];
-    uint32_t* row = hist + (int64_t)blockIdx.x * nblk;
+    __shared__ uint32_t tot[4];
+    uint32_t* col = hist + blockIdx.x;
     uint32_t carry = 0;
     for (int base = 0; base < nblk; base += 256) {
         const int i = base + threadIdx.x;
-        const uint32_t v = i < nblk ? row[i] : 0;
-        sm[threadIdx.x] = v;
+        const uint32_t v = i < nblk ? col[(int64_t)i * RS_BINS] : 0, in = scan256(v, tot);
+        if (i < nblk) col[(int64_t)i * RS_BINS] = carry + in - v;
         __syncthreads();
-        for (int o = 1; o < 256; o <<= 1) {
-            const uint32_t add = (int)threadIdx.x >= o ? sm[threadIdx.x - o] : 0;
-            __syncthreads();
-            sm[threadIdx.x] += add;
-            __syncthreads();
-        }
-        if (i < nblk) row[i] = carry + sm[threadIdx.x] - v;
-        carry += sm[255];
-        __syncthreads();
+        carry += tot[0] + tot[1] + tot[2] + tot[3];
     }
     if (threadIdx.x == 0) total[blockIdx.x] = carry;
 }
 
+// total == NULL: hist holds the blocks' own counts, nblk <= RS_DIRECT
 __global__ __launch_bounds__(256) void rows_scatter_kernel(const void* ids, int wide, const uint32_t* key, const uint32_t* pos, int64_t S,
                                                            int64_t N, int shift, const uint32_t* hist, const uint32_t* total, int nblk,
                                                            uint32_t* key_out, uint32_t* pos_out) {
     __shared__ uint32_t cnt[4][RS_BINS];       // first the wavefronts' counts, then where each one's items of a digit go
-    __shared__ uint32_t sm[RS_BINS];
+    __shared__ uint32_t tot[4];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int64_t b = (int64_t)blockIdx.x * RS_ITEMS + wv * (64 * RS_ROUNDS) + lane;
+    uint32_t k[RS_ROUNDS], ps[RS_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r) {
+        const int64_t n = b + r * 64;
+        k[r] = n < N ? row_key(ids, wide, key, S, n) : 0xffffffffu;
+        ps[r] = n < N && pos ? pos[n] : (uint32_t)n;
+    }
+    uint32_t all = 0, before = 0;              // of digit `tid`: items everywhere, items in earlier blocks
+    if (total) { all = total[tid]; before = hist[(int64_t)blockIdx.x * RS_BINS + tid]; }
+    else
+        for (int i = 0; i < nblk; ++i) {
+            const uint32_t c = hist[(int64_t)i * RS_BINS + tid];
+            all += c;
+            before += i < (int)blockIdx.x ? c : 0;
+        }
 #pragma unroll
     for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
-    sm[tid] = total[tid];
-    __syncthreads();
-    for (int o = 1; o < RS_BINS; o <<= 1) {    // inclusive scan of the digits' totals
-        const uint32_t add = tid >= o ? sm[tid - o] : 0;
-        __syncthreads();
-        sm[tid] += add;
-        __syncthreads();
-    }
-    const int64_t b = (int64_t)blockIdx.x * RS_ITEMS + wv * (RS_ITEMS / 4);
-    for (int r = 0; r < RS_ITEMS / 256; ++r) {
-        const int64_t n = b + r * 64 + lane;
-        if (n < N) atomicAdd(&cnt[wv][(row_key(ids, wide, key, S, n) >> shift) & (RS_BINS - 1)], 1u);
-    }
-    __syncthreads();
-    {
-        uint32_t at = (tid ? sm[tid - 1] : 0) + hist[(int64_t)tid * nblk + blockIdx.x];
+    const uint32_t first = scan256(all, tot) - all;        // (its barriers: the counts are cleared)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) { const uint32_t c = cnt[w][tid]; cnt[w][tid] = at; at += c; }
-    }
+    for (int r = 0; r < RS_ROUNDS; ++r)
+        if (b + r * 64 < N) atomicAdd(&cnt[wv][(k[r] >> shift) & (RS_BINS - 1)], 1u);
     __syncthreads();
-    for (int r = 0; r < RS_ITEMS / 256; ++r) {
-        const int64_t n = b + r * 64 + lane;
-        const bool live = n < N;
-        const uint32_t k = live ? row_key(ids, wide, key, S, n) : 0xffffffffu;
-        const uint32_t dig = (k >> shift) & (RS_BINS - 1);
+    uint32_t at = first + before;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) { const uint32_t c = cnt[w][tid]; cnt[w][tid] = at; at += c; }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RS_ROUNDS; ++r) {
+        const bool live = b + r * 64 < N;
+        const uint32_t dig = (k[r] >> shift) & (RS_BINS - 1);
         unsigned long long same = __ballot(live);
 #pragma unroll
         for (int j = 0; j < RS_BITS; ++j) {
@@ -146,14 +180,14 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(const void* ids, int 
             same &= (dig >> j) & 1 ? bit : ~bit;
         }
         const int rank = __popcll(same & ((1ull << lane) - 1));
-        uint32_t at = 0;
-        if (live) at = cnt[wv][dig];
+        uint32_t to = 0;
+        if (live) to = cnt[wv][dig];
         __builtin_amdgcn_wave_barrier();       // every lane has read its digit's place before the first lane of a group moves it on
-        if (live && rank == 0) cnt[wv][dig] = at + (uint32_t)__popcll(same);
+        if (live && rank == 0) cnt[wv][dig] = to + (uint32_t)__popcll(same);
         __builtin_amdgcn_wave_barrier();
         if (live) {
-            key_out[at + rank] = k;
-            pos_out[at + rank] = pos ? pos[n] : (uint32_t)n;
+            key_out[to + rank] = k[r];
+            pos_out[to + rank] = ps[r];
         }
     }
 }
@@ -230,9 +264,38 @@ __global__ __launch_bounds__(RW_THREADS) void rows_chunk_kernel(const uint32_t* 
     }
 }
 
+// The runs of more than RW_CHUNK * RW_SUPER places: the partial sums of the chunks of one super chunk, joined the same way
+// (T: only the type of the sums matters here).
+template <typename Acc, int VEC>
+__global__ __launch_bounds__(RW_THREADS) void rows_super_kernel(const uint32_t* key, const uint32_t* begin, int64_t N, int64_t S, int64_t D, int lanes,
+                                                                const Acc* part, Acc* super) {
+    __shared__ Acc lds[RW_THREADS * VEC];
+    const RowLane l = row_lane<VEC>(lanes, D);
+    constexpr int64_t PLACES = RW_CHUNK * RW_SUPER;
+    const int64_t b = (int64_t)blockIdx.x * PLACES, e = b + PLACES < N ? b + PLACES : N;
+    const uint32_t first = key[b], last = key[e - 1];
+    for (int slot = 0; slot < 2; ++slot) {
+        const uint32_t k = slot ? last : first;
+        if ((slot && last == first) || k >= S) continue;
+        const int64_t rb = begin[k], re = begin[k + 1];
+        if (re - rb <= PLACES) continue;
+        const int64_t c0 = (rb > b ? rb : b) / RW_CHUNK, m = ((re < e ? re : e) - 1) / RW_CHUNK - c0 + 1;
+        const int64_t each = (m + l.R - 1) / l.R, from = l.r * each, to = from + each < m ? from + each : m;
+        Acc sum[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] = 0;
+        if (l.live && from < to)
+            rows_add<Acc, VEC>(sum, to - from, [&](int64_t i) { return part + ((c0 + from + i) * 2 + ((c0 + from + i) * RW_CHUNK < rb)) * D + l.cb; });
+        rows_join<VEC>(sum, lds, l, lanes);
+        if (l.live && l.r == 0)
+            for (int i = 0; i < VEC; ++i) super[((int64_t)blockIdx.x * 2 + slot) * D + l.cb + i] = sum[i];
+    }
+}
+
 template <typename T, int VEC>
 __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* begin, const uint32_t* pos, const T* dout, int64_t ldd, int64_t S,
-                                                              int64_t D, int lanes, double scale, const typename SeqType<T>::Acc* part, T* grad) {
+                                                              int64_t D, int lanes, double scale, const typename SeqType<T>::Acc* part,
+                                                              const typename SeqType<T>::Acc* super, T* grad) {
     using Acc = typename SeqType<T>::Acc;
     __shared__ Acc lds[RW_THREADS * VEC];
     const RowLane l = row_lane<VEC>(lanes, D);
@@ -260,12 +323,15 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
     for (int r = 0; r < l.R && s0 + r < S; ++r) {          // the long ones, the whole workgroup at each: partial sums of their chunks
         const int64_t b = begin[s0 + r], e = begin[s0 + r + 1];
         if (e - b <= RW_CHUNK) continue;
-        const int64_t c0 = b / RW_CHUNK, m = (e - 1) / RW_CHUNK - c0 + 1;
+        const bool very = e - b > RW_CHUNK * RW_SUPER;
+        const int64_t places = very ? RW_CHUNK * RW_SUPER : RW_CHUNK;
+        const Acc* from_part = very ? super : part;
+        const int64_t c0 = b / places, m = (e - 1) / places - c0 + 1;
         const int64_t each = (m + l.R - 1) / l.R, from = l.r * each, to = from + each < m ? from + each : m;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) sum[i] = 0;
         if (l.live && from < to)
-            rows_add<Acc, VEC>(sum, to - from, [&](int64_t i) { return part + ((c0 + from + i) * 2 + (from + i == 0 && b % RW_CHUNK != 0)) * D + l.cb; });
+            rows_add<Acc, VEC>(sum, to - from, [&](int64_t i) { return from_part + ((c0 + from + i) * 2 + ((c0 + from + i) * places < b)) * D + l.cb; });
         rows_join<VEC>(sum, lds, l, lanes);
         if (l.live && l.r == 0) put(s0 + r, sum);
     }
@@ -274,7 +340,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------
 struct RowsPlan {
     int nblk, passes;
-    int64_t key0, key1, pos0, pos1, hist, total, begin, part, bytes;
+    int64_t key0, key1, pos0, pos1, hist, total, begin, part, super, bytes;
 };
 static int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 static RowsPlan rows_plan(int64_t N, int64_t S, int64_t D, int type) {
@@ -288,6 +354,7 @@ static RowsPlan rows_plan(int64_t N, int64_t S, int64_t D, int type) {
     p.key0 = take(N); p.key1 = take(N); p.pos0 = take(N); p.pos1 = take(N);
     p.hist = take((int64_t)RS_BINS * p.nblk); p.total = take(RS_BINS); p.begin = take(S + 1);
     p.part = take((N + RW_CHUNK - 1) / RW_CHUNK * 2 * D * (type == DCARL_F64 ? 2 : 1));
+    p.super = take((N + RW_CHUNK * RW_SUPER - 1) / (RW_CHUNK * RW_SUPER) * 2 * D * (type == DCARL_F64 ? 2 : 1));
     p.bytes = at;
     return p;
 }
@@ -310,7 +377,7 @@ void launch_rows_gather(int type, const void* table, int64_t ld, int64_t S, cons
                         void* out, hipStream_t st) {
     rows_with(type, D, [&](auto t, auto V, int lanes, unsigned across) {
         using T = decltype(t);
-        const int64_t need = (N + RW_THREADS / lanes - 1) / (RW_THREADS / lanes);
+        const int64_t each = (int64_t)(RW_THREADS / lanes) * RW_ROWS, need = (N + each - 1) / each;
         hipLaunchKernelGGL((rows_gather_kernel<T, V()>), dim3((unsigned)(need < (1 << 20) ? need : 1 << 20), across), dim3(RW_THREADS), 0, st,
                            (const T*)table, ld, S, ids, id_bytes == 8, N, D, lanes, scale, (T*)out);
     });
@@ -323,10 +390,11 @@ void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* i
     auto at = [&](int64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
     uint32_t *k_in = nullptr, *p_in = nullptr, *k_out = at(p.key0), *p_out = at(p.pos0);
     for (int i = 0; i < p.passes && N > 0; ++i) {
-        hipLaunchKernelGGL(rows_hist_kernel, dim3(p.nblk), dim3(256), 0, st, ids, id_bytes == 8, k_in, S, N, i * RS_BITS, at(p.hist), p.nblk);
-        hipLaunchKernelGGL(rows_scan_kernel, dim3(RS_BINS), dim3(256), 0, st, at(p.hist), p.nblk, at(p.total));
+        const bool direct = p.nblk <= RS_DIRECT;
+        hipLaunchKernelGGL(rows_hist_kernel, dim3(p.nblk), dim3(256), 0, st, ids, id_bytes == 8, k_in, S, N, i * RS_BITS, at(p.hist));
+        if (!direct) hipLaunchKernelGGL(rows_scan_kernel, dim3(RS_BINS), dim3(256), 0, st, at(p.hist), p.nblk, at(p.total));
         hipLaunchKernelGGL(rows_scatter_kernel, dim3(p.nblk), dim3(256), 0, st, ids, id_bytes == 8, k_in, p_in, S, N, i * RS_BITS, at(p.hist),
-                           at(p.total), p.nblk, k_out, p_out);
+                           direct ? nullptr : at(p.total), p.nblk, k_out, p_out);
         k_in = k_out; p_in = p_out;
         k_out = at(i % 2 ? p.key0 : p.key1); p_out = at(i % 2 ? p.pos0 : p.pos1);
     }
@@ -334,13 +402,16 @@ void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* i
     rows_with(type, D, [&](auto t, auto V, int lanes, unsigned across) {
         using T = decltype(t);
         using Acc = typename SeqType<T>::Acc;
-        Acc* part = reinterpret_cast<Acc*>(w + p.part);
+        Acc *part = reinterpret_cast<Acc*>(w + p.part), *super = reinterpret_cast<Acc*>(w + p.super);
         const int64_t R = RW_THREADS / lanes;
         if (N > RW_CHUNK)
             hipLaunchKernelGGL((rows_chunk_kernel<T, V()>), dim3((unsigned)((N + RW_CHUNK - 1) / RW_CHUNK), across), dim3(RW_THREADS), 0, st, k_in,
                                at(p.begin), p_in, (const T*)dout, ldd, N, S, D, lanes, part);
+        if (N > RW_CHUNK * RW_SUPER)
+            hipLaunchKernelGGL((rows_super_kernel<Acc, V()>), dim3((unsigned)((N + RW_CHUNK * RW_SUPER - 1) / (RW_CHUNK * RW_SUPER)), across),
+                               dim3(RW_THREADS), 0, st, k_in, at(p.begin), N, S, D, lanes, part, super);
         hipLaunchKernelGGL((rows_sum_kernel<T, V()>), dim3((unsigned)((S + R - 1) / R), across), dim3(RW_THREADS), 0, st, at(p.begin), p_in,
-                           (const T*)dout, ldd, S, D, lanes, scale, part, (T*)grad);
+                           (const T*)dout, ldd, S, D, lanes, scale, part, super, (T*)grad);
     });
 }
 
