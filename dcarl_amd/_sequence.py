@@ -2,8 +2,6 @@
 checks of ids and offsets, the device a call runs on."""
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
@@ -33,22 +31,39 @@ def on_device(*named) -> torch.device:
     return dev[1].device
 
 
-@contextlib.contextmanager
-def running_on(device: torch.device):
-    """Everything inside — allocations, the current stream, the launches — on `device`, whatever the current device is."""
+def run_on(device: torch.device, call, *args):
+    """call(*args) with everything in it — allocations, the current stream, the launches — on `device`, whatever the current device is."""
     if torch.cuda.current_device() == device.index:
-        yield
-    else:
-        with torch.cuda.device(device):
-            yield
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
+
+
+def stream(device: torch.device) -> int:
+    """The handle of the device's current stream (the wrapper object that torch.cuda.current_stream builds costs 3 us a call)."""
+    return _raw_stream(device.index)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def at(t):
+    """The address of a tensor, None where there is none."""
+    return None if t is None else t.data_ptr()
+
+
+def wants_gradient(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def rows_of(t: torch.Tensor):
     """(tensor, elements between its rows) of a 2-D operand whose channels are contiguous; a copy where they are not.  Rows may lie
     anywhere at a non-negative distance (slices, one row expanded to many)."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.stride(0) < 0:
+    step, one = t.stride()
+    if one != 1 and t.shape[1] > 1 or step < 0:
         t = t.contiguous()
-    return t, t.stride(0)
+        step = t.stride(0)
+    return t, step
 
 
 def capturing() -> bool:
@@ -56,7 +71,8 @@ def capturing() -> bool:
 
 
 def whole_numbers(name: str, t) -> torch.Tensor:
-    t = torch.as_tensor(t)
+    if not isinstance(t, torch.Tensor):
+        t = torch.as_tensor(t)
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
     return t
@@ -76,4 +92,4 @@ def offsets(name: str, off, n: int, segments, validate: bool) -> torch.Tensor:
         host = off.cpu().to(torch.int64)
         if int(host[0]) != 0 or int(host[-1]) > n or bool((host[1:] < host[:-1]).any()):
             raise ValueError(f"{name} must rise from 0 to at most {n}")
-    return off.to(torch.int64).contiguous()
+    return off if off.dtype == torch.int64 and off.is_contiguous() else off.to(torch.int64).contiguous()

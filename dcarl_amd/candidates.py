@@ -88,13 +88,18 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
             raise ValueError("out requires a gradient")
     dev = _seq.on_device(("scores", scores), ("taken", taken), ("taken_off", off), ("given", given), ("repetition", rep), ("frequency", freq),
                          ("presence", pres), ("bias", bias), ("allowed", allowed), ("out", out))
-    with _seq.running_on(dev):
-        s, ld = _seq.rows_of(scores)
-        z = torch.empty(B, V, dtype=s.dtype, device=dev) if out is None else out
-        given = None if given is None else given.contiguous()
-        at = lambda t: 0 if t is None else t.data_ptr()      # noqa: E731
-        a = _lib.CScores(at(s), B, V, ld, at(taken), at(off), 0 if taken is None else taken.numel(), at(given), at(rep), at(freq), at(pres), at(bias),
-                         ld_bias, at(allowed), ld_allowed, rep0 if rep is None else 1.0, freq0, pres0, _seq.TYPES[s.dtype],
-                         4 if taken is None else taken.element_size(), 0)
-        _lib.check(_lib.load().dcarl_adjust_scores(C.byref(a), _lib.ptr(z), z.stride(0), _lib.stream_ptr()), "dcarl_adjust_scores")
+    return _seq.run_on(dev, _adjust, scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias, ld_bias, allowed, ld_allowed, out)
+
+
+def _adjust(scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias, ld_bias, allowed, ld_allowed, out):
+    B, V = scores.shape
+    dev = scores.device
+    s, ld = _seq.rows_of(scores)
+    z = torch.empty(B, V, dtype=s.dtype, device=dev) if out is None else out
+    given = None if given is None else given.contiguous()
+    at = _seq.at
+    a = _lib.CScores(at(s), B, V, ld, at(taken), at(off), 0 if taken is None else taken.numel(), at(given), at(rep), at(freq), at(pres), at(bias),
+                     ld_bias, at(allowed), ld_allowed, rep0 if rep is None else 1.0, freq0, pres0, _seq.TYPES[s.dtype],
+                     4 if taken is None else taken.element_size(), 0)
+    _lib.check(_lib.load().dcarl_adjust_scores(C.byref(a), at(z), z.stride(0), _seq.stream(dev)), "dcarl_adjust_scores")
     return z

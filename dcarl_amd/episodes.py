@@ -96,37 +96,35 @@ def _bytes(n, dev):
 
 def _recurrence_forward(x, gate, ep_off, h0, gate_value, reverse, want_last, want_states):
     lib, dev = _lib.load(), x.device
-    with _seq.running_on(dev):
-        a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        last = torch.empty(a.E, a.D, dtype=x.dtype, device=dev) if want_last else None
-        sizes = (a.N, a.D, a.E, a.type, a.gate_kind)
-        states = _bytes(lib.dcarl_recurrence_states_bytes(*sizes), dev) if want_states else None
-        ws = _bytes(lib.dcarl_recurrence_workspace_bytes(*sizes), dev)
-        _lib.check(lib.dcarl_recurrence_forward(C.byref(a), _lib.ptr(states), _lib.ptr(ws), _lib.ptr(h), _lib.ptr(last), _lib.stream_ptr()),
-                   "dcarl_recurrence_forward")
+    a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    last = torch.empty(a.E, a.D, dtype=x.dtype, device=dev) if want_last else None
+    sizes = (a.N, a.D, a.E, a.type, a.gate_kind)
+    states = _bytes(lib.dcarl_recurrence_states_bytes(*sizes), dev) if want_states else None
+    ws = _bytes(lib.dcarl_recurrence_workspace_bytes(*sizes), dev)
+    _lib.check(lib.dcarl_recurrence_forward(C.byref(a), _seq.at(states), _seq.at(ws), _seq.at(h), _seq.at(last), _seq.stream(dev)),
+               "dcarl_recurrence_forward")
     return h, last, states
 
 
 def _recurrence_backward(x, gate, ep_off, h0, gate_value, reverse, states, dh, dlast, want):
     lib, dev = _lib.load(), x.device
-    with _seq.running_on(dev):
-        a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
-        dh, lddh = _seq.rows_of(dh)
-        dlast = None if dlast is None else dlast.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
-        dgate = torch.empty(gate.shape, dtype=x.dtype, device=dev) if want[1] else None
-        dh0 = torch.empty(h0.shape, dtype=x.dtype, device=dev) if want[2] else None
-        ws = _bytes(lib.dcarl_recurrence_workspace_bytes(a.N, a.D, a.E, a.type, a.gate_kind), dev)
-        _lib.check(lib.dcarl_recurrence_backward(C.byref(a), _lib.ptr(states), _lib.ptr(ws), _lib.ptr(dh), lddh, _lib.ptr(dlast), _lib.ptr(dx),
-                                                 _lib.ptr(dgate), _lib.ptr(dh0), _lib.stream_ptr()), "dcarl_recurrence_backward")
+    a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
+    dh, lddh = _seq.rows_of(dh)
+    dlast = None if dlast is None else dlast.contiguous()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+    dgate = torch.empty(gate.shape, dtype=x.dtype, device=dev) if want[1] else None
+    dh0 = torch.empty(h0.shape, dtype=x.dtype, device=dev) if want[2] else None
+    ws = _bytes(lib.dcarl_recurrence_workspace_bytes(a.N, a.D, a.E, a.type, a.gate_kind), dev)
+    _lib.check(lib.dcarl_recurrence_backward(C.byref(a), _seq.at(states), _seq.at(ws), _seq.at(dh), lddh, _seq.at(dlast), _seq.at(dx),
+                                             _seq.at(dgate), _seq.at(dh0), _seq.stream(dev)), "dcarl_recurrence_backward")
     return dx, dgate, dh0
 
 
 class _Recurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, h0, ep_off, gate_value, reverse, want_last):
-        h, last, states = _recurrence_forward(x, gate, ep_off, h0, gate_value, reverse, want_last, any(ctx.needs_input_grad))
+        h, last, states = _seq.run_on(x.device, _recurrence_forward, x, gate, ep_off, h0, gate_value, reverse, want_last, True)
         ctx.save_for_backward(x, gate, h0, ep_off, states)
         ctx.rest = gate_value, reverse
         return (h, last) if want_last else h
@@ -136,7 +134,7 @@ class _Recurrence(torch.autograd.Function):
     def backward(ctx, dh, dlast=None):
         x, gate, h0, ep_off, states = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dgate, dh0 = _recurrence_backward(x, gate, ep_off, h0, *ctx.rest, states, dh, dlast, need[:3])
+        dx, dgate, dh0 = _seq.run_on(x.device, _recurrence_backward, x, gate, ep_off, h0, *ctx.rest, states, dh, dlast, need[:3])
         return dx, dgate, dh0, None, None, None, None
 
 
@@ -184,7 +182,11 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
         x, h0 = x.unsqueeze(1), None if h0 is None else h0.unsqueeze(1)
     if gate is not None and gate.dim() == 1 and x.shape[1] == 1:
         gate = gate.unsqueeze(1)                              # one channel: shared or not is the same
-    out = _Recurrence.apply(x, gate, h0, off, value, bool(reverse), bool(want_last))
+    if _seq.wants_gradient(x, gate, h0):
+        out = _Recurrence.apply(x, gate, h0, off, value, bool(reverse), bool(want_last))
+    else:
+        h, last, _ = _seq.run_on(dev, _recurrence_forward, x, gate, off, h0, value, bool(reverse), bool(want_last), False)
+        out = (h, last) if want_last else h
     if flat:
         out = tuple(o.squeeze(1) for o in out) if want_last else out.squeeze(1)
     return out

@@ -21,26 +21,24 @@ def _check_ids(ids, n_rows: int, validate: bool):
 
 
 def _gather(table, ids, scale):
-    lib = _lib.load()
-    with _seq.running_on(table.device):
-        t, ld = _seq.rows_of(table)
-        D = t.shape[1]
-        out = torch.empty(*ids.shape, D, dtype=t.dtype, device=t.device)
-        _lib.check(lib.dcarl_rows_gather(_lib.ptr(t), _seq.TYPES[t.dtype], ld, t.shape[0], _lib.ptr(ids), ids.element_size(), ids.numel(), D,
-                                         scale, _lib.ptr(out), _lib.stream_ptr()), "dcarl_rows_gather")
+    dev = table.device
+    t, ld = _seq.rows_of(table)
+    S, D = t.shape
+    out = torch.empty(*ids.shape, D, dtype=t.dtype, device=dev)
+    _lib.check(_lib.load().dcarl_rows_gather(_seq.at(t), _seq.TYPES[t.dtype], ld, S, _seq.at(ids), ids.element_size(), ids.numel(), D, scale,
+                                             _seq.at(out), _seq.stream(dev)), "dcarl_rows_gather")
     return out
 
 
 def _gradient(dout, ids, n_rows, scale):
-    lib = _lib.load()
-    with _seq.running_on(dout.device):
-        N, D = ids.numel(), dout.shape[-1]
-        d, ldd = _seq.rows_of(dout.reshape(N, D))
-        code = _seq.TYPES[d.dtype]
-        grad = torch.empty(n_rows, D, dtype=d.dtype, device=d.device)
-        ws = torch.empty(max(lib.dcarl_rows_workspace_bytes(N, n_rows, D, code), 16), dtype=torch.uint8, device=d.device)
-        _lib.check(lib.dcarl_rows_gradient(_lib.ptr(d), code, ldd, _lib.ptr(ids), ids.element_size(), N, D, n_rows, scale, _lib.ptr(ws),
-                                           _lib.ptr(grad), _lib.stream_ptr()), "dcarl_rows_gradient")
+    lib, dev = _lib.load(), dout.device
+    N, D = ids.numel(), dout.shape[-1]
+    d, ldd = _seq.rows_of(dout if dout.dim() == 2 else dout.reshape(N, D))
+    code = _seq.TYPES[d.dtype]
+    grad = torch.empty(n_rows, D, dtype=d.dtype, device=dev)
+    ws = torch.empty(max(lib.dcarl_rows_workspace_bytes(N, n_rows, D, code), 16), dtype=torch.uint8, device=dev)
+    _lib.check(lib.dcarl_rows_gradient(_seq.at(d), code, ldd, _seq.at(ids), ids.element_size(), N, D, n_rows, scale, _seq.at(ws), _seq.at(grad),
+                                       _seq.stream(dev)), "dcarl_rows_gradient")
     return grad
 
 
@@ -49,12 +47,12 @@ class _Lookup(torch.autograd.Function):
     def forward(ctx, table, ids, scale):
         ctx.save_for_backward(ids)
         ctx.rest = table.shape[0], scale
-        return _gather(table, ids, scale)
+        return _seq.run_on(table.device, _gather, table, ids, scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        return _gradient(dout, ctx.saved_tensors[0], *ctx.rest), None, None
+        return _seq.run_on(dout.device, _gradient, dout, ctx.saved_tensors[0], *ctx.rest), None, None
 
 
 def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
@@ -73,7 +71,9 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
         if _seq.capturing():
             raise ValueError("ids must lie on the GPU while a graph is captured")
         ids = ids.to(dev)
-    return _Lookup.apply(table, ids, float(scale))
+    if _seq.wants_gradient(table):
+        return _Lookup.apply(table, ids, float(scale))
+    return _seq.run_on(dev, _gather, table, ids, float(scale))
 
 
 def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: bool = True):
@@ -90,4 +90,4 @@ def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: boo
         if _seq.capturing():
             raise ValueError("ids must lie on the GPU while a graph is captured")
         ids = ids.to(dev)
-    return _gradient(dout, ids, n_rows, float(scale))
+    return _seq.run_on(dev, _gradient, dout, ids, n_rows, float(scale))
