@@ -1047,7 +1047,7 @@ int32_t dcarl_index_states_f64(const double* obs, int64_t N, int32_t D, const do
 
 // ---- sequence operators ------------------------------------------------------------------------------------------------
 constexpr int64_t SEQ_MAX = (int64_t)1 << 31;          // steps, channels, episodes, rows, ids of one call
-constexpr int64_t SEQ_MAX_ELEMENTS = (int64_t)1 << 46; // of one operand: byte offsets stay far inside 63 bits
+constexpr int64_t SEQ_MAX_ELEMENTS = (int64_t)1 << 40; // of one operand: a launch's workgroups stay below 2^31
 
 static int check_seq(const char* who, int32_t type, int64_t n, int64_t d, int64_t e) {
     if (type < DCARL_F64 || type > DCARL_F16) return fail(DCARL_EINVAL, "%s: type=%d is none of DCARL_F64/F32/BF16/F16", who, type);

@@ -7,10 +7,8 @@ namespace dcarl {
 template <typename T> void rec_launch_backward(const RecWalk<T>& a, int gate_kind, const RecPlan& p, hipStream_t st) {
     rec_with_shape<T>(a.D, [&](auto C, auto V) {
         auto go = [&](auto GK) {
-            if (p.P > 1)
-                hipLaunchKernelGGL((rec_backward_kernel<T, C(), V(), GK(), true>), dim3(p.blocks, p.P), dim3(REC_THREADS), 0, st, a);
-            const unsigned empty = rec_empty_blocks(a.dh0, a.E);
-            hipLaunchKernelGGL((rec_backward_kernel<T, C(), V(), GK(), false>), dim3(p.blocks, p.P + empty), dim3(REC_THREADS), 0, st, a);
+            const dim3 grid((unsigned)(p.tiles * p.blocks + rec_empty_blocks(a.dh0, a.E)));
+            if (grid.x) hipLaunchKernelGGL((rec_backward_kernel<T, C(), V(), GK()>), grid, dim3(REC_THREADS), 0, st, a);
         };
         if (gate_kind == 2) go(std::integral_constant<int, 2>{});
         else go(std::integral_constant<int, 1>{});

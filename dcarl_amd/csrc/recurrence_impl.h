@@ -4,21 +4,23 @@
 // A step is the affine map s -> g s + x; the composition of consecutive steps is one again, (A, B) with A the product of the gates, so
 // the time axis can be cut anywhere.  Three levels:
 //   * a thread walks K consecutive steps of VEC channels held in registers; the 64 / C groups of a wavefront and the four wavefronts of a
-//     workgroup hold consecutive segments, so a workgroup takes a tile of 4 * (64 / C) * K steps of C * VEC channels at a time: the
-//     segments' maps are composed by shuffles and through LDS (one barrier per tile), then each thread walks its steps once more
-//     from the state that reaches it.  x and g are read once; the next tile is in flight meanwhile.
-//   * a workgroup walks its part of the time axis tile by tile, the state in registers.
-//   * where channels alone do not fill the GPU the axis is cut into parts; a first launch composes the maps of the parts whose last episode
-//     goes on in the next one (from that episode's start: the others end early), and a part folds those of the parts before it.  The cuts
-//     are moved to the nearest episode start within a quarter of a part, which spares that reading where episodes are short.
+//     workgroup hold consecutive segments, so a workgroup takes one tile of 4 * (64 / C) * K steps of C * VEC channels;
+//   * the segments' maps are composed by shuffles and through LDS, then each thread walks its steps once more from the state that reaches it;
+//   * the state that reaches a tile: every tile publishes its own map as soon as it has it, and takes those of the tiles before it back to its
+//     episode's start, or to the start of its group of REC_GROUP tiles and from there the state that the last tile of the group before has
+//     published.  So the tiles wait for one another in a chain, of one link per group, and x and g are read once.
+// The waits end: a workgroup takes its tile by a ticket, in time order, so whatever it waits for belongs to workgroups that run already and
+// publish their maps without waiting; a wait that takes REC_POLLS polls all the same gives up with NaN.  A published word is its own flag: the
+// words are cleared to a pattern before the launch that no result has (rec_word), written and polled by relaxed atomics of device scope, and
+// nothing else passes between workgroups, so no fence is needed.
 // An episode's start is a flag, never a gate of zero: what lies before it is dropped, so a NaN there stays there.
-// All compositions happen in a fixed order: run-to-run identical.
+// All compositions happen in a fixed order, whoever comes first: run-to-run identical.
 #pragma once
 #include "seq_common.h"
 
 namespace dcarl {
 
-constexpr int REC_THREADS = 256, REC_WAVES = 4, REC_MAX_PARTS = 256;
+constexpr int REC_THREADS = 256, REC_WAVES = 4, REC_GROUP = 16, REC_POLLS = 1 << 20;
 constexpr int REC_START = 1, REC_END = 2, REC_OUT = 4;     // of a step, in walking order; OUT: behind the last episode
 
 // everything in walking order: step r of the walk is step r, or N - 1 - r for `reverse` (base addresses and strides say so)
@@ -26,15 +28,17 @@ template <typename T> struct RecWalk {
     using Acc = typename SeqType<T>::Acc;
     int64_t N, D, E;
     const int64_t* ep_off;
-    int reverse, P;
+    int reverse;
+    int64_t tiles, blocks;     // tiles along the time axis, blocks of channels
     const T *x, *g, *h0;
     int64_t sx, sg, ldh0;
     Acc gval;
     const uint8_t* flag;       // [N]
     const int32_t* ep;         // [N]
-    const int64_t* part;       // [P + 1]
-    Acc* agg;                  // [P][2][D]: the maps of the parts
-    Acc* state;                // [slots][D]: the state before each tile (nullable in the forward pass)
+    uint32_t* ticket;
+    Acc* map;                  // [tiles][D][2]: the published maps
+    Acc* through;              // [tiles / REC_GROUP + 1][D]: the published states between groups
+    Acc* state;                // [tiles][D]: the state before each tile (nullable in the forward pass)
     T* h; int64_t sh;          // forward: the result
     T* last;
     const T *dh, *dlast; int64_t sdh;
@@ -42,8 +46,8 @@ template <typename T> struct RecWalk {
     Acc* dgp;                  // shared gate: [channel blocks][N] partial sums, or null: one block, straight to dg
 };
 
-// K consecutive steps (16-byte loads of f32, 8-byte ones of 16-bit types; registers allow twice the steps of the narrow types)
-template <typename T> constexpr int REC_K = sizeof(T) == 2 ? 8 : 4;
+// K consecutive steps of VEC channels per thread (16-byte loads of f32, 8-byte ones of 16-bit types)
+template <typename T> constexpr int REC_K = sizeof(T) == 8 ? 4 : 8;
 template <typename T> constexpr int REC_VEC = sizeof(T) == 8 ? 2 : 4;
 
 template <typename T, int VEC> struct RecRaw { T v[VEC]; };
@@ -232,256 +236,276 @@ __device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecT
 
 template <int C, typename T> constexpr int REC_TILE = REC_WAVES * (64 / C) * REC_K<T>;
 
-template <typename T, int C, int VEC, int GK, bool AGG>
+// ---- between workgroups -----------------------------------------------------------------------------------------------------------------
+// a published value as a word that is never the cleared pattern (all ones, a NaN): every NaN is published as the quiet one
+__device__ __forceinline__ uint32_t rec_word(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v); }
+__device__ __forceinline__ uint64_t rec_word(double v) { return v != v ? 0x7ff8000000000000ull : (uint64_t)__double_as_longlong(v); }
+template <typename W> __device__ __forceinline__ void rec_put(W* p, W w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename W> __device__ __forceinline__ W rec_poll(const W* p) {
+    W w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = 0; w == (W)~(W)0 && i < REC_POLLS; ++i) {
+        __builtin_amdgcn_s_sleep(1);
+        w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    return w;                                              // given up: all ones, a NaN
+}
+// a map of f32 is one 8-byte word, one of f64 two
+__device__ __forceinline__ void rec_put_map(float* p, float A, float B) {
+    rec_put(reinterpret_cast<uint64_t*>(p), (uint64_t)rec_word(B) << 32 | rec_word(A));
+}
+__device__ __forceinline__ void rec_put_map(double* p, double A, double B) {
+    rec_put(reinterpret_cast<uint64_t*>(p), rec_word(A));
+    rec_put(reinterpret_cast<uint64_t*>(p) + 1, rec_word(B));
+}
+__device__ __forceinline__ void rec_get_map(const float* p, float& A, float& B) {
+    const uint64_t w = rec_poll(reinterpret_cast<const uint64_t*>(p));
+    A = __uint_as_float((uint32_t)w); B = __uint_as_float((uint32_t)(w >> 32));
+}
+__device__ __forceinline__ void rec_get_map(const double* p, double& A, double& B) {
+    A = __longlong_as_double((long long)rec_poll(reinterpret_cast<const uint64_t*>(p)));
+    B = __longlong_as_double((long long)rec_poll(reinterpret_cast<const uint64_t*>(p) + 1));
+}
+__device__ __forceinline__ void rec_put_state(float* p, float v) { rec_put(reinterpret_cast<uint32_t*>(p), rec_word(v)); }
+__device__ __forceinline__ void rec_put_state(double* p, double v) { rec_put(reinterpret_cast<uint64_t*>(p), rec_word(v)); }
+__device__ __forceinline__ float rec_get_state(const float* p) { return __uint_as_float(rec_poll(reinterpret_cast<const uint32_t*>(p))); }
+__device__ __forceinline__ double rec_get_state(const double* p) { return __longlong_as_double((long long)rec_poll(reinterpret_cast<const uint64_t*>(p))); }
+
+// the tile's own number in time order; one tile needs no order
+template <typename T> __device__ __forceinline__ int64_t rec_ticket(const RecWalk<T>& a) {
+    if (a.tiles <= 1) return blockIdx.x;
+    __shared__ uint32_t mine;
+    if (threadIdx.x == 0) mine = atomicAdd(a.ticket, 1u);
+    __syncthreads();
+    return mine;
+}
+
+// the whole tile's map, from the wavefronts' totals
+template <typename Acc, int C, int VEC, int DIR>
+__device__ __forceinline__ RecMap<Acc, VEC> rec_total(const RecShare<Acc, C, VEC>& sh, int c) {
+    RecMap<Acc, VEC> t;
+    t.one();
+#pragma unroll
+    for (int i = 0; i < REC_WAVES; ++i) {
+        const int w = DIR > 0 ? i : REC_WAVES - 1 - i;
+        RecMap<Acc, VEC> m;
+        m.cut = sh.cut[w] != 0;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) { m.A[v] = sh.A[w][c * VEC + v]; m.B[v] = sh.B[w][c * VEC + v]; }
+        m.after(t);
+        t = m;
+    }
+    return t;
+}
+
+// What reaches `tile` of an episode that comes in from the tile `from` (DIR > 0: an earlier one; < 0: a later one).  The thread group j takes the map
+// of tile j of the group, as if it were a segment of its own, and the maps are joined as segments are; `from` itself passes on its B alone.
+template <typename T, int C, int VEC, int DIR>
+__device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int64_t from, int64_t cb, int lane, int wv,
+                                          RecShare<typename SeqType<T>::Acc, C, VEC>& sh, typename SeqType<T>::Acc (&carry)[VEC]) {
+    using Acc = typename SeqType<T>::Acc;
+    const int64_t group = tile / REC_GROUP;
+    const int j = wv * (64 / C) + lane / C;
+    const int64_t src = group * REC_GROUP + j;
+    RecMap<Acc, VEC> m;
+    m.one();
+    if (j < REC_GROUP && (DIR > 0 ? src < tile && src >= from : src > tile && src <= from)) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) rec_get_map(a.map + (src * a.D + cb + v) * 2, m.A[v], m.B[v]);
+        m.cut = src == from;
+    }
+    const bool outside = DIR > 0 ? from < group * REC_GROUP : from >= (group + 1) * REC_GROUP;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) carry[v] = outside ? rec_get_state(a.through + (DIR > 0 ? group : group + 1) * a.D + cb + v) : Acc(0);
+    rec_scan_wave<Acc, C, VEC, DIR>(m, sh, lane, wv);
+    __syncthreads();
+    const RecMap<Acc, VEC> t = rec_total<Acc, C, VEC, DIR>(sh, lane % C);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) carry[v] = t.cut ? t.B[v] : fma(t.A[v], carry[v], t.B[v]);
+}
+
+template <typename T, int C, int VEC, int GK>
 __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
-    __shared__ RecShare<Acc, C, VEC> share[2];
+    __shared__ RecShare<Acc, C, VEC> share, reach;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
-    const int64_t c0 = ((int64_t)blockIdx.x * C + c) * VEC;
-    const bool mine = c0 < a.D;
-    const int64_t cb = c0 < a.D - VEC ? c0 : a.D - VEC;    // the last lanes move back to whole vectors: the same channels, the same values
-    if (!AGG && (int)blockIdx.y >= a.P) {                  // the states that empty episodes end with
-        const int64_t step = (int64_t)(gridDim.y - a.P) * REC_WAVES * (64 / C);
-        for (int64_t e = (((int64_t)blockIdx.y - a.P) * REC_WAVES + wv) * (64 / C) + lane / C; e < a.E; e += step)
-            if (rec_ep_begin(a.ep_off, e, a.reverse, a.N) >= rec_ep_end(a.ep_off, e, a.reverse, a.N) && mine)
-                for (int v = 0; v < VEC; ++v) a.last[e * a.D + cb + v] = a.h0 ? a.h0[e * a.ldh0 + cb + v] : narrow<T>(0.0f);
+    const int64_t ticket = rec_ticket(a), tile = ticket / a.blocks, blk = ticket - tile * a.blocks;
+    if (tile >= a.tiles) {                                 // the states that empty episodes end with
+        const int64_t groups = REC_THREADS / 64, first = (ticket - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
+        for (int64_t e = first; e < a.E; e += step)
+            if (rec_ep_begin(a.ep_off, e, a.reverse, a.N) >= rec_ep_end(a.ep_off, e, a.reverse, a.N))
+                for (int64_t d = lane; d < a.D; d += 64) a.last[e * a.D + d] = a.h0 ? a.h0[e * a.ldh0 + d] : narrow<T>(0.0f);
         return;
     }
-    const int p = blockIdx.y;
-    int64_t row0 = a.part[p];
-    const int64_t row1 = a.part[p + 1];
-    if (row0 >= row1) return;
-    int64_t slot = row0 / TILE + p;
-    Acc carry[VEC];
-    RecMap<Acc, VEC> whole;
-    if constexpr (AGG) {
-        if (row1 >= a.N || (a.flag[row1] & (REC_START | REC_OUT))) return;         // no episode goes on behind this part
-        const int64_t s = rec_ep_begin(a.ep_off, a.ep[row1], a.reverse, a.N);
-        row0 = s > row0 && s < row1 ? s : row0;
-        whole.one();
-    } else {
+    const int64_t c0 = (blk * C + c) * VEC;
+    const bool mine = c0 < a.D;
+    const int64_t cb = c0 < a.D - VEC ? c0 : a.D - VEC;    // the last lanes move back to whole vectors: the same channels, the same values
+    const int64_t row0 = tile * TILE, row1 = row0 + TILE < a.N ? row0 + TILE : a.N;
+    const int64_t r0 = row0 + (int64_t)(wv * (64 / C) + lane / C) * K;
+    RecTile<T, C, VEC, GK, false> t;
+    t.load(a, r0, row1, cb, true);
+    RecMap<Acc, VEC> m;
+    rec_map_forward(a, t, r0, cb, m);
+    rec_scan_wave<Acc, C, VEC, 1>(m, share, lane, wv);
+    __syncthreads();
+    const bool first = wv == 0 && lane < C && mine;        // the threads that publish
+    Acc carry[VEC], s[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) carry[v] = 0;
-        if (p > 0 && !(a.flag[row0] & (REC_START | REC_OUT))) {
-            const int64_t s = rec_ep_begin(a.ep_off, a.ep[row0], a.reverse, a.N);
-            int q = p - 1;
-            while (q > 0 && a.part[q] > s) --q;
-            for (bool first = true; q < p; ++q, first = false) {
-                if (a.part[q] >= a.part[q + 1]) continue;
-                const Acc* m = a.agg + (int64_t)q * 2 * a.D + cb;
+    for (int v = 0; v < VEC; ++v) carry[v] = 0;
+    if (a.tiles > 1) {
+        const RecMap<Acc, VEC> total = rec_total<Acc, C, VEC, 1>(share, c);
+        if (first && tile + 1 < a.tiles)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) carry[v] = first ? m[a.D + v] : fma(m[v], carry[v], m[a.D + v]);
+            for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
+        if (tile > 0 && !(a.flag[row0] & (REC_START | REC_OUT))) {
+            const int64_t from = rec_ep_begin(a.ep_off, a.ep[row0], a.reverse, a.N) / TILE;
+            rec_reach<T, C, VEC, 1>(a, tile, from < tile ? from : tile - 1, cb, lane, wv, reach, carry);
+        }
+        if (first && tile % REC_GROUP == REC_GROUP - 1 && tile + 1 < a.tiles)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                rec_put_state(a.through + (tile / REC_GROUP + 1) * a.D + cb + v, total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
+    }
+    if (a.state && first)
+        for (int v = 0; v < VEC; ++v) a.state[tile * a.D + cb + v] = carry[v];
+    rec_carry<Acc, C, VEC, 1>(m, share, lane, wv, carry, s);
+    const bool plain = __all(t.fl == 0 && t.n == K);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (!plain) {
+            if (k >= t.n) continue;
+            if (t.flag(k) & REC_START) {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[a.ep[r0 + k] * a.ldh0 + cb + v]) : Acc(0);
             }
         }
-    }
-    const int64_t seg = (int64_t)(wv * (64 / C) + lane / C) * K;
-    RecTile<T, C, VEC, GK, false> t, next;
-    t.load(a, row0 + seg, row1, cb, true);
-    int buf = 0;
-    for (int64_t base = row0; base < row1; base += TILE, buf ^= 1, ++slot) {
-        if (base + TILE < row1) next.load(a, base + TILE + seg, row1, cb, true);
-        const int64_t r0 = base + seg;
-        RecMap<Acc, VEC> m;
-        rec_map_forward(a, t, r0, cb, m);
-        rec_scan_wave<Acc, C, VEC, 1>(m, share[buf], lane, wv);
-        __syncthreads();
-        if constexpr (AGG) {
+        RecRaw<T, VEC> o;
 #pragma unroll
-            for (int w = 0; w < REC_WAVES; ++w) {
-                RecMap<Acc, VEC> f = whole;
-                whole.cut = share[buf].cut[w] != 0;
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) { whole.A[v] = share[buf].A[w][c * VEC + v]; whole.B[v] = share[buf].B[w][c * VEC + v]; }
-                whole.after(f);
-            }
-        } else {
-            Acc s[VEC];
-            if (a.state && mine && wv == 0 && lane < C)
-                for (int v = 0; v < VEC; ++v) a.state[slot * a.D + cb + v] = carry[v];
-            rec_carry<Acc, C, VEC, 1>(m, share[buf], lane, wv, carry, s);
-            const bool plain = __all(t.fl == 0 && t.n == K);
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (!plain) {
-                    if (k >= t.n) continue;
-                    const int f = t.flag(k);
-                    if (f & REC_START) {
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[a.ep[r0 + k] * a.ldh0 + cb + v]) : Acc(0);
-                    }
-                }
-                RecRaw<T, VEC> o;
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    s[v] = fma(t.gate(a, k, v), s[v], (Acc)widen(t.x[k].v[v]));
-                    o.v[v] = narrow<T>(s[v]);
-                }
-                if (!plain && (t.flag(k) & REC_OUT)) {
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) { s[v] = 0; o.v[v] = narrow<T>(0.0f); }
-                }
-                if (mine) {
-                    __builtin_memcpy(a.h + (r0 + k) * a.sh + cb, &o, sizeof(o));
-                    if (a.last && !plain && (t.flag(k) & REC_END)) __builtin_memcpy(a.last + a.ep[r0 + k] * a.D + cb, &o, sizeof(o));
-                }
-            }
+        for (int v = 0; v < VEC; ++v) {
+            s[v] = fma(t.gate(a, k, v), s[v], (Acc)widen(t.x[k].v[v]));
+            o.v[v] = narrow<T>(s[v]);
         }
-        t = next;
-    }
-    if constexpr (AGG) {
-        if (mine && wv == 0 && lane < C)
-            for (int v = 0; v < VEC; ++v) {
-                a.agg[(int64_t)p * 2 * a.D + cb + v] = whole.A[v];
-                a.agg[((int64_t)p * 2 + 1) * a.D + cb + v] = whole.B[v];
-            }
+        if (!plain && (t.flag(k) & REC_OUT)) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) { s[v] = 0; o.v[v] = narrow<T>(0.0f); }
+        }
+        if (mine) {
+            __builtin_memcpy(a.h + (r0 + k) * a.sh + cb, &o, sizeof(o));
+            if (a.last && !plain && (t.flag(k) & REC_END)) __builtin_memcpy(a.last + a.ep[r0 + k] * a.D + cb, &o, sizeof(o));
+        }
     }
 }
 
-template <typename T, int C, int VEC, int GK, bool AGG>
+template <typename T, int C, int VEC, int GK>
 __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
-    __shared__ RecShare<Acc, C, VEC> share_b[2], share_f[2];
+    __shared__ RecShare<Acc, C, VEC> share_b, share_f, reach;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
-    const int64_t c0 = ((int64_t)blockIdx.x * C + c) * VEC;
-    const bool mine = c0 < a.D;
-    const int64_t cb = c0 < a.D - VEC ? c0 : a.D - VEC;
-    if (!AGG && (int)blockIdx.y >= a.P) {                  // an empty episode hands its dlast through
-        const int64_t step = (int64_t)(gridDim.y - a.P) * REC_WAVES * (64 / C);
-        for (int64_t e = (((int64_t)blockIdx.y - a.P) * REC_WAVES + wv) * (64 / C) + lane / C; e < a.E; e += step)
-            if (rec_ep_begin(a.ep_off, e, a.reverse, a.N) >= rec_ep_end(a.ep_off, e, a.reverse, a.N) && mine)
-                for (int v = 0; v < VEC; ++v) a.dh0[e * a.D + cb + v] = a.dlast ? a.dlast[e * a.D + cb + v] : narrow<T>(0.0f);
+    const int64_t ticket = rec_ticket(a), order = ticket / a.blocks, blk = ticket - order * a.blocks;
+    if (order >= a.tiles) {                                // an empty episode hands its dlast through
+        const int64_t groups = REC_THREADS / 64, first = (ticket - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
+        for (int64_t e = first; e < a.E; e += step)
+            if (rec_ep_begin(a.ep_off, e, a.reverse, a.N) >= rec_ep_end(a.ep_off, e, a.reverse, a.N))
+                for (int64_t d = lane; d < a.D; d += 64) a.dh0[e * a.D + d] = a.dlast ? a.dlast[e * a.D + d] : narrow<T>(0.0f);
         return;
     }
-    const int p = blockIdx.y;
-    const int64_t row0 = a.part[p];
-    int64_t row1 = a.part[p + 1];
-    if (row0 >= row1) return;
-    Acc carry[VEC];
-    RecMap<Acc, VEC> whole;
-    if constexpr (AGG) {
-        if (row0 == 0 || (a.flag[row0 - 1] & (REC_END | REC_OUT))) return;          // no episode comes in from before this part
-        const int64_t e = rec_ep_end(a.ep_off, a.ep[row0 - 1], a.reverse, a.N);
-        row1 = e < row1 && e > row0 ? e : row1;
-        whole.one();
-    } else {
+    const int64_t tile = a.tiles - 1 - order;              // from the end of time
+    const int64_t c0 = (blk * C + c) * VEC;
+    const bool mine = c0 < a.D;
+    const int64_t cb = c0 < a.D - VEC ? c0 : a.D - VEC;
+    const int64_t row0 = tile * TILE, row1 = row0 + TILE < a.N ? row0 + TILE : a.N;
+    const int64_t r0 = row0 + (int64_t)(wv * (64 / C) + lane / C) * K;
+    RecTile<T, C, VEC, GK, true> t;
+    t.load(a, r0, row1, cb, true);
+    Acc state[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) carry[v] = 0;
+    for (int v = 0; v < VEC; ++v) state[v] = a.state[tile * a.D + cb + v];
+    RecMap<Acc, VEC> mb, mf;
+    rec_map_backward(a, t, r0, cb, mb);
+    rec_scan_wave<Acc, C, VEC, -1>(mb, share_b, lane, wv);
+    rec_map_forward(a, t, r0, cb, mf);
+    rec_scan_wave<Acc, C, VEC, 1>(mf, share_f, lane, wv);
+    __syncthreads();
+    const bool first = wv == 0 && lane < C && mine;
+    Acc carry[VEC], s[VEC], back[VEC], prev[K][VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) carry[v] = 0;
+    if (a.tiles > 1) {
+        const RecMap<Acc, VEC> total = rec_total<Acc, C, VEC, -1>(share_b, c);
+        if (first && tile > 0)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
         if (row1 < a.N && !(a.flag[row1 - 1] & (REC_END | REC_OUT))) {
-            const int64_t e = rec_ep_end(a.ep_off, a.ep[row1 - 1], a.reverse, a.N);       // one behind its last step
-            int q = p + 1;
-            while (q < a.P - 1 && a.part[q + 1] < e) ++q;
-            for (bool first = true; q > p; --q, first = false) {
-                if (a.part[q] >= a.part[q + 1]) continue;
-                const Acc* m = a.agg + (int64_t)q * 2 * a.D + cb;
+            const int64_t from = (rec_ep_end(a.ep_off, a.ep[row1 - 1], a.reverse, a.N) - 1) / TILE;
+            rec_reach<T, C, VEC, -1>(a, tile, from > tile ? from : tile + 1, cb, lane, wv, reach, carry);
+        }
+        if (first && tile % REC_GROUP == 0 && tile > 0)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) carry[v] = first ? m[a.D + v] : fma(m[v], carry[v], m[a.D + v]);
+            for (int v = 0; v < VEC; ++v)
+                rec_put_state(a.through + tile / REC_GROUP * a.D + cb + v, total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
+    }
+    rec_carry<Acc, C, VEC, -1>(mb, share_b, lane, wv, carry, back);
+    rec_carry<Acc, C, VEC, 1>(mf, share_f, lane, wv, state, s);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {                          // the states before each step once more, in 32 bits
+        if (k < t.n && (t.flag(k) & REC_START)) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[a.ep[r0 + k] * a.ldh0 + cb + v]) : Acc(0);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            prev[k][v] = s[v];
+            s[v] = fma(t.gate(a, k, v), s[v], (Acc)widen(t.x[k].v[v]));
+        }
+    }
+    Acc sum[K];
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k) {
+        sum[k] = 0;
+        if (k >= t.n) continue;
+        const int f = t.flag(k);
+        if (f & REC_END) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) back[v] = a.dlast ? (Acc)widen(a.dlast[a.ep[r0 + k] * a.D + cb + v]) : Acc(0);
+        }
+        RecRaw<T, VEC> ox, og;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const Acc d = widen(t.dh[k].v[v]) + back[v], term = d * prev[k][v];
+            ox.v[v] = narrow<T>(d);
+            og.v[v] = narrow<T>(term);
+            if (GK == 1 && cb + v >= c0 && !(f & REC_OUT)) sum[k] += term;       // a channel counts in one lane only
+            back[v] = t.gate(a, k, v) * d;
+        }
+        if (f & REC_OUT) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) { ox.v[v] = og.v[v] = narrow<T>(0.0f); back[v] = 0; }
+        }
+        if (mine) {
+            if (a.dx) __builtin_memcpy(a.dx + (r0 + k) * a.sh + cb, &ox, sizeof(ox));
+            if (GK == 2 && a.dg) __builtin_memcpy(a.dg + (r0 + k) * a.sh + cb, &og, sizeof(og));
+            if (a.dh0 && (f & REC_START)) {
+                RecRaw<T, VEC> o0;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) o0.v[v] = narrow<T>(back[v]);
+                __builtin_memcpy(a.dh0 + a.ep[r0 + k] * a.D + cb, &o0, sizeof(o0));
             }
         }
     }
-    const int64_t seg = (int64_t)(wv * (64 / C) + lane / C) * K;
-    int64_t tiles = (row1 - row0 + TILE - 1) / TILE;
-    int64_t base = row0 + (tiles - 1) * TILE, slot = row0 / TILE + p + tiles - 1;
-    RecTile<T, C, VEC, GK, true> t, next;
-    t.load(a, base + seg, row1, cb, !AGG);
-    int buf = 0;
-    for (; base >= row0; base -= TILE, buf ^= 1, --slot) {
-        if (base > row0) next.load(a, base - TILE + seg, row1, cb, !AGG);
-        const int64_t r0 = base + seg;
-        RecMap<Acc, VEC> mb, mf;
-        rec_map_backward(a, t, r0, cb, mb);
-        rec_scan_wave<Acc, C, VEC, -1>(mb, share_b[buf], lane, wv);
-        Acc state[VEC];
-        if constexpr (!AGG) {
+    if constexpr (GK == 1) {
+        if (a.dg) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) state[v] = a.state[slot * a.D + cb + v];
-            rec_map_forward(a, t, r0, cb, mf);
-            rec_scan_wave<Acc, C, VEC, 1>(mf, share_f[buf], lane, wv);
-        }
-        __syncthreads();
-        if constexpr (AGG) {
+            for (int k = 0; k < K; ++k) {
+                Acc v = mine ? sum[k] : Acc(0);
 #pragma unroll
-            for (int w = REC_WAVES - 1; w >= 0; --w) {
-                RecMap<Acc, VEC> f = whole;
-                whole.cut = share_b[buf].cut[w] != 0;
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) { whole.A[v] = share_b[buf].A[w][c * VEC + v]; whole.B[v] = share_b[buf].B[w][c * VEC + v]; }
-                whole.after(f);
-            }
-        } else {
-            Acc s[VEC], back[VEC], prev[K][VEC];
-            rec_carry<Acc, C, VEC, -1>(mb, share_b[buf], lane, wv, carry, back);
-            rec_carry<Acc, C, VEC, 1>(mf, share_f[buf], lane, wv, state, s);
-#pragma unroll
-            for (int k = 0; k < K; ++k) {                  // the states before each step once more, in 32 bits
-                if (k < t.n && (t.flag(k) & REC_START)) {
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[a.ep[r0 + k] * a.ldh0 + cb + v]) : Acc(0);
-                }
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    prev[k][v] = s[v];
-                    s[v] = fma(t.gate(a, k, v), s[v], (Acc)widen(t.x[k].v[v]));
-                }
-            }
-            Acc sum[K];
-#pragma unroll
-            for (int k = K - 1; k >= 0; --k) {
-                sum[k] = 0;
-                if (k >= t.n) continue;
-                const int f = t.flag(k);
-                if (f & REC_END) {
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) back[v] = a.dlast ? (Acc)widen(a.dlast[a.ep[r0 + k] * a.D + cb + v]) : Acc(0);
-                }
-                RecRaw<T, VEC> ox, og;
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const Acc d = widen(t.dh[k].v[v]) + back[v], term = d * prev[k][v];
-                    ox.v[v] = narrow<T>(d);
-                    og.v[v] = narrow<T>(term);
-                    if (GK == 1 && cb + v >= c0 && !(f & REC_OUT)) sum[k] += term;   // a channel counts in one lane only
-                    back[v] = t.gate(a, k, v) * d;
-                }
-                if (f & REC_OUT) {
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) { ox.v[v] = og.v[v] = narrow<T>(0.0f); back[v] = 0; }
-                }
-                if (mine) {
-                    if (a.dx) __builtin_memcpy(a.dx + (r0 + k) * a.sh + cb, &ox, sizeof(ox));
-                    if (GK == 2 && a.dg) __builtin_memcpy(a.dg + (r0 + k) * a.sh + cb, &og, sizeof(og));
-                    if (a.dh0 && (f & REC_START)) {
-                        RecRaw<T, VEC> o0;
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) o0.v[v] = narrow<T>(back[v]);
-                        __builtin_memcpy(a.dh0 + a.ep[r0 + k] * a.D + cb, &o0, sizeof(o0));
-                    }
-                }
-            }
-            if constexpr (GK == 1) {
-                if (a.dg) {
-#pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        Acc v = mine ? sum[k] : Acc(0);
-#pragma unroll
-                        for (int o = 1; o < C; o <<= 1) v += __shfl_xor(v, o);
-                        if (c == 0 && k < t.n) {
-                            if (a.dgp) a.dgp[(int64_t)blockIdx.x * a.N + r0 + k] = v;
-                            else a.dg[(r0 + k) * (a.reverse ? -1 : 1)] = narrow<T>(v);
-                        }
-                    }
+                for (int o = 1; o < C; o <<= 1) v += __shfl_xor(v, o);
+                if (c == 0 && k < t.n) {
+                    if (a.dgp) a.dgp[blk * a.N + r0 + k] = v;
+                    else a.dg[(r0 + k) * (a.reverse ? -1 : 1)] = narrow<T>(v);
                 }
             }
         }
-        t = next;
-    }
-    if constexpr (AGG) {
-        if (mine && wv == 0 && lane < C)
-            for (int v = 0; v < VEC; ++v) {
-                a.agg[(int64_t)p * 2 * a.D + cb + v] = whole.A[v];
-                a.agg[((int64_t)p * 2 + 1) * a.D + cb + v] = whole.B[v];
-            }
     }
 }
 
@@ -494,15 +518,16 @@ template <typename T, typename F> inline void rec_with_shape(int64_t D, F&& f) {
     else f(std::integral_constant<int, 16>{}, std::integral_constant<int, V>{});
 }
 
-// workgroups that look for empty episodes, beside those of the parts
+// workgroups that look for empty episodes, beside those of the tiles
 inline unsigned rec_empty_blocks(bool wanted, int64_t E) { return wanted ? (unsigned)((E + 1023) / 1024 < 1024 ? (E + 1023) / 1024 : 1024) : 0; }
 
 struct RecPlan {
-    int P, blocks, tile;
-    int64_t slots;
-    int64_t flag, ep, part, plan_bytes;                    // the walk: in the states where there are any, else in the workspace
+    int tile;
+    int64_t tiles, blocks;
+    int64_t flag, ep, plan_bytes;                          // the walk: in the states where there are any, else in the workspace
     int64_t state, states_bytes;
-    int64_t agg, dgp, ws_plan, ws_bytes;
+    int64_t ticket, map, through, clear_bytes;             // what passes between workgroups: cleared before each launch
+    int64_t dgp, ws_plan, ws_bytes;
 };
 RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind);
 
