@@ -56,11 +56,11 @@ def wants_gradient(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def rows_of(t: torch.Tensor):
+def rows_of(t: torch.Tensor, far: int = 1 << 62):
     """(tensor, elements between its rows) of a 2-D operand whose channels are contiguous; a copy where they are not.  Rows may lie
-    anywhere at a non-negative distance (slices, one row expanded to many)."""
+    anywhere at a non-negative distance (slices, one row expanded to many) of up to `far` elements, or of their own width."""
     step, one = t.stride()
-    if one != 1 and t.shape[1] > 1 or step < 0:
+    if one != 1 and t.shape[1] > 1 or step < 0 or step > far and step > t.shape[1]:
         t = t.contiguous()
         step = t.stride(0)
     return t, step

@@ -88,6 +88,7 @@ int launch_true_step(const uint8_t*, const int64_t*, const int32_t*, const int32
 int launch_census_table(const double*, int, int, const DevParams&, unsigned long long*, hipStream_t);
 template <typename T>
 int launch_census_trace(const T*, const uint8_t*, const int64_t*, const int32_t*, int, int, const DevParams&, unsigned long long*, hipStream_t);
+int64_t recurrence_max_ld(int64_t, int);
 int64_t recurrence_workspace_bytes(int64_t, int64_t, int64_t, int, int);
 int64_t recurrence_states_bytes(int64_t, int64_t, int64_t, int, int);
 void launch_recurrence_forward(const dcarl_recurrence_t&, void*, void*, void*, void*, hipStream_t);
@@ -1063,8 +1064,9 @@ static int check_recurrence(const char* who, const dcarl_recurrence_t* r) {
     if (!r) return fail(DCARL_EINVAL, "%s: arguments are NULL", who);
     if (int rc = check_seq(who, r->type, r->N, r->D, r->E)) return rc;
     if (r->gate_kind < 0 || r->gate_kind > 2) return fail(DCARL_EINVAL, "%s: gate_kind=%d outside [0,2]", who, r->gate_kind);
-    if (int rc = check_ld(who, "ldx", r->ldx)) return rc;
-    if (int rc = check_ld(who, "ldg", r->ldg)) return rc;
+    const int64_t far = r->D ? dcarl::recurrence_max_ld(r->D, r->type) : 0;
+    if (r->D > far || r->ldx < 0 || r->ldx > (r->D ? far : r->ldx) || r->ldg < 0 || r->ldg > (r->D ? far : r->ldg))
+        return fail(DCARL_EINVAL, "%s: D=%lld, ldx=%lld or ldg=%lld outside [0,%lld]", who, (long long)r->D, (long long)r->ldx, (long long)r->ldg, (long long)far);
     if (int rc = check_ld(who, "ldh0", r->ldh0)) return rc;
     if (r->E && !r->ep_off) return fail(DCARL_EINVAL, "%s: ep_off is NULL", who);
     if (r->N && r->D && (!r->x || (r->gate_kind && !r->gate))) return fail(DCARL_EINVAL, "%s: x / gate is NULL", who);
@@ -1095,7 +1097,7 @@ int32_t dcarl_recurrence_backward(const dcarl_recurrence_t* r, const void* state
                                   void* dx, void* dgate, void* dh0, void* stream) {
     const char* who = "dcarl_recurrence_backward";
     if (int rc = check_recurrence(who, r)) return rc;
-    if (int rc = check_ld(who, "lddh", lddh)) return rc;
+    if (lddh < 0 || (r->D && lddh > dcarl::recurrence_max_ld(r->D, r->type))) return fail(DCARL_EINVAL, "%s: lddh=%lld out of range", who, (long long)lddh);
     if (dgate && r->gate_kind == 0) return fail(DCARL_EINVAL, "%s: a gate that is a number has no gradient", who);
     if (r->D == 0 || (r->N == 0 && r->E == 0)) return DCARL_OK;
     if (r->N && (!dh || !states)) return fail(DCARL_EINVAL, "%s: dh / states is NULL", who);

@@ -4,12 +4,14 @@
 
 namespace dcarl {
 
-// flags and episode of every step of the walk
-__global__ __launch_bounds__(256) void rec_walk_kernel(const int64_t* off, int64_t E, int64_t N, int reverse, uint8_t* flag, int32_t* ep, uint32_t* ticket,
-                                                       uint4* clear, int64_t clear16) {
+// flags and episode of every step of the walk; where the episodes that cross a tile's borders begin and end
+__global__ __launch_bounds__(256) void rec_walk_kernel(const int64_t* off, int64_t E, int64_t N, int reverse, int tile, int64_t tiles, uint8_t* flag,
+                                                       int32_t* ep, int32_t* from, int32_t* till, uint32_t* ticket,
+                                                       int64_t blocks, uint4* clear, int64_t clear16) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r == 0) *ticket = 0;
-    for (int64_t i = r; i < clear16; i += (int64_t)gridDim.x * 256) clear[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+    const int64_t all = (int64_t)gridDim.x * 256;
+    for (int64_t i = r; i < blocks; i += all) ticket[i * REC_TICKET] = 0;
+    for (int64_t i = r; i < clear16; i += all) clear[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
     if (r >= N || !off) return;
     const int64_t t = reverse ? N - 1 - r : r;
     int64_t lo = 0, hi = E + 1;                            // the first offset above t
@@ -26,14 +28,24 @@ __global__ __launch_bounds__(256) void rec_walk_kernel(const int64_t* off, int64
     }
     flag[r] = (uint8_t)f;
     ep[r] = (int32_t)e;
+    // (held inside the walk whatever the offsets say: a tile waits for tiles between itself and these)
+    const int64_t at = r / tile, lr = r - at * tile;
+    if (lr == 0) {
+        int64_t b = out || (f & REC_START) || at == 0 ? -1 : rec_ep_begin(off, e, reverse, N) / tile;
+        from[at] = (int32_t)(b >= at ? at - 1 : b);
+    }
+    if (lr == tile - 1 || r == N - 1) {
+        int64_t z = out || (f & REC_END) || at + 1 == tiles ? -1 : (rec_ep_end(off, e, reverse, N) - 1) / tile;
+        till[at] = (int32_t)(z >= 0 && z <= at ? at + 1 : z);
+    }
 }
 
-template <typename T> __global__ __launch_bounds__(256) void rec_share_kernel(const typename SeqType<T>::Acc* dgp, int blocks, int64_t N, int step, T* dg) {
+template <typename T> __global__ __launch_bounds__(256) void rec_share_kernel(const typename SeqType<T>::Acc* dgp, int blocks, int64_t N, int reverse, T* dg) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (r >= N) return;
     typename SeqType<T>::Acc s = 0;
     for (int b = 0; b < blocks; ++b) s += dgp[b * N + r];
-    dg[r * step] = narrow<T>(s);
+    dg[reverse ? N - 1 - r : r] = narrow<T>(s);
 }
 
 static int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
@@ -51,7 +63,7 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
     p.tiles = (N + p.tile - 1) / p.tile;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t here = at; at += up16(bytes); return here; };
-    p.flag = take(N + 8); p.ep = take(4 * N);
+    p.flag = take(N + 8); p.ep = take(4 * N); p.from = take(4 * p.tiles); p.till = take(4 * p.tiles);
     p.plan_bytes = at;
     p.state = take(p.tiles * D * acc);
     p.states_bytes = at;
@@ -59,11 +71,15 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
     p.map = take(p.tiles > 1 ? 2 * p.tiles * D * acc : 0);
     p.through = take(p.tiles > 1 ? (p.tiles / REC_GROUP + 2) * D * acc : 0);
     p.clear_bytes = at;
-    p.ticket = take(16);
+    p.ticket = take(p.tiles > 1 ? 4 * REC_TICKET * p.blocks : 0);
     p.ws_plan = take(p.plan_bytes);
     p.dgp = take(gate_kind == 1 && p.blocks > 1 ? p.blocks * N * acc : 0);
     p.ws_bytes = at;
     return p;
+}
+// the largest row distance: a tile's rows are addressed by 32-bit offsets
+int64_t recurrence_max_ld(int64_t D, int type) {
+    return ((int64_t)1 << 31) / rec_plan(1, D, type, 2).tile / (type == DCARL_F64 ? 8 : type == DCARL_F32 ? 4 : 2);
 }
 int64_t recurrence_workspace_bytes(int64_t N, int64_t D, int64_t, int type, int gate_kind) { return D ? rec_plan(N, D, type, gate_kind).ws_bytes : 0; }
 int64_t recurrence_states_bytes(int64_t N, int64_t D, int64_t, int type, int gate_kind) { return D ? rec_plan(N, D, type, gate_kind).states_bytes : 0; }
@@ -72,9 +88,8 @@ template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, co
     using Acc = typename SeqType<T>::Acc;
     RecWalk<T> a{};
     a.N = r.N; a.D = r.D; a.E = r.E; a.ep_off = r.ep_off; a.reverse = r.reverse; a.tiles = p.tiles; a.blocks = p.blocks;
-    const int64_t top = r.reverse ? r.N - 1 : 0, dir = r.reverse ? -1 : 1;
-    a.x = static_cast<const T*>(r.x) + top * r.ldx; a.sx = dir * r.ldx;
-    a.g = r.gate_kind ? static_cast<const T*>(r.gate) + top * r.ldg : nullptr; a.sg = dir * r.ldg;
+    a.x = static_cast<const T*>(r.x); a.ldx = (uint32_t)r.ldx;
+    a.g = r.gate_kind ? static_cast<const T*>(r.gate) : nullptr; a.ldg = (uint32_t)r.ldg;
     a.h0 = static_cast<const T*>(r.h0); a.ldh0 = r.ldh0;
     a.gval = (Acc)r.gate_value;
     a.flag = reinterpret_cast<uint8_t*>(plan + p.flag);
@@ -82,7 +97,8 @@ template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, co
     a.ticket = reinterpret_cast<uint32_t*>(ws + p.ticket);
     a.map = reinterpret_cast<Acc*>(ws + p.map);
     a.through = reinterpret_cast<Acc*>(ws + p.through);
-    a.sh = dir * r.D;
+    a.from = reinterpret_cast<int32_t*>(plan + p.from);
+    a.till = reinterpret_cast<int32_t*>(plan + p.till);
     return a;
 }
 
@@ -99,9 +115,10 @@ template <typename T> void rec_launch_forward(const RecWalk<T>& a, int gate_kind
 
 // the walk (off given) and what the launch behind it needs cleared
 static void rec_launch_walk(const dcarl_recurrence_t& r, const RecPlan& p, const int64_t* off, char* plan, char* ws, hipStream_t st) {
-    hipLaunchKernelGGL(rec_walk_kernel, dim3((unsigned)(r.N / 256 + 1)), dim3(256), 0, st, off, r.E, r.N, r.reverse,
-                       reinterpret_cast<uint8_t*>(plan + p.flag), reinterpret_cast<int32_t*>(plan + p.ep), reinterpret_cast<uint32_t*>(ws + p.ticket),
-                       reinterpret_cast<uint4*>(ws), p.clear_bytes / 16);
+    hipLaunchKernelGGL(rec_walk_kernel, dim3((unsigned)(r.N / 256 + 1)), dim3(256), 0, st, off, r.E, r.N, r.reverse, p.tile, p.tiles,
+                       reinterpret_cast<uint8_t*>(plan + p.flag), reinterpret_cast<int32_t*>(plan + p.ep),
+                       reinterpret_cast<int32_t*>(plan + p.from), reinterpret_cast<int32_t*>(plan + p.till), reinterpret_cast<uint32_t*>(ws + p.ticket),
+                       p.tiles > 1 ? p.blocks : 0, reinterpret_cast<uint4*>(ws), p.clear_bytes / 16);
 }
 
 void launch_recurrence_forward(const dcarl_recurrence_t& r, void* states, void* workspace, void* h, void* last, hipStream_t st) {
@@ -112,7 +129,7 @@ void launch_recurrence_forward(const dcarl_recurrence_t& r, void* states, void* 
     with_type(r.type, [&](auto t) {
         using T = decltype(t);
         RecWalk<T> a = rec_walk<T>(r, p, plan, ws);
-        a.h = static_cast<T*>(h) + (r.reverse ? (r.N - 1) * r.D : 0);
+        a.h = static_cast<T*>(h);
         a.last = static_cast<T*>(last);
         if (states) a.state = reinterpret_cast<typename SeqType<T>::Acc*>(plan + p.state);
         rec_launch_forward<T>(a, r.gate_kind, p, st);
@@ -130,16 +147,15 @@ void launch_recurrence_backward(const dcarl_recurrence_t& r, const void* states,
         using Acc = typename SeqType<T>::Acc;
         RecWalk<T> a = rec_walk<T>(r, p, plan, ws);
         a.state = reinterpret_cast<Acc*>(plan + p.state);
-        const int64_t top = r.reverse ? r.N - 1 : 0;
-        a.dh = static_cast<const T*>(dh) + top * lddh; a.sdh = (r.reverse ? -1 : 1) * lddh;
+        a.dh = static_cast<const T*>(dh); a.lddh = (uint32_t)lddh;
         a.dlast = static_cast<const T*>(dlast);
-        a.dx = dx ? static_cast<T*>(dx) + top * r.D : nullptr;
-        a.dg = dgate ? static_cast<T*>(dgate) + top * (r.gate_kind == 2 ? r.D : 1) : nullptr;
+        a.dx = static_cast<T*>(dx);
+        a.dg = static_cast<T*>(dgate);
         a.dh0 = static_cast<T*>(dh0);
         a.dgp = r.gate_kind == 1 && p.blocks > 1 ? reinterpret_cast<Acc*>(ws + p.dgp) : nullptr;
         rec_launch_backward<T>(a, r.gate_kind, p, st);
         if (a.dgp && a.dg)
-            hipLaunchKernelGGL((rec_share_kernel<T>), dim3((unsigned)((r.N + 255) / 256)), dim3(256), 0, st, a.dgp, (int)p.blocks, r.N, r.reverse ? -1 : 1, a.dg);
+            hipLaunchKernelGGL((rec_share_kernel<T>), dim3((unsigned)((r.N + 255) / 256)), dim3(256), 0, st, a.dgp, (int)p.blocks, r.N, r.reverse, a.dg);
     });
 }
 

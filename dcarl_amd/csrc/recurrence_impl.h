@@ -20,29 +20,33 @@
 
 namespace dcarl {
 
-constexpr int REC_THREADS = 256, REC_WAVES = 4, REC_GROUP = 16, REC_POLLS = 1 << 20;
+constexpr int REC_THREADS = 256, REC_WAVES = 4, REC_GROUP = 16, REC_POLLS = 1 << 20, REC_TICKET = 32;
 constexpr int REC_START = 1, REC_END = 2, REC_OUT = 4;     // of a step, in walking order; OUT: behind the last episode
 
-// everything in walking order: step r of the walk is step r, or N - 1 - r for `reverse` (base addresses and strides say so)
+// Step r of the walk is step r, or N - 1 - r for `reverse`: flags, episodes, tiles and maps are in walking order, the operands in their own.
 template <typename T> struct RecWalk {
     using Acc = typename SeqType<T>::Acc;
     int64_t N, D, E;
     const int64_t* ep_off;
     int reverse;
-    int64_t tiles, blocks;     // tiles along the time axis, blocks of channels
+    int64_t tiles;             // along the time axis
+    uint32_t blocks;           // of channels
     const T *x, *g, *h0;
-    int64_t sx, sg, ldh0;
+    uint32_t ldx, ldg;
+    int64_t ldh0;
     Acc gval;
     const uint8_t* flag;       // [N]
     const int32_t* ep;         // [N]
+    const int32_t* from;       // [tiles]: the tile in which the episode that comes into a tile starts; -1: none comes in
+    const int32_t* till;       // [tiles]: ... in which the episode that goes on behind it ends; -1: none goes on
     uint32_t* ticket;
     Acc* map;                  // [tiles][D][2]: the published maps
-    Acc* through;              // [tiles / REC_GROUP + 1][D]: the published states between groups
+    Acc* through;              // [tiles / REC_GROUP + 2][D]: the published states between groups
     Acc* state;                // [tiles][D]: the state before each tile (nullable in the forward pass)
-    T* h; int64_t sh;          // forward: the result
-    T* last;
-    const T *dh, *dlast; int64_t sdh;
-    T *dx, *dg, *dh0;          // sh is their stride, too (dg of a shared gate: 1 or -1)
+    T *h, *last;               // forward: the results
+    const T *dh, *dlast;
+    uint32_t lddh;
+    T *dx, *dg, *dh0;
     Acc* dgp;                  // shared gate: [channel blocks][N] partial sums, or null: one block, straight to dg
 };
 
@@ -51,11 +55,23 @@ template <typename T> constexpr int REC_K = sizeof(T) == 8 ? 4 : 8;
 template <typename T> constexpr int REC_VEC = sizeof(T) == 8 ? 2 : 4;
 
 template <typename T, int VEC> struct RecRaw { T v[VEC]; };
-template <typename T, int VEC> __device__ __forceinline__ RecRaw<T, VEC> rec_load(const T* p) {
+// `at` elements behind a workgroup's own base: one scalar address and 32-bit offsets (the host holds TILE * ld to 32 bits).  Rows lie at any multiple of
+// the type: unaligned vector accesses.
+template <typename T, int VEC> __device__ __forceinline__ RecRaw<T, VEC> rec_load(const T* base, uint32_t at) {
     RecRaw<T, VEC> r;
-    __builtin_memcpy(&r, p, sizeof(r));                    // rows lie at any multiple of the type: an unaligned vector load
+    __builtin_memcpy(&r, reinterpret_cast<const char*>(base) + (uint32_t)(at * (uint32_t)sizeof(T)), sizeof(r));
     return r;
 }
+template <typename T, int VEC> __device__ __forceinline__ void rec_store(T* base, uint32_t at, const RecRaw<T, VEC>& r) {
+    __builtin_memcpy(reinterpret_cast<char*>(base) + (uint32_t)(at * (uint32_t)sizeof(T)), &r, sizeof(r));
+}
+
+// a workgroup's tile: the steps row0 .. row0 + rows - 1 of the walk, the first of its rows in memory
+struct RecSpan {
+    int64_t tile, row0, low;
+    int rows;
+    uint32_t blk;
+};
 
 __device__ __forceinline__ int64_t rec_ep_begin(const int64_t* off, int64_t e, int reverse, int64_t N) {
     const int64_t s = reverse ? N - off[e + 1] : off[e];
@@ -74,20 +90,23 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
     T gs[GK == 2 ? 1 : K];
     uint64_t fl;
     int n;                                                 // steps that exist
-    __device__ __forceinline__ void load(const RecWalk<T>& a, int64_t r0, int64_t row1, int64_t cb, bool want_x) {
-        const int64_t left = row1 - r0;
-        n = left < 0 ? 0 : left > K ? K : (int)left;
+    // lr: the thread's first step within the tile; at(k): where its k-th lies among the tile's rows in memory
+    __device__ __forceinline__ void load(const RecWalk<T>& a, const RecSpan& w, int tile_rows, int lr, uint32_t cb) {
+        const int left = w.rows - lr;
+        n = left < 0 ? 0 : left > K ? K : left;
         fl = 0;
-        if (n > 0) __builtin_memcpy(&fl, a.flag + r0, K);  // the array has K bytes of room behind it
+        if (n > 0) __builtin_memcpy(&fl, a.flag + w.row0 + lr, K);       // the array has K bytes of room behind it
         if (n < K) fl = n <= 0 ? 0 : fl & ((1ull << (8 * n)) - 1);
+        const T *xb = a.x + w.low * (int64_t)a.ldx, *gb = a.g ? a.g + w.low * (int64_t)a.ldg : nullptr;
+        const T* db = BACK ? a.dh + w.low * (int64_t)a.lddh : nullptr;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            int64_t r = r0 + k;
-            r = r < row1 ? r : row1 - 1;
-            if (want_x) x[k] = rec_load<T, VEC>(a.x + r * a.sx + cb);
-            if constexpr (GK == 2) g[k] = rec_load<T, VEC>(a.g + r * a.sg + cb);
-            else if (a.g) gs[k] = a.g[r * a.sg];
-            if constexpr (BACK) dh[k] = rec_load<T, VEC>(a.dh + r * a.sdh + cb);
+            const int l = lr + k < w.rows ? lr + k : w.rows - 1;         // steps that do not exist repeat the last
+            const uint32_t at = (uint32_t)(a.reverse ? tile_rows - 1 - l : l);
+            x[k] = rec_load<T, VEC>(xb, at * a.ldx + cb);
+            if constexpr (GK == 2) g[k] = rec_load<T, VEC>(gb, at * a.ldg + cb);
+            else if (a.g) gs[k] = rec_load<T, 1>(gb, at * a.ldg).v[0];
+            if constexpr (BACK) dh[k] = rec_load<T, VEC>(db, at * a.lddh + cb);
         }
     }
     __device__ __forceinline__ int flag(int k) const { return (int)(fl >> (8 * k)) & 7; }
@@ -174,7 +193,7 @@ __device__ __forceinline__ void rec_carry(const RecMap<Acc, VEC>& m, const RecSh
 
 // the thread's steps as one map, forward in time
 template <typename T, int C, int VEC, int GK, bool BACK>
-__device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecTile<T, C, VEC, GK, BACK>& t, int64_t r0, int64_t cb,
+__device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecTile<T, C, VEC, GK, BACK>& t, int64_t r0, uint32_t cb,
                                                 RecMap<typename SeqType<T>::Acc, VEC>& m) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>;
@@ -210,7 +229,7 @@ __device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecTi
 }
 // ... and backward: c -> g (dh + c), from behind; an episode's last step takes dlast instead of what comes from behind it
 template <typename T, int C, int VEC, int GK>
-__device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecTile<T, C, VEC, GK, true>& t, int64_t r0, int64_t cb,
+__device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecTile<T, C, VEC, GK, true>& t, int64_t r0, uint32_t cb,
                                                  RecMap<typename SeqType<T>::Acc, VEC>& m) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>;
@@ -270,13 +289,23 @@ __device__ __forceinline__ void rec_put_state(double* p, double v) { rec_put(rei
 __device__ __forceinline__ float rec_get_state(const float* p) { return __uint_as_float(rec_poll(reinterpret_cast<const uint32_t*>(p))); }
 __device__ __forceinline__ double rec_get_state(const double* p) { return __longlong_as_double((long long)rec_poll(reinterpret_cast<const uint64_t*>(p))); }
 
-// the tile's own number in time order; one tile needs no order
-template <typename T> __device__ __forceinline__ int64_t rec_ticket(const RecWalk<T>& a) {
-    if (a.tiles <= 1) return blockIdx.x;
-    __shared__ uint32_t mine;
-    if (threadIdx.x == 0) mine = atomicAdd(a.ticket, 1u);
-    __syncthreads();
-    return mine;
+// The tile's number in time order within its block of channels (a counter per block: the chains of two blocks do not meet, and one counter for all
+// of 16384 workgroups takes them 16 ns each).
+template <typename T> __device__ __forceinline__ RecSpan rec_span(const RecWalk<T>& a, int tile_rows, bool back) {
+    RecSpan w;
+    w.blk = blockIdx.x % a.blocks;
+    w.tile = 0;
+    if (a.tiles > 1) {
+        __shared__ uint32_t mine;
+        if (threadIdx.x == 0) mine = atomicAdd(a.ticket + w.blk * REC_TICKET, 1u);
+        __syncthreads();
+        w.tile = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine);
+    }
+    if (back) w.tile = a.tiles - 1 - w.tile;
+    w.row0 = w.tile * tile_rows;
+    w.rows = (int)(a.N - w.row0 < tile_rows ? a.N - w.row0 : tile_rows);
+    w.low = a.reverse ? a.N - w.row0 - tile_rows : w.row0;
+    return w;
 }
 
 // the whole tile's map, from the wavefronts' totals
@@ -300,7 +329,7 @@ __device__ __forceinline__ RecMap<Acc, VEC> rec_total(const RecShare<Acc, C, VEC
 // What reaches `tile` of an episode that comes in from the tile `from` (DIR > 0: an earlier one; < 0: a later one).  The thread group j takes the map
 // of tile j of the group, as if it were a segment of its own, and the maps are joined as segments are; `from` itself passes on its B alone.
 template <typename T, int C, int VEC, int DIR>
-__device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int64_t from, int64_t cb, int lane, int wv,
+__device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int64_t from, uint32_t cb, int lane, int wv,
                                           RecShare<typename SeqType<T>::Acc, C, VEC>& sh, typename SeqType<T>::Acc (&carry)[VEC]) {
     using Acc = typename SeqType<T>::Acc;
     const int64_t group = tile / REC_GROUP;
@@ -329,21 +358,23 @@ __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) 
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share, reach;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
-    const int64_t ticket = rec_ticket(a), tile = ticket / a.blocks, blk = ticket - tile * a.blocks;
-    if (tile >= a.tiles) {                                 // the states that empty episodes end with
-        const int64_t groups = REC_THREADS / 64, first = (ticket - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
+    if (blockIdx.x >= a.tiles * a.blocks) {                                 // the states that empty episodes end with
+        const int64_t groups = REC_THREADS / 64, first = (blockIdx.x - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
         for (int64_t e = first; e < a.E; e += step)
             if (rec_ep_begin(a.ep_off, e, a.reverse, a.N) >= rec_ep_end(a.ep_off, e, a.reverse, a.N))
                 for (int64_t d = lane; d < a.D; d += 64) a.last[e * a.D + d] = a.h0 ? a.h0[e * a.ldh0 + d] : narrow<T>(0.0f);
         return;
     }
-    const int64_t c0 = (blk * C + c) * VEC;
+    const RecSpan w = rec_span(a, TILE, false);
+    const int64_t tile = w.tile;
+    const int from = a.tiles > 1 ? a.from[tile] : -1;
+    const int64_t c0 = ((int64_t)w.blk * C + c) * VEC;
     const bool mine = c0 < a.D;
-    const int64_t cb = c0 < a.D - VEC ? c0 : a.D - VEC;    // the last lanes move back to whole vectors: the same channels, the same values
-    const int64_t row0 = tile * TILE, row1 = row0 + TILE < a.N ? row0 + TILE : a.N;
-    const int64_t r0 = row0 + (int64_t)(wv * (64 / C) + lane / C) * K;
+    const uint32_t cb = (uint32_t)(c0 < a.D - VEC ? c0 : a.D - VEC);     // the last lanes move back to whole vectors: the same channels, the same values
+    const int lr = (wv * (64 / C) + lane / C) * K;
+    const int64_t r0 = w.row0 + lr;
     RecTile<T, C, VEC, GK, false> t;
-    t.load(a, r0, row1, cb, true);
+    t.load(a, w, TILE, lr, cb);
     RecMap<Acc, VEC> m;
     rec_map_forward(a, t, r0, cb, m);
     rec_scan_wave<Acc, C, VEC, 1>(m, share, lane, wv);
@@ -357,10 +388,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) 
         if (first && tile + 1 < a.tiles)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
-        if (tile > 0 && !(a.flag[row0] & (REC_START | REC_OUT))) {
-            const int64_t from = rec_ep_begin(a.ep_off, a.ep[row0], a.reverse, a.N) / TILE;
-            rec_reach<T, C, VEC, 1>(a, tile, from < tile ? from : tile - 1, cb, lane, wv, reach, carry);
-        }
+        if (from >= 0) rec_reach<T, C, VEC, 1>(a, tile, from, cb, lane, wv, reach, carry);
         if (first && tile % REC_GROUP == REC_GROUP - 1 && tile + 1 < a.tiles)
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
@@ -370,6 +398,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) 
         for (int v = 0; v < VEC; ++v) a.state[tile * a.D + cb + v] = carry[v];
     rec_carry<Acc, C, VEC, 1>(m, share, lane, wv, carry, s);
     const bool plain = __all(t.fl == 0 && t.n == K);
+    T* hb = a.h + w.low * a.D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         if (!plain) {
@@ -390,7 +419,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) 
             for (int v = 0; v < VEC; ++v) { s[v] = 0; o.v[v] = narrow<T>(0.0f); }
         }
         if (mine) {
-            __builtin_memcpy(a.h + (r0 + k) * a.sh + cb, &o, sizeof(o));
+            rec_store(hb, (uint32_t)(a.reverse ? TILE - 1 - lr - k : lr + k) * (uint32_t)a.D + cb, o);
             if (a.last && !plain && (t.flag(k) & REC_END)) __builtin_memcpy(a.last + a.ep[r0 + k] * a.D + cb, &o, sizeof(o));
         }
     }
@@ -402,22 +431,23 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share_b, share_f, reach;
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
-    const int64_t ticket = rec_ticket(a), order = ticket / a.blocks, blk = ticket - order * a.blocks;
-    if (order >= a.tiles) {                                // an empty episode hands its dlast through
-        const int64_t groups = REC_THREADS / 64, first = (ticket - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
+    if (blockIdx.x >= a.tiles * a.blocks) {                                // an empty episode hands its dlast through
+        const int64_t groups = REC_THREADS / 64, first = (blockIdx.x - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
         for (int64_t e = first; e < a.E; e += step)
             if (rec_ep_begin(a.ep_off, e, a.reverse, a.N) >= rec_ep_end(a.ep_off, e, a.reverse, a.N))
                 for (int64_t d = lane; d < a.D; d += 64) a.dh0[e * a.D + d] = a.dlast ? a.dlast[e * a.D + d] : narrow<T>(0.0f);
         return;
     }
-    const int64_t tile = a.tiles - 1 - order;              // from the end of time
-    const int64_t c0 = (blk * C + c) * VEC;
+    const RecSpan w = rec_span(a, TILE, true);             // from the end of time
+    const int64_t tile = w.tile;
+    const int till = a.tiles > 1 ? a.till[tile] : -1;
+    const int64_t c0 = ((int64_t)w.blk * C + c) * VEC;
     const bool mine = c0 < a.D;
-    const int64_t cb = c0 < a.D - VEC ? c0 : a.D - VEC;
-    const int64_t row0 = tile * TILE, row1 = row0 + TILE < a.N ? row0 + TILE : a.N;
-    const int64_t r0 = row0 + (int64_t)(wv * (64 / C) + lane / C) * K;
+    const uint32_t cb = (uint32_t)(c0 < a.D - VEC ? c0 : a.D - VEC);
+    const int lr = (wv * (64 / C) + lane / C) * K;
+    const int64_t r0 = w.row0 + lr;
     RecTile<T, C, VEC, GK, true> t;
-    t.load(a, r0, row1, cb, true);
+    t.load(a, w, TILE, lr, cb);
     Acc state[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) state[v] = a.state[tile * a.D + cb + v];
@@ -436,10 +466,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
         if (first && tile > 0)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
-        if (row1 < a.N && !(a.flag[row1 - 1] & (REC_END | REC_OUT))) {
-            const int64_t from = (rec_ep_end(a.ep_off, a.ep[row1 - 1], a.reverse, a.N) - 1) / TILE;
-            rec_reach<T, C, VEC, -1>(a, tile, from > tile ? from : tile + 1, cb, lane, wv, reach, carry);
-        }
+        if (till >= 0) rec_reach<T, C, VEC, -1>(a, tile, till, cb, lane, wv, reach, carry);
         if (first && tile % REC_GROUP == 0 && tile > 0)
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
@@ -460,6 +487,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
         }
     }
     Acc sum[K];
+    T *dxb = a.dx + w.low * a.D, *dgb = a.dg + (GK == 2 ? w.low * a.D : w.low);
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
         sum[k] = 0;
@@ -483,8 +511,9 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
             for (int v = 0; v < VEC; ++v) { ox.v[v] = og.v[v] = narrow<T>(0.0f); back[v] = 0; }
         }
         if (mine) {
-            if (a.dx) __builtin_memcpy(a.dx + (r0 + k) * a.sh + cb, &ox, sizeof(ox));
-            if (GK == 2 && a.dg) __builtin_memcpy(a.dg + (r0 + k) * a.sh + cb, &og, sizeof(og));
+            const uint32_t at = (uint32_t)(a.reverse ? TILE - 1 - lr - k : lr + k) * (uint32_t)a.D + cb;
+            if (a.dx) rec_store(dxb, at, ox);
+            if (GK == 2 && a.dg) rec_store(dgb, at, og);
             if (a.dh0 && (f & REC_START)) {
                 RecRaw<T, VEC> o0;
 #pragma unroll
@@ -501,8 +530,8 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
 #pragma unroll
                 for (int o = 1; o < C; o <<= 1) v += __shfl_xor(v, o);
                 if (c == 0 && k < t.n) {
-                    if (a.dgp) a.dgp[blk * a.N + r0 + k] = v;
-                    else a.dg[(r0 + k) * (a.reverse ? -1 : 1)] = narrow<T>(v);
+                    if (a.dgp) a.dgp[(int64_t)w.blk * a.N + r0 + k] = v;
+                    else dgb[a.reverse ? TILE - 1 - lr - k : lr + k] = narrow<T>(v);
                 }
             }
         }
@@ -524,7 +553,7 @@ inline unsigned rec_empty_blocks(bool wanted, int64_t E) { return wanted ? (unsi
 struct RecPlan {
     int tile;
     int64_t tiles, blocks;
-    int64_t flag, ep, plan_bytes;                          // the walk: in the states where there are any, else in the workspace
+    int64_t flag, ep, from, till, plan_bytes;                          // the walk: in the states where there are any, else in the workspace
     int64_t state, states_bytes;
     int64_t ticket, map, through, clear_bytes;             // what passes between workgroups: cleared before each launch
     int64_t dgp, ws_plan, ws_bytes;

@@ -73,14 +73,17 @@ def nstep_backup(rew, ep_off, ep_done, gamma: float = 0.95, horizon: int = 10):
 
 
 # ---- the recurrence along episodes --------------------------------------------------------------------------------------------
+_FAR = 1 << 17          # a tile's rows are addressed by 32-bit offsets: operands with rows further apart are copied
+
+
 def _recurrence_args(x, gate, ep_off, h0, gate_value, reverse):
     kind = 0 if gate is None else 2 if gate.dim() == 2 else 1
-    x, ldx = _seq.rows_of(x)
+    x, ldx = _seq.rows_of(x, _FAR)
     ldg = 0
     if kind == 2:
-        gate, ldg = _seq.rows_of(gate)
+        gate, ldg = _seq.rows_of(gate, _FAR)
     elif kind == 1:
-        gate, ldg = (gate, gate.stride(0)) if gate.stride(0) >= 0 else (gate.contiguous(), 1)
+        gate, ldg = (gate, gate.stride(0)) if 0 <= gate.stride(0) <= _FAR else (gate.contiguous(), 1)
     ldh0 = 0
     if h0 is not None:
         h0, ldh0 = _seq.rows_of(h0)
@@ -110,7 +113,7 @@ def _recurrence_forward(x, gate, ep_off, h0, gate_value, reverse, want_last, wan
 def _recurrence_backward(x, gate, ep_off, h0, gate_value, reverse, states, dh, dlast, want):
     lib, dev = _lib.load(), x.device
     a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
-    dh, lddh = _seq.rows_of(dh)
+    dh, lddh = _seq.rows_of(dh, _FAR)
     dlast = None if dlast is None else dlast.contiguous()
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
     dgate = torch.empty(gate.shape, dtype=x.dtype, device=dev) if want[1] else None
