@@ -69,7 +69,8 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
     p.states_bytes = at;
     at = 0;
     p.map = take(p.tiles > 1 ? 2 * p.tiles * D * acc : 0);
-    p.through = take(p.tiles > 1 ? (p.tiles / REC_GROUP + 2) * D * acc : 0);
+    p.group = take(p.tiles > 1 ? 2 * (p.tiles / REC_GROUP + 1) * D * acc : 0);
+    p.through = take(p.tiles > 1 ? (p.tiles / REC_GROUP + 1) * D * acc : 0);
     p.clear_bytes = at;
     p.ticket = take(p.tiles > 1 ? 4 * REC_TICKET * p.blocks : 0);
     p.ws_plan = take(p.plan_bytes);
@@ -96,6 +97,7 @@ template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, co
     a.ep = reinterpret_cast<int32_t*>(plan + p.ep);
     a.ticket = reinterpret_cast<uint32_t*>(ws + p.ticket);
     a.map = reinterpret_cast<Acc*>(ws + p.map);
+    a.group = reinterpret_cast<Acc*>(ws + p.group);
     a.through = reinterpret_cast<Acc*>(ws + p.through);
     a.from = reinterpret_cast<int32_t*>(plan + p.from);
     a.till = reinterpret_cast<int32_t*>(plan + p.till);

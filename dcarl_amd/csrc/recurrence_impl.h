@@ -6,11 +6,11 @@
 //   * a thread walks K consecutive steps of VEC channels held in registers; the 64 / C groups of a wavefront and the four wavefronts of a
 //     workgroup hold consecutive segments, so a workgroup takes one tile of 4 * (64 / C) * K steps of C * VEC channels;
 //   * the segments' maps are composed by shuffles and through LDS, then each thread walks its steps once more from the state that reaches it;
-//   * the state that reaches a tile: every tile publishes its own map as soon as it has it, and takes those of the tiles before it back to its
-//     episode's start, or to the start of its group of REC_GROUP tiles and from there the state that the last tile of the group before has
-//     published.  So the tiles wait for one another in a chain, of one link per group, and x and g are read once.
+//   * the state that reaches a tile: every tile publishes its own map as soon as it has it, every group of REC_GROUP tiles its map; a tile joins those
+//     between its episode's start and itself, tiles in its own group, whole groups before, and beyond REC_BACK groups the state published there.
+//     x and g are read once.
 // The waits end: a workgroup takes its tile by a ticket, in time order, so whatever it waits for belongs to workgroups that run already and
-// publish their maps without waiting; a wait that takes REC_POLLS polls all the same gives up with NaN.  A published word is its own flag: the
+// wait in turn only for earlier ones; a wait that takes REC_POLLS polls all the same gives up with NaN.  A published word is its own flag: the
 // words are cleared to a pattern before the launch that no result has (rec_word), written and polled by relaxed atomics of device scope, and
 // nothing else passes between workgroups, so no fence is needed.
 // An episode's start is a flag, never a gate of zero: what lies before it is dropped, so a NaN there stays there.
@@ -20,7 +20,7 @@
 
 namespace dcarl {
 
-constexpr int REC_THREADS = 256, REC_WAVES = 4, REC_GROUP = 16, REC_POLLS = 1 << 20, REC_TICKET = 32;
+constexpr int REC_THREADS = 256, REC_WAVES = 4, REC_GROUP = 16, REC_BACK = 4, REC_POLLS = 1 << 20, REC_TICKET = 32;
 constexpr int REC_START = 1, REC_END = 2, REC_OUT = 4;     // of a step, in walking order; OUT: behind the last episode
 
 // Step r of the walk is step r, or N - 1 - r for `reverse`: flags, episodes, tiles and maps are in walking order, the operands in their own.
@@ -41,7 +41,8 @@ template <typename T> struct RecWalk {
     const int32_t* till;       // [tiles]: ... in which the episode that goes on behind it ends; -1: none goes on
     uint32_t* ticket;
     Acc* map;                  // [tiles][D][2]: the published maps
-    Acc* through;              // [tiles / REC_GROUP + 2][D]: the published states between groups
+    Acc* group;                // [tiles / REC_GROUP + 1][D][2]: ... of whole groups
+    Acc* through;              // [tiles / REC_GROUP + 1][D]: the published states that reach the groups
     Acc* state;                // [tiles][D]: the state before each tile (nullable in the forward pass)
     T *h, *last;               // forward: the results
     const T *dh, *dlast;
@@ -326,30 +327,69 @@ __device__ __forceinline__ RecMap<Acc, VEC> rec_total(const RecShare<Acc, C, VEC
     return t;
 }
 
-// What reaches `tile` of an episode that comes in from the tile `from` (DIR > 0: an earlier one; < 0: a later one).  The thread group j takes the map
-// of tile j of the group, as if it were a segment of its own, and the maps are joined as segments are; `from` itself passes on its B alone.
+// What reaches `tile` of an episode that comes in from the tile `from` (DIR > 0: an earlier one; < 0: a later one):
+//   P, the map of the tiles of its own group between `from` and itself: the thread group j takes the map of tile j of the group, as if it were a segment of
+//   its own, and they are joined as segments are; `from` itself passes on its B alone;
+//   the state that reaches the group: the maps of the up to REC_BACK groups before, on what reaches the first of them -- published REC_BACK groups ago, so
+//   that a chain of episodes longer than that has one link per REC_BACK groups (with a link per group the longest streams ran at 60 % of the rate of
+//   short ones).
+// The group's last tile publishes the group's map before it waits for that state, and then what leaves the group.
 template <typename T, int C, int VEC, int DIR>
-__device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int64_t from, uint32_t cb, int lane, int wv,
-                                          RecShare<typename SeqType<T>::Acc, C, VEC>& sh, typename SeqType<T>::Acc (&carry)[VEC]) {
+__device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int from, uint32_t cb, int lane, int wv, bool first,
+                                          const RecMap<typename SeqType<T>::Acc, VEC>& total, RecShare<typename SeqType<T>::Acc, C, VEC>& sh,
+                                          typename SeqType<T>::Acc (&reached)[C * VEC], typename SeqType<T>::Acc (&carry)[VEC]) {
     using Acc = typename SeqType<T>::Acc;
     const int64_t group = tile / REC_GROUP;
-    const int j = wv * (64 / C) + lane / C;
+    const bool closes = DIR > 0 ? tile % REC_GROUP == REC_GROUP - 1 && tile + 1 < a.tiles : tile % REC_GROUP == 0 && tile > 0;
+    const int c = lane % C, j = wv * (64 / C) + lane / C;
     const int64_t src = group * REC_GROUP + j;
     RecMap<Acc, VEC> m;
     m.one();
-    if (j < REC_GROUP && (DIR > 0 ? src < tile && src >= from : src > tile && src <= from)) {
+    if (from >= 0) {                                       // (otherwise an episode starts with the tile: its map is all there is)
+        if (j < REC_GROUP && (DIR > 0 ? src < tile && src >= from : src > tile && src <= from)) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) rec_get_map(a.map + (src * a.D + cb + v) * 2, m.A[v], m.B[v]);
-        m.cut = src == from;
+            for (int v = 0; v < VEC; ++v) rec_get_map(a.map + (src * a.D + cb + v) * 2, m.A[v], m.B[v]);
+            m.cut = src == from;
+        }
+        rec_scan_wave<Acc, C, VEC, DIR>(m, sh, lane, wv);
+        __syncthreads();
+        m = rec_total<Acc, C, VEC, DIR>(sh, c);            // P
     }
-    const bool outside = DIR > 0 ? from < group * REC_GROUP : from >= (group + 1) * REC_GROUP;
+    const bool outside = from >= 0 && (DIR > 0 ? from < group * REC_GROUP : from >= (group + 1) * REC_GROUP);
+    if (closes && first) {
+        RecMap<Acc, VEC> g = total;
+        g.after(m);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = outside ? rec_get_state(a.through + (DIR > 0 ? group : group + 1) * a.D + cb + v) : Acc(0);
-    rec_scan_wave<Acc, C, VEC, DIR>(m, sh, lane, wv);
-    __syncthreads();
-    const RecMap<Acc, VEC> t = rec_total<Acc, C, VEC, DIR>(sh, lane % C);
+        for (int v = 0; v < VEC; ++v) rec_put_map(a.group + (group * a.D + cb + v) * 2, g.A[v], g.B[v]);
+    }
+    if (outside) {
+        if (first) {
+            const int64_t fg = from / REC_GROUP;
+            Acc st[VEC];
+            // the groups fg .. group - 1 (DIR > 0), at most the last REC_BACK of them; fg itself passes on its B alone
+            const int64_t far = DIR > 0 ? group - REC_BACK : group + REC_BACK;
+            const bool chain = DIR > 0 ? fg < far : fg > far;
+            int64_t g = chain ? far : fg;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = t.cut ? t.B[v] : fma(t.A[v], carry[v], t.B[v]);
+            for (int v = 0; v < VEC; ++v) st[v] = chain ? rec_get_state(a.through + (g * a.D + cb + v)) : Acc(0);
+            for (bool only = !chain; g != group; g += DIR, only = false)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    Acc A, B;
+                    rec_get_map(a.group + (g * a.D + cb + v) * 2, A, B);
+                    st[v] = only ? B : fma(A, st[v], B);
+                }
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) reached[c * VEC + v] = st[v];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) carry[v] = from < 0 ? Acc(0) : m.cut ? m.B[v] : fma(m.A[v], outside ? reached[c * VEC + v] : Acc(0), m.B[v]);
+    if (closes && first)                                   // what reaches the next group
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+            rec_put_state(a.through + ((group + DIR) * a.D + cb + v), total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
 }
 
 template <typename T, int C, int VEC, int GK>
@@ -357,6 +397,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) 
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share, reach;
+    __shared__ Acc reached[C * VEC];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
     if (blockIdx.x >= a.tiles * a.blocks) {                                 // the states that empty episodes end with
         const int64_t groups = REC_THREADS / 64, first = (blockIdx.x - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
@@ -388,11 +429,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) 
         if (first && tile + 1 < a.tiles)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
-        if (from >= 0) rec_reach<T, C, VEC, 1>(a, tile, from, cb, lane, wv, reach, carry);
-        if (first && tile % REC_GROUP == REC_GROUP - 1 && tile + 1 < a.tiles)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                rec_put_state(a.through + (tile / REC_GROUP + 1) * a.D + cb + v, total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
+        rec_reach<T, C, VEC, 1>(a, tile, from, cb, lane, wv, first, total, reach, reached, carry);
     }
     if (a.state && first)
         for (int v = 0; v < VEC; ++v) a.state[tile * a.D + cb + v] = carry[v];
@@ -430,6 +467,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share_b, share_f, reach;
+    __shared__ Acc reached[C * VEC];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
     if (blockIdx.x >= a.tiles * a.blocks) {                                // an empty episode hands its dlast through
         const int64_t groups = REC_THREADS / 64, first = (blockIdx.x - a.tiles * a.blocks) * groups + wv, step = ((int64_t)gridDim.x - a.tiles * a.blocks) * groups;
@@ -466,11 +504,7 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
         if (first && tile > 0)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
-        if (till >= 0) rec_reach<T, C, VEC, -1>(a, tile, till, cb, lane, wv, reach, carry);
-        if (first && tile % REC_GROUP == 0 && tile > 0)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                rec_put_state(a.through + tile / REC_GROUP * a.D + cb + v, total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
+        rec_reach<T, C, VEC, -1>(a, tile, till, cb, lane, wv, first, total, reach, reached, carry);
     }
     rec_carry<Acc, C, VEC, -1>(mb, share_b, lane, wv, carry, back);
     rec_carry<Acc, C, VEC, 1>(mf, share_f, lane, wv, state, s);
@@ -555,7 +589,7 @@ struct RecPlan {
     int64_t tiles, blocks;
     int64_t flag, ep, from, till, plan_bytes;                          // the walk: in the states where there are any, else in the workspace
     int64_t state, states_bytes;
-    int64_t ticket, map, through, clear_bytes;             // what passes between workgroups: cleared before each launch
+    int64_t ticket, map, group, through, clear_bytes;             // what passes between workgroups: cleared before each launch
     int64_t dgp, ws_plan, ws_bytes;
 };
 RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind);
