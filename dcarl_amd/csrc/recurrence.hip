@@ -58,6 +58,7 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
         rec_with_shape<T>(D, [&](auto C, auto V) {
             p.tile = REC_TILE<C(), T>;
             p.blocks = (D + C() * V() - 1) / (C() * V());
+            p.wide = p.blocks * C() * V();
         });
     });
     p.tiles = (N + p.tile - 1) / p.tile;
@@ -68,9 +69,9 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
     p.state = take(p.tiles * D * acc);
     p.states_bytes = at;
     at = 0;
-    p.map = take(p.tiles > 1 ? 2 * p.tiles * D * acc : 0);
-    p.group = take(p.tiles > 1 ? 2 * (p.tiles / REC_GROUP + 1) * D * acc : 0);
-    p.through = take(p.tiles > 1 ? (p.tiles / REC_GROUP + 1) * D * acc : 0);
+    p.map = take(p.tiles > 1 ? 2 * p.tiles * p.wide * acc : 0);
+    p.group = take(p.tiles > 1 ? 2 * (p.tiles / REC_GROUP + 1) * p.wide * acc : 0);
+    p.through = take(p.tiles > 1 ? (p.tiles / REC_GROUP + 1) * p.wide * acc : 0);
     p.clear_bytes = at;
     p.ticket = take(p.tiles > 1 ? 4 * REC_TICKET * p.blocks : 0);
     p.ws_plan = take(p.plan_bytes);

@@ -40,9 +40,9 @@ template <typename T> struct RecWalk {
     const int32_t* from;       // [tiles]: the tile in which the episode that comes into a tile starts; -1: none comes in
     const int32_t* till;       // [tiles]: ... in which the episode that goes on behind it ends; -1: none goes on
     uint32_t* ticket;
-    Acc* map;                  // [tiles][D][2]: the published maps
-    Acc* group;                // [tiles / REC_GROUP + 1][D][2]: ... of whole groups
-    Acc* through;              // [tiles / REC_GROUP + 1][D]: the published states that reach the groups
+    Acc* map;                  // [tiles][lanes][2] (rec_at): the published maps
+    Acc* group;                // [tiles / REC_GROUP + 1][lanes][2]: ... of whole groups
+    Acc* through;              // [tiles / REC_GROUP + 1][lanes]: the published states that reach the groups
     Acc* state;                // [tiles][D]: the state before each tile (nullable in the forward pass)
     T *h, *last;               // forward: the results
     const T *dh, *dlast;
@@ -327,6 +327,12 @@ __device__ __forceinline__ RecMap<Acc, VEC> rec_total(const RecShare<Acc, C, VEC
     return t;
 }
 
+// Where the v-th word of lane c lies among those of tile (group) n: the lanes side by side, so that a wavefront's access is a few whole lines (channel by
+// channel, 8 bytes every 32, the polls cost the longest streams a third of their rate).
+template <int C, int VEC> __device__ __forceinline__ int64_t rec_at(int64_t n, uint32_t blocks, uint32_t blk, int v, int c) {
+    return ((n * blocks + blk) * VEC + v) * C + c;
+}
+
 // What reaches `tile` of an episode that comes in from the tile `from` (DIR > 0: an earlier one; < 0: a later one):
 //   P, the map of the tiles of its own group between `from` and itself: the thread group j takes the map of tile j of the group, as if it were a segment of
 //   its own, and they are joined as segments are; `from` itself passes on its B alone;
@@ -335,20 +341,22 @@ __device__ __forceinline__ RecMap<Acc, VEC> rec_total(const RecShare<Acc, C, VEC
 //   short ones).
 // The group's last tile publishes the group's map before it waits for that state, and then what leaves the group.
 template <typename T, int C, int VEC, int DIR>
-__device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int from, uint32_t cb, int lane, int wv, bool first,
+__device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int from, uint32_t blk, int lane, int wv, bool mine,
                                           const RecMap<typename SeqType<T>::Acc, VEC>& total, RecShare<typename SeqType<T>::Acc, C, VEC>& sh,
                                           typename SeqType<T>::Acc (&reached)[C * VEC], typename SeqType<T>::Acc (&carry)[VEC]) {
     using Acc = typename SeqType<T>::Acc;
     const int64_t group = tile / REC_GROUP;
     const bool closes = DIR > 0 ? tile % REC_GROUP == REC_GROUP - 1 && tile + 1 < a.tiles : tile % REC_GROUP == 0 && tile > 0;
     const int c = lane % C, j = wv * (64 / C) + lane / C;
+    const bool first = wv == 0 && lane < C && mine;        // the threads that publish
+    auto at = [&](int64_t n, int v) { return rec_at<C, VEC>(n, a.blocks, blk, v, c); };
     const int64_t src = group * REC_GROUP + j;
     RecMap<Acc, VEC> m;
     m.one();
     if (from >= 0) {                                       // (otherwise an episode starts with the tile: its map is all there is)
-        if (j < REC_GROUP && (DIR > 0 ? src < tile && src >= from : src > tile && src <= from)) {
+        if (j < REC_GROUP && mine && (DIR > 0 ? src < tile && src >= from : src > tile && src <= from)) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) rec_get_map(a.map + (src * a.D + cb + v) * 2, m.A[v], m.B[v]);
+            for (int v = 0; v < VEC; ++v) rec_get_map(a.map + at(src, v) * 2, m.A[v], m.B[v]);
             m.cut = src == from;
         }
         rec_scan_wave<Acc, C, VEC, DIR>(m, sh, lane, wv);
@@ -360,7 +368,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
         RecMap<Acc, VEC> g = total;
         g.after(m);
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) rec_put_map(a.group + (group * a.D + cb + v) * 2, g.A[v], g.B[v]);
+        for (int v = 0; v < VEC; ++v) rec_put_map(a.group + at(group, v) * 2, g.A[v], g.B[v]);
     }
     if (outside) {
         if (first) {
@@ -371,12 +379,12 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
             const bool chain = DIR > 0 ? fg < far : fg > far;
             int64_t g = chain ? far : fg;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) st[v] = chain ? rec_get_state(a.through + (g * a.D + cb + v)) : Acc(0);
+            for (int v = 0; v < VEC; ++v) st[v] = chain ? rec_get_state(a.through + at(g, v)) : Acc(0);
             for (bool only = !chain; g != group; g += DIR, only = false)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
                     Acc A, B;
-                    rec_get_map(a.group + (g * a.D + cb + v) * 2, A, B);
+                    rec_get_map(a.group + at(g, v) * 2, A, B);
                     st[v] = only ? B : fma(A, st[v], B);
                 }
 #pragma unroll
@@ -389,7 +397,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
     if (closes && first)                                   // what reaches the next group
 #pragma unroll
         for (int v = 0; v < VEC; ++v)
-            rec_put_state(a.through + ((group + DIR) * a.D + cb + v), total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
+            rec_put_state(a.through + at(group + DIR, v), total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
 }
 
 template <typename T, int C, int VEC, int GK>
@@ -428,8 +436,8 @@ __global__ __launch_bounds__(REC_THREADS) void rec_forward_kernel(RecWalk<T> a) 
         const RecMap<Acc, VEC> total = rec_total<Acc, C, VEC, 1>(share, c);
         if (first && tile + 1 < a.tiles)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
-        rec_reach<T, C, VEC, 1>(a, tile, from, cb, lane, wv, first, total, reach, reached, carry);
+            for (int v = 0; v < VEC; ++v) rec_put_map(a.map + rec_at<C, VEC>(tile, a.blocks, w.blk, v, c) * 2, total.A[v], total.B[v]);
+        rec_reach<T, C, VEC, 1>(a, tile, from, w.blk, lane, wv, mine, total, reach, reached, carry);
     }
     if (a.state && first)
         for (int v = 0; v < VEC; ++v) a.state[tile * a.D + cb + v] = carry[v];
@@ -503,8 +511,8 @@ __global__ __launch_bounds__(REC_THREADS) void rec_backward_kernel(RecWalk<T> a)
         const RecMap<Acc, VEC> total = rec_total<Acc, C, VEC, -1>(share_b, c);
         if (first && tile > 0)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) rec_put_map(a.map + (tile * a.D + cb + v) * 2, total.A[v], total.B[v]);
-        rec_reach<T, C, VEC, -1>(a, tile, till, cb, lane, wv, first, total, reach, reached, carry);
+            for (int v = 0; v < VEC; ++v) rec_put_map(a.map + rec_at<C, VEC>(tile, a.blocks, w.blk, v, c) * 2, total.A[v], total.B[v]);
+        rec_reach<T, C, VEC, -1>(a, tile, till, w.blk, lane, wv, mine, total, reach, reached, carry);
     }
     rec_carry<Acc, C, VEC, -1>(mb, share_b, lane, wv, carry, back);
     rec_carry<Acc, C, VEC, 1>(mf, share_f, lane, wv, state, s);
@@ -586,7 +594,7 @@ inline unsigned rec_empty_blocks(bool wanted, int64_t E) { return wanted ? (unsi
 
 struct RecPlan {
     int tile;
-    int64_t tiles, blocks;
+    int64_t tiles, blocks, wide;                           // wide: channels of all blocks' lanes
     int64_t flag, ep, from, till, plan_bytes;                          // the walk: in the states where there are any, else in the workspace
     int64_t state, states_bytes;
     int64_t ticket, map, group, through, clear_bytes;             // what passes between workgroups: cleared before each launch
