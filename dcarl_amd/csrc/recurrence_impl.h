@@ -149,16 +149,20 @@ template <typename Acc, int C, int VEC> struct RecShare {
     int cut[REC_WAVES];
 };
 // within the wavefront: inclusive scan over the groups; the wavefront's total goes to LDS
-template <typename Acc, int C, int VEC, int DIR>
-__device__ __forceinline__ void rec_scan_wave(RecMap<Acc, VEC>& m, RecShare<Acc, C, VEC>& sh, int lane, int wv) {
-    const int c = lane % C, grp = lane / C;
+template <typename Acc, int C, int VEC, int DIR> __device__ __forceinline__ void rec_scan_groups(RecMap<Acc, VEC>& m, int lane) {
+    const int grp = lane / C;
     constexpr int G = 64 / C;
 #pragma unroll
     for (int o = 1; o < G; o <<= 1) {
         const RecMap<Acc, VEC> f = rec_from_lane(m, (lane - DIR * o * C) & 63);
         if (DIR > 0 ? grp >= o : grp < G - o) m.after(f);
     }
-    if (grp == (DIR > 0 ? G - 1 : 0)) {
+}
+template <typename Acc, int C, int VEC, int DIR>
+__device__ __forceinline__ void rec_scan_wave(RecMap<Acc, VEC>& m, RecShare<Acc, C, VEC>& sh, int lane, int wv) {
+    const int c = lane % C;
+    rec_scan_groups<Acc, C, VEC, DIR>(m, lane);
+    if (lane / C == (DIR > 0 ? 64 / C - 1 : 0)) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) { sh.A[wv][c * VEC + v] = m.A[v]; sh.B[wv][c * VEC + v] = m.B[v]; }
         if (c == 0) sh.cut[wv] = m.cut;
@@ -261,13 +265,17 @@ template <int C, typename T> constexpr int REC_TILE = REC_WAVES * (64 / C) * REC
 __device__ __forceinline__ uint32_t rec_word(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v); }
 __device__ __forceinline__ uint64_t rec_word(double v) { return v != v ? 0x7ff8000000000000ull : (uint64_t)__double_as_longlong(v); }
 template <typename W> __device__ __forceinline__ void rec_put(W* p, W w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-template <typename W> __device__ __forceinline__ W rec_poll(const W* p) {
-    W w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int i = 0; w == (W)~(W)0 && i < REC_POLLS; ++i) {
-        __builtin_amdgcn_s_sleep(1);
-        w = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    return w;                                              // given up: all ones, a NaN
+// n words, p(i) the address of the i-th, all in flight together
+template <int n, typename W, typename P> __device__ __forceinline__ void rec_poll(W (&w)[n], P&& p) {
+    bool all = false;
+    for (int tries = 0; !all && tries < REC_POLLS; ++tries) {
+        if (tries) __builtin_amdgcn_s_sleep(1);
+        all = true;
+#pragma unroll
+        for (int i = 0; i < n; ++i) w[i] = __hip_atomic_load(p(i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int i = 0; i < n; ++i) all = all && w[i] != (W)~(W)0;
+    }                                                      // given up: all ones, a NaN
 }
 // a map of f32 is one 8-byte word, one of f64 two
 __device__ __forceinline__ void rec_put_map(float* p, float A, float B) {
@@ -277,18 +285,33 @@ __device__ __forceinline__ void rec_put_map(double* p, double A, double B) {
     rec_put(reinterpret_cast<uint64_t*>(p), rec_word(A));
     rec_put(reinterpret_cast<uint64_t*>(p) + 1, rec_word(B));
 }
-__device__ __forceinline__ void rec_get_map(const float* p, float& A, float& B) {
-    const uint64_t w = rec_poll(reinterpret_cast<const uint64_t*>(p));
-    A = __uint_as_float((uint32_t)w); B = __uint_as_float((uint32_t)(w >> 32));
+// maps of VEC channels, p(v) where the v-th lies
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_maps(P&& p, float (&A)[VEC], float (&B)[VEC]) {
+    uint64_t w[VEC];
+    rec_poll(w, [&](int v) { return reinterpret_cast<const uint64_t*>(p(v)); });
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { A[v] = __uint_as_float((uint32_t)w[v]); B[v] = __uint_as_float((uint32_t)(w[v] >> 32)); }
 }
-__device__ __forceinline__ void rec_get_map(const double* p, double& A, double& B) {
-    A = __longlong_as_double((long long)rec_poll(reinterpret_cast<const uint64_t*>(p)));
-    B = __longlong_as_double((long long)rec_poll(reinterpret_cast<const uint64_t*>(p) + 1));
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_maps(P&& p, double (&A)[VEC], double (&B)[VEC]) {
+    uint64_t w[2 * VEC];
+    rec_poll(w, [&](int i) { return reinterpret_cast<const uint64_t*>(p(i / 2)) + i % 2; });
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) { A[v] = __longlong_as_double((long long)w[2 * v]); B[v] = __longlong_as_double((long long)w[2 * v + 1]); }
 }
 __device__ __forceinline__ void rec_put_state(float* p, float v) { rec_put(reinterpret_cast<uint32_t*>(p), rec_word(v)); }
 __device__ __forceinline__ void rec_put_state(double* p, double v) { rec_put(reinterpret_cast<uint64_t*>(p), rec_word(v)); }
-__device__ __forceinline__ float rec_get_state(const float* p) { return __uint_as_float(rec_poll(reinterpret_cast<const uint32_t*>(p))); }
-__device__ __forceinline__ double rec_get_state(const double* p) { return __longlong_as_double((long long)rec_poll(reinterpret_cast<const uint64_t*>(p))); }
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_states(P&& p, float (&s)[VEC]) {
+    uint32_t w[VEC];
+    rec_poll(w, [&](int v) { return reinterpret_cast<const uint32_t*>(p(v)); });
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s[v] = __uint_as_float(w[v]);
+}
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_states(P&& p, double (&s)[VEC]) {
+    uint64_t w[VEC];
+    rec_poll(w, [&](int v) { return reinterpret_cast<const uint64_t*>(p(v)); });
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) s[v] = __longlong_as_double((long long)w[v]);
+}
 
 // The tile's number in time order within its block of channels (a counter per block: the chains of two blocks do not meet, and one counter for all
 // of 16384 workgroups takes them 16 ns each).
@@ -355,8 +378,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
     m.one();
     if (from >= 0) {                                       // (otherwise an episode starts with the tile: its map is all there is)
         if (j < REC_GROUP && mine && (DIR > 0 ? src < tile && src >= from : src > tile && src <= from)) {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) rec_get_map(a.map + at(src, v) * 2, m.A[v], m.B[v]);
+            rec_get_maps<VEC>([&](int v) { return a.map + at(src, v) * 2; }, m.A, m.B);
             m.cut = src == from;
         }
         rec_scan_wave<Acc, C, VEC, DIR>(m, sh, lane, wv);
@@ -371,24 +393,26 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
         for (int v = 0; v < VEC; ++v) rec_put_map(a.group + at(group, v) * 2, g.A[v], g.B[v]);
     }
     if (outside) {
-        if (first) {
-            const int64_t fg = from / REC_GROUP;
-            Acc st[VEC];
-            // the groups fg .. group - 1 (DIR > 0), at most the last REC_BACK of them; fg itself passes on its B alone
-            const int64_t far = DIR > 0 ? group - REC_BACK : group + REC_BACK;
+        if (wv == 0) {
+            // the groups fg .. group - 1 (DIR > 0), at most the last REC_BACK of them, a thread group each; fg itself passes on its B alone
+            const int64_t fg = from / REC_GROUP, far = group - DIR * REC_BACK;
             const bool chain = DIR > 0 ? fg < far : fg > far;
-            int64_t g = chain ? far : fg;
+            const int64_t g = DIR > 0 ? (chain ? far : fg) + lane / C : group + 1 + lane / C;
+            RecMap<Acc, VEC> q;
+            q.one();
+            if (mine && (DIR > 0 ? g < group : g <= (chain ? far : fg))) {
+                rec_get_maps<VEC>([&](int v) { return a.group + at(g, v) * 2; }, q.A, q.B);
+                q.cut = g == fg;
+            }
+            rec_scan_groups<Acc, C, VEC, DIR>(q, lane);
+            if (mine && lane / C == (DIR > 0 ? 64 / C - 1 : 0)) {
+                Acc st[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) st[v] = chain ? rec_get_state(a.through + at(g, v)) : Acc(0);
-            for (bool only = !chain; g != group; g += DIR, only = false)
+                for (int v = 0; v < VEC; ++v) st[v] = 0;
+                if (chain) rec_get_states<VEC>([&](int v) { return a.through + at(far, v); }, st);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    Acc A, B;
-                    rec_get_map(a.group + at(g, v) * 2, A, B);
-                    st[v] = only ? B : fma(A, st[v], B);
-                }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) reached[c * VEC + v] = st[v];
+                for (int v = 0; v < VEC; ++v) reached[c * VEC + v] = q.cut ? q.B[v] : fma(q.A[v], st[v], q.B[v]);
+            }
         }
         __syncthreads();
     }
