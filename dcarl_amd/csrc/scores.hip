@@ -6,7 +6,7 @@
 
 namespace dcarl {
 
-constexpr int SC_THREADS = 256;
+constexpr int SC_EPT = 8;                      // candidates per thread: 16 and 32 take registers that waiting workgroups need (91 -> 100, 122 us without history)
 constexpr uint32_t SC_SEEN = 0x80000000u;
 template <typename T> constexpr int SC_VEC = 16 / sizeof(T);
 
@@ -21,45 +21,53 @@ struct ScoreArgs {
     int id_wide;
 };
 
-template <typename I> struct SixteenBytes { I v[16 / sizeof(I)]; };
-
-// counts the history [lo, hi) of a row among the tile's nv candidates from v0 on; its entries before `own` were given
-template <typename I>
-__device__ __forceinline__ void scores_count(const I* taken, int64_t lo, int64_t hi, int64_t own, int64_t v0, int nv, uint32_t* cnt) {
-    constexpr int W = 16 / sizeof(I), DEEP = 4;            // 16-byte loads, four in flight: 4096 entries of 32 bits a trip
-    auto one = [&](I id, int64_t i) {
-        const uint64_t v = (uint64_t)((int64_t)id - v0);
-        if (v < (uint64_t)nv) {
-            if (i < own) atomicOr(&cnt[v], SC_SEEN);
+// The history [lo, hi) of a row, counted among the tile's nv candidates from v0 on; its entries before `own` were given.  16-byte loads; each thread's
+// first one is issued before the scores' (loads return in order: behind them it would wait for memory, not for the cache).
+template <int THREADS, typename I> struct ScoreHistory {
+    static constexpr int W = 16 / sizeof(I), DEEP = 4;
+    static constexpr int64_t STEP = (int64_t)THREADS * W;
+    struct Ids { I v[W]; } first;
+    int64_t i;
+    __device__ __forceinline__ void begin(const I* taken, int64_t lo, int64_t hi) {
+        i = lo + (int64_t)threadIdx.x * W;
+        if (i + W <= hi) __builtin_memcpy(&first, taken + i, 16);
+    }
+    __device__ __forceinline__ static void one(I id, int64_t at, int64_t own, int64_t v0, int nv, uint32_t* cnt) {
+        using U = std::conditional_t<sizeof(I) == 4, uint32_t, uint64_t>;
+        const U v = (U)id - (U)v0;
+        if (id >= 0 && v < (U)nv) {
+            if (at < own) atomicOr(&cnt[v], SC_SEEN);
             else atomicAdd(&cnt[v], 1u);
         }
-    };
-    int64_t i = lo + threadIdx.x * W;
-    constexpr int64_t STEP = (int64_t)SC_THREADS * W;
-    for (; i + (DEEP - 1) * STEP + W <= hi; i += DEEP * STEP) {
-        SixteenBytes<I> t[DEEP];
-#pragma unroll
-        for (int d = 0; d < DEEP; ++d) __builtin_memcpy(&t[d], taken + i + d * STEP, 16);
-#pragma unroll
-        for (int d = 0; d < DEEP; ++d)
-#pragma unroll
-            for (int k = 0; k < W; ++k) one(t[d].v[k], i + d * STEP + k);
     }
-    for (; i < hi; i += STEP) {
-        if (i + W <= hi) {
-            SixteenBytes<I> t;
-            __builtin_memcpy(&t, taken + i, 16);
+    __device__ __forceinline__ static void vec(const Ids& t, int64_t at, int64_t own, int64_t v0, int nv, uint32_t* cnt) {
 #pragma unroll
-            for (int k = 0; k < W; ++k) one(t.v[k], i + k);
-        } else
-            for (int k = 0; i + k < hi; ++k) one(taken[i + k], i + k);
+        for (int k = 0; k < W; ++k) one(t.v[k], at + k, own, v0, nv, cnt);
     }
-}
+    __device__ __forceinline__ void count(const I* taken, int64_t hi, int64_t own, int64_t v0, int nv, uint32_t* cnt) {
+        if (i + W <= hi) { vec(first, i, own, v0, nv, cnt); i += STEP; }
+        for (; i + (DEEP - 1) * STEP + W <= hi; i += DEEP * STEP) {
+            Ids t[DEEP];
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) __builtin_memcpy(&t[d], taken + i + d * STEP, 16);
+#pragma unroll
+            for (int d = 0; d < DEEP; ++d) vec(t[d], i + d * STEP, own, v0, nv, cnt);
+        }
+        for (; i < hi; i += STEP) {
+            if (i + W <= hi) {
+                Ids t;
+                __builtin_memcpy(&t, taken + i, 16);
+                vec(t, i, own, v0, nv, cnt);
+            } else
+                for (int64_t k = i; k < hi; ++k) one(taken[k], k, own, v0, nv, cnt);
+        }
+    }
+};
 
-// A workgroup takes EPT * 256 candidates of a row: their scores are on the way while the row's history is counted in LDS.
-template <typename T, int EPT>
-__global__ __launch_bounds__(SC_THREADS) void scores_kernel(const T* in, T* out, ScoreArgs a) {
-    constexpr int VEC = SC_VEC<T>, PIECES = EPT / VEC, TILE = EPT * SC_THREADS;
+// A workgroup takes SC_EPT * THREADS candidates of a row: their scores, biases and masks are on the way while the row's history is counted in LDS.
+template <typename T, typename I, int THREADS>
+__global__ __launch_bounds__(THREADS) void scores_kernel(const T* in, T* out, ScoreArgs a) {
+    constexpr int VEC = SC_VEC<T>, PIECES = SC_EPT / VEC, TILE = SC_EPT * THREADS;
     struct Raw { T v[VEC]; };
     __shared__ uint4 cnt4[TILE / 4];                       // bit 31: given, the rest: times chosen
     uint32_t* cnt = reinterpret_cast<uint32_t*>(cnt4);
@@ -68,35 +76,49 @@ __global__ __launch_bounds__(SC_THREADS) void scores_kernel(const T* in, T* out,
     for (int64_t b = blockIdx.y; b < a.B; b += gridDim.y) {
         const T* src = in + b * a.ld_in + v0;
         T* dst = out + b * a.ld_out + v0;
-        Raw raw[PIECES];
-#pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-            const int i = (p * SC_THREADS + (int)threadIdx.x) * VEC;
-            if (i + VEC <= nv) __builtin_memcpy(&raw[p], src + i, sizeof(Raw));
-            else
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    if (i + k < nv) raw[p].v[k] = src[i + k];
-        }
         int64_t lo = 0, hi = 0;
         if (a.off) {
             lo = a.off[b]; hi = a.off[b + 1];
             lo = lo < 0 ? 0 : lo > a.n_taken ? a.n_taken : lo;
             hi = hi < lo ? lo : hi > a.n_taken ? a.n_taken : hi;
         }
+        const I* taken = static_cast<const I*>(a.taken);
+        ScoreHistory<THREADS, I> ids;
+        if (lo < hi) ids.begin(taken, lo, hi);
+        Raw raw[PIECES];
+        float add[PIECES][VEC];
+        uint32_t bits[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const int i = (p * THREADS + (int)threadIdx.x) * VEC;
+            bits[p] = ~0u;                                 // VEC candidates lie in one word
+            if (a.allowed && i < nv) bits[p] = a.allowed[b * a.ld_allowed + ((v0 + i) >> 5)] >> ((v0 + i) & 31);
+            if (a.bias) {
+                const float* bias = a.bias + b * a.ld_bias + v0 + i;
+                if (i + VEC <= nv) __builtin_memcpy(add[p], bias, sizeof(add[p]));
+                else
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k)
+                        if (i + k < nv) add[p][k] = bias[k];
+            }
+            if (i + VEC <= nv) __builtin_memcpy(&raw[p], src + i, sizeof(Raw));
+            else
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    if (i + k < nv) raw[p].v[k] = src[i + k];
+        }
         if (lo < hi) {
             __syncthreads();                               // the previous row's counts have been read
-            for (int i = threadIdx.x; i < TILE / 4; i += SC_THREADS) cnt4[i] = make_uint4(0, 0, 0, 0);
+            for (int i = threadIdx.x; i < TILE / 4; i += THREADS) cnt4[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
             const int64_t own = lo + (a.given ? a.given[b] : 0);
-            if (a.id_wide) scores_count(static_cast<const int64_t*>(a.taken), lo, hi, own, v0, nv, cnt);
-            else scores_count(static_cast<const int32_t*>(a.taken), lo, hi, own, v0, nv, cnt);
+            ids.count(taken, hi, own, v0, nv, cnt);
             __syncthreads();
         }
         const float r = a.rep ? a.rep[b] : a.rep0, f = a.freq ? a.freq[b] : a.freq0, p0 = a.pres ? a.pres[b] : a.pres0;
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
-            const int i = (p * SC_THREADS + (int)threadIdx.x) * VEC;
+            const int i = (p * THREADS + (int)threadIdx.x) * VEC;
             if (i >= nv) continue;
             float z[VEC];
 #pragma unroll
@@ -110,20 +132,11 @@ __global__ __launch_bounds__(SC_THREADS) void scores_kernel(const T* in, T* out,
                 }
             }
             if (a.bias) {
-                const float* bias = a.bias + b * a.ld_bias + v0 + i;
-                float add[VEC];
-                if (i + VEC <= nv) __builtin_memcpy(add, bias, sizeof(add));
-                else
 #pragma unroll
-                    for (int k = 0; k < VEC; ++k) add[k] = i + k < nv ? bias[k] : 0.0f;
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) z[k] += add[k];
+                for (int k = 0; k < VEC; ++k) z[k] += add[p][k];
             }
-            if (a.allowed) {                               // VEC candidates lie in one word
-                const uint32_t bits = a.allowed[b * a.ld_allowed + ((v0 + i) >> 5)] >> ((v0 + i) & 31);
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) z[k] = bits >> k & 1 ? z[k] : -__builtin_inff();
-            }
+            for (int k = 0; k < VEC; ++k) z[k] = bits[p] >> k & 1 ? z[k] : -__builtin_inff();
             Raw o;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) o.v[k] = narrow<T>(z[k]);
@@ -142,15 +155,18 @@ void launch_scores(const dcarl_scores_t& s, void* out, int64_t ld_out, hipStream
     with_type(s.type, [&](auto t) {
         using T = decltype(t);
         if constexpr (!__is_same(T, double)) {
-            // short tiles while they are what fills the GPU, long ones (a quarter of the readings of each history) where there are enough of those
             const unsigned rows = (unsigned)(s.B < 65535 ? s.B : 65535);
-            auto go = [&](auto ept) {
-                constexpr int tile = ept() * SC_THREADS;
-                hipLaunchKernelGGL((scores_kernel<T, ept()>), dim3((unsigned)((s.V + tile - 1) / tile), rows), dim3(SC_THREADS), 0, st,
-                                   (const T*)s.scores, (T*)out, a);
+            auto go = [&](auto threads) {
+                constexpr int tile = SC_EPT * threads();
+                const dim3 grid((unsigned)((s.V + tile - 1) / tile), rows);
+                if (a.id_wide) hipLaunchKernelGGL((scores_kernel<T, int64_t, threads()>), grid, dim3(threads()), 0, st, (const T*)s.scores, (T*)out, a);
+                else hipLaunchKernelGGL((scores_kernel<T, int32_t, threads()>), grid, dim3(threads()), 0, st, (const T*)s.scores, (T*)out, a);
             };
-            if (s.B * ((s.V + 8191) / 8192) >= 1024) go(std::integral_constant<int, 32>{});
-            else go(std::integral_constant<int, 8>{});
+            // Every tile reads the whole history of its row.  512 threads read it half as often, 256 leave more workgroups to wait side by side:
+            // 256 rows of 151643 f32, histories of 1000: 82 (256) and 85 us (512); of 2000: 91 and 88; of 8000: 121 and 111.
+            using std::integral_constant;
+            if (s.taken_off && s.n_taken / s.B >= 1536) go(integral_constant<int, 512>{});
+            else go(integral_constant<int, 256>{});
         }
     });
 }
