@@ -26,6 +26,13 @@ template <typename T, int VEC> __device__ __forceinline__ RowVec<T, VEC> row_loa
     return r;
 }
 
+// a result that nothing here reads again: past the caches (DCARL streams, common.h), at any alignment of the type
+typedef unsigned row_u4 __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T, int VEC> __device__ __forceinline__ void row_store(T* p, const RowVec<T, VEC>& r) {
+    if constexpr (sizeof(r) == 16) __builtin_nontemporal_store(__builtin_bit_cast(row_u4, r), reinterpret_cast<row_u4*>(p));
+    else __builtin_memcpy(p, &r, sizeof(r));
+}
+
 // A workgroup is `lanes` threads along a row (VEC channels each) times 256 / lanes rows; blockIdx.y: 256 * VEC channels each.  The last thread
 // of a row moves back to whole vectors: the same channels as its neighbour, the same values.
 struct RowLane {
@@ -70,7 +77,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_gather_kernel(const T* table,
             RowVec<T, VEC> o;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) o.v[i] = in ? narrow<T>(widen(v[j].v[i]) * (Acc)scale) : narrow<T>(0.0f);
-            if (n < N) __builtin_memcpy(out + n * D + l.cb, &o, sizeof(o));
+            if (n < N) row_store(out + n * D + l.cb, o);
         }
     }
 }
@@ -153,6 +160,7 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(const void* ids, int 
     uint32_t all = 0, before = 0;              // of digit `tid`: items everywhere, items in earlier blocks
     if (total) { all = total[tid]; before = hist[(int64_t)blockIdx.x * RS_BINS + tid]; }
     else
+#pragma unroll 8
         for (int i = 0; i < nblk; ++i) {
             const uint32_t c = hist[(int64_t)i * RS_BINS + tid];
             all += c;
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
         RowVec<T, VEC> o;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o.v[i] = narrow<T>(sum[i] * (Acc)scale);
-        __builtin_memcpy(grad + s * D + l.cb, &o, sizeof(o));
+        row_store(grad + s * D + l.cb, o);
     };
     const int64_t s0 = (int64_t)blockIdx.x * l.R * ROWS;
     const int rows = l.R * ROWS;
