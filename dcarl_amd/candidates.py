@@ -46,6 +46,24 @@ def _per_row(name, t, B, width, dtype):
     return _seq.rows_of(t)
 
 
+def _half_over(scores, out) -> bool:
+    """Whether rows of out share memory with other places of scores (out being scores itself is fine)."""
+    B, V = scores.shape
+    if not (B and V) or out.device != scores.device or (out.data_ptr() == scores.data_ptr() and (B == 1 or out.stride(0) == scores.stride(0)) and (V == 1 or scores.stride(1) == 1)):
+        return False
+    if V > 1 and scores.stride(1) != 1 or scores.stride(0) < 0:
+        return False                                         # read from a copy
+    size = scores.element_size()
+    a0, b0 = scores.data_ptr(), out.data_ptr()
+    la, lb = scores.stride(0), out.stride(0)
+    if a0 + ((B - 1) * la + V) * size <= b0 or b0 + ((B - 1) * lb + V) * size <= a0:
+        return False
+    if B > 1 and la == lb and (b0 - a0) % size == 0:         # side by side in one wider buffer
+        d = (b0 - a0) // size % la
+        return d < V or la - d < V
+    return True
+
+
 def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, out=None,
            validate: bool = False):
     """For each of B rows of V scores:  z = score;  taken before: z = z / r if z > 0 else z * r;  z -= f * n + p where n > 0;
@@ -62,8 +80,8 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
         raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
     if scores.dim() != 2:
         raise ValueError(f"scores must be (B, V), not {tuple(scores.shape)}")
-    if torch.is_grad_enabled() and scores.requires_grad:
-        raise ValueError("adjust has no gradient: detach the scores")
+    if _seq.wants_gradient(scores, *(t for t in (repetition, frequency, presence, bias) if isinstance(t, torch.Tensor))):
+        raise ValueError("adjust has no gradient: detach the scores, strengths and biases")
     B, V = scores.shape
     if (taken is None) != (taken_off is None):
         raise ValueError("taken and taken_off come together")
@@ -84,8 +102,10 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
             raise ValueError(f"out must be a {scores.dtype} tensor {tuple(scores.shape)}")
         if V > 1 and out.stride(1) != 1 or B > 1 and out.stride(0) < V:
             raise ValueError("out must have contiguous rows that do not overlap")
-        if torch.is_grad_enabled() and out.requires_grad:
+        if out.requires_grad:
             raise ValueError("out requires a gradient")
+        if _half_over(scores, out):
+            raise ValueError("out lies partly over scores: it is scores itself or apart from it")
     dev = _seq.on_device(("scores", scores), ("taken", taken), ("taken_off", off), ("given", given), ("repetition", rep), ("frequency", freq),
                          ("presence", pres), ("bias", bias), ("allowed", allowed), ("out", out))
     return _seq.run_on(dev, _adjust, scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias, ld_bias, allowed, ld_allowed, out)

@@ -1048,6 +1048,7 @@ int32_t dcarl_index_states_f64(const double* obs, int64_t N, int32_t D, const do
 
 // ---- sequence operators ------------------------------------------------------------------------------------------------
 constexpr int64_t SEQ_MAX = (int64_t)1 << 31;          // steps, channels, episodes, rows, ids of one call
+constexpr int64_t SEQ_MAX_WIDE = (int64_t)1 << 23;     // channels of a table row: 65535 blocks of 256 threads and more
 constexpr int64_t SEQ_MAX_ELEMENTS = (int64_t)1 << 40; // of one operand: a launch's workgroups stay below 2^31
 
 static int check_seq(const char* who, int32_t type, int64_t n, int64_t d, int64_t e) {
@@ -1118,6 +1119,7 @@ int32_t dcarl_rows_gather(const void* table, int32_t type, int64_t ld, int64_t S
     if (int rc = check_seq(who, type, N, D, S)) return rc;
     if (int rc = check_ld(who, "ld", ld)) return rc;
     if (id_bytes != 4 && id_bytes != 8) return fail(DCARL_EINVAL, "%s: id_bytes=%d is neither 4 nor 8", who, id_bytes);
+    if (D > SEQ_MAX_WIDE) return fail(DCARL_EINVAL, "%s: D=%lld above %lld", who, (long long)D, (long long)SEQ_MAX_WIDE);
     if (N == 0 || D == 0) return DCARL_OK;
     if ((S && !table) || !ids || !out) return fail(DCARL_EINVAL, "%s: NULL argument", who);
     dcarl::launch_rows_gather(type, table, ld, S, ids, id_bytes, N, D, scale, out, static_cast<hipStream_t>(stream));
@@ -1130,6 +1132,7 @@ int32_t dcarl_rows_gradient(const void* dout, int32_t type, int64_t ldd, const v
     if (int rc = check_seq(who, type, N, D, S)) return rc;
     if (int rc = check_ld(who, "ldd", ldd)) return rc;
     if (id_bytes != 4 && id_bytes != 8) return fail(DCARL_EINVAL, "%s: id_bytes=%d is neither 4 nor 8", who, id_bytes);
+    if (D > SEQ_MAX_WIDE) return fail(DCARL_EINVAL, "%s: D=%lld above %lld", who, (long long)D, (long long)SEQ_MAX_WIDE);
     if (S == 0 || D == 0) return DCARL_OK;
     if ((N && (!dout || !ids)) || !workspace || !grad) return fail(DCARL_EINVAL, "%s: NULL argument", who);
     if (!aligned16(workspace)) return fail(DCARL_EINVAL, "%s: workspace needs 16-byte alignment", who);

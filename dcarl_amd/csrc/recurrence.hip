@@ -89,7 +89,7 @@ int64_t recurrence_states_bytes(int64_t N, int64_t D, int64_t, int type, int gat
 template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, const RecPlan& p, char* plan, char* ws) {
     using Acc = typename SeqType<T>::Acc;
     RecWalk<T> a{};
-    a.N = r.N; a.D = r.D; a.E = r.E; a.ep_off = r.ep_off; a.reverse = r.reverse; a.tiles = p.tiles; a.blocks = p.blocks;
+    a.N = r.N; a.D = r.D; a.E = r.E; a.ep_off = r.ep_off; a.reverse = r.reverse; a.past = r.D * sizeof(T) % 128 == 0; a.tiles = p.tiles; a.blocks = p.blocks;
     a.x = static_cast<const T*>(r.x); a.ldx = (uint32_t)r.ldx;
     a.g = r.gate_kind ? static_cast<const T*>(r.gate) : nullptr; a.ldg = (uint32_t)r.ldg;
     a.h0 = static_cast<const T*>(r.h0); a.ldh0 = r.ldh0;

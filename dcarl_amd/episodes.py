@@ -121,6 +121,8 @@ def _recurrence_backward(x, gate, ep_off, h0, gate_value, reverse, states, dh, d
     ws = _bytes(lib.dcarl_recurrence_workspace_bytes(a.N, a.D, a.E, a.type, a.gate_kind), dev)
     _lib.check(lib.dcarl_recurrence_backward(C.byref(a), _seq.at(states), _seq.at(ws), _seq.at(dh), lddh, _seq.at(dlast), _seq.at(dx),
                                              _seq.at(dgate), _seq.at(dh0), _seq.stream(dev)), "dcarl_recurrence_backward")
+    if a.D == 0 and dgate is not None:
+        dgate.zero_()                                        # a sum over no channels
     return dx, dgate, dh0
 
 
@@ -130,11 +132,14 @@ class _Recurrence(torch.autograd.Function):
         h, last, states = _seq.run_on(x.device, _recurrence_forward, x, gate, ep_off, h0, gate_value, reverse, want_last, True)
         ctx.save_for_backward(x, gate, h0, ep_off, states)
         ctx.rest = gate_value, reverse
+        ctx.captured = _seq.capturing()
         return (h, last) if want_last else h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast=None):
+        if not ctx.captured and _seq.capturing():
+            raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
         x, gate, h0, ep_off, states = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dgate, dh0 = _seq.run_on(x.device, _recurrence_backward, x, gate, ep_off, h0, *ctx.rest, states, dh, dlast, need[:3])
@@ -153,8 +158,10 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
     validate: check ep_off's values; where it lies on the GPU this waits for it.  ``validate=False`` never waits and is what a captured call
     needs; offsets that do not rise from 0 to at most N then give unspecified results (and no access out of range).
 
-    Everything runs on the tensors' device and its current stream; nothing is kept between calls.  A backward pass that is to be captured
-    into a graph goes through ``torch.autograd.grad`` of a forward pass captured with it, with no other graph of the same leaves alive."""
+    Everything runs on the tensors' device and its current stream; nothing is kept between calls.  The gradient has no gradient of its own.
+    A backward pass can be captured into a graph together with its forward pass, through ``torch.autograd.grad``; by itself, of a forward pass
+    that ran outside, it is refused.  (``Tensor.backward`` inside a capture while an eager graph of the same leaves is alive makes autograd wait
+    for the eager stream, which ends the process: capture with leaves of their own, as ``torch.autograd.grad`` on detached tensors has.)"""
     code = _seq.type_code("x", x)
     flat = x.dim() == 1
     if x.dim() not in (1, 2):
@@ -197,7 +204,10 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
 
 def discounted_returns(rew, ep_off, gamma: float = 0.95, *, validate: bool = True):
     """``R[t] = rew[t] + gamma * R[t+1]`` to the end of each episode: the cumulative-reward column for a discount, where ``nstep_backup``
-    has the field recorder's ten-step rule.  rew: (N,) tensor on the GPU; float64 sums for float64 rewards."""
+    has the field recorder's ten-step rule.  rew: (N,) (or (N, D): D streams side by side), a tensor of a type of ``gated_recurrence`` or anything
+    that becomes a float64 one; moved to the GPU where it lies elsewhere."""
     if not isinstance(rew, torch.Tensor):
         rew = _dev64(rew, _lib.require_gpu())
+    elif rew.device.type != "cuda":
+        rew = rew.to(_lib.require_gpu())
     return gated_recurrence(rew, float(gamma), ep_off, reverse=True, validate=validate)

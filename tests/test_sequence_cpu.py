@@ -147,11 +147,25 @@ S = torch.zeros(2, 40)
     (S, dict(out=S.half()), ValueError, "out must be"),
     (S, dict(out=torch.zeros(1, 40).expand(2, 40)), ValueError, "overlap"),
     (S, dict(out=torch.zeros(40, 2).t()), ValueError, "contiguous rows"),
+    (S, dict(out=torch.zeros(2, 40, requires_grad=True)), ValueError, "out requires"),
+    (S, dict(bias=torch.zeros(40, requires_grad=True)), ValueError, "no gradient"),
+    (S, dict(presence=torch.zeros(2, requires_grad=True)), ValueError, "no gradient"),
     (S, {}, DcarlError, "no CPU path"),
 ])
 def test_adjust_refusals(scores, kw, error, text):
     with pytest.raises(error, match=text):
         candidates.adjust(scores, **kw)
+
+
+def test_adjust_refuses_out_half_over_scores():
+    wide = torch.zeros(4, 100)
+    for s, o in ((wide[:, :40], wide[:, 39:79]), (wide[:, 10:50], wide[:, :40]), (wide[:, 60:], wide[1:, :40]), (wide[:3, :40], wide[1:, :40]), (wide[0:1, :40], wide[0:1, 20:60])):
+        if s.shape == o.shape:
+            with pytest.raises(ValueError, match="partly over"):
+                candidates.adjust(s, out=o)
+    for s, o in ((wide[:, :40], wide[:, 40:80]), (wide[:, 60:], wide[:, :40]), (wide[:2, :40], wide[2:, :40]), (wide[:, :40], wide[:, :40]), (wide[0:1, :40], wide[0:1, 40:80])):
+        with pytest.raises(DcarlError, match="no CPU path"):            # past every other check
+            candidates.adjust(s, out=o)
 
 
 # ---- the C-ABI: refused before any launch (the addresses are fakes) --------------------------------------------------------
@@ -171,18 +185,20 @@ def test_c_abi_refusals():
     for kw, text in ((dict(type=4), "type=4"), (dict(N=-1), "out of range"), (dict(N=1 << 31), "out of range"), (dict(N=1 << 30, D=1 << 30), "out of range"),
                      (dict(gate_kind=3), "gate_kind"), (dict(ldx=-1), "ldx"), (dict(ep_off=0), "ep_off"), (dict(x=0), "x / gate"), (dict(gate=0), "x / gate")):
         assert fwd(rec(**kw)) == -1 and text in err(), kw
+    assert fwd(rec(ldx=1 << 40)) == -1 and fwd(rec(ldg=1 << 40)) == -1 and "ldg" in err()
     assert lib.dcarl_recurrence_forward(None, null, one, one, null, null) == -1
     assert fwd(rec(), h=null) == -1 and "h is NULL" in err()
     assert fwd(rec(), states=odd) == -1 and "alignment" in err()
     assert fwd(rec(N=0, E=0)) == 0 and fwd(rec(D=0)) == 0
     bwd = lambda r, dh=one, lddh=3, dg=null, st=one: lib.dcarl_recurrence_backward(r, st, one, dh, lddh, null, one, dg, null, null)      # noqa: E731
     assert bwd(rec(gate_kind=0), dg=one) == -1 and "no gradient" in err()
-    assert bwd(rec(), dh=null) == -1 and bwd(rec(), st=null) == -1 and bwd(rec(), lddh=-3) == -1
+    assert bwd(rec(), dh=null) == -1 and bwd(rec(), st=null) == -1 and bwd(rec(), lddh=-3) == bwd(rec(), lddh=1 << 40) == -1
     assert lib.dcarl_recurrence_workspace_bytes(-1, 3, 2, 1, 2) == 0 and lib.dcarl_recurrence_states_bytes(4, 3, 2, 9, 2) == 0
 
     g = lambda t=one, ty=1, ld=3, ids=one, ib=8, n=4, out=one: lib.dcarl_rows_gather(t, ty, ld, 5, ids, ib, n, 3, 1.0, out, null)      # noqa: E731
     assert g(t=null) == g(ids=null) == g(out=null) == g(ty=7) == g(ib=2) == g(ld=-1) == g(n=-4) == -1 and g(n=0) == 0
     gr = lambda d=one, ids=one, ws=one, out=one, n=4, s=5: lib.dcarl_rows_gradient(d, 1, 3, ids, 4, n, 3, s, 1.0, ws, out, null)      # noqa: E731
+    assert lib.dcarl_rows_gather(one, 1, 3, 5, one, 8, 4, (1 << 23) + 1, 1.0, one, null) == -1 and "above" in err()
     assert gr(d=null) == gr(ids=null) == gr(ws=null) == gr(out=null) == gr(s=-5) == -1 and gr(ws=odd) == -1 and "alignment" in err() and gr(s=0) == 0
     assert lib.dcarl_rows_workspace_bytes(1 << 31, 5, 3, 1) == 0 and lib.dcarl_rows_workspace_bytes(100, 5, 3, 1) > 0
 

@@ -197,6 +197,34 @@ def test_recurrence_episodes_do_not_touch(dc):
             assert torch.equal(clean[3][[0, 2, 4]], got[3][[0, 2, 4]])
 
 
+def test_recurrence_odd_calls(dc):
+    off = [0, 3, 5]
+    x, g = torch.randn(5, 4, device="cuda", requires_grad=True), torch.rand(5, device="cuda", requires_grad=True)
+    h = dc.episodes.gated_recurrence(x, g, off)
+    d, = torch.autograd.grad((h * h).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        d.sum().backward()
+    h = dc.episodes.gated_recurrence(x, g, off)
+    a = torch.autograd.grad(h.sum(), (x, g), retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, torch.autograd.grad(h.sum(), (x, g))))        # twice through one graph
+    assert torch.equal(a[0], torch.autograd.grad(dc.episodes.gated_recurrence(x, g.detach(), off).sum(), x)[0])
+    assert torch.equal(a[1], torch.autograd.grad(dc.episodes.gated_recurrence(x.detach(), g, off).sum(), g)[0])
+    h = dc.episodes.gated_recurrence(x, g, off)
+    with torch.no_grad():
+        g.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        h.sum().backward()
+    none = torch.zeros(5, 0, device="cuda")
+    leaf = torch.ones(5, device="cuda", requires_grad=True)
+    h, last = dc.episodes.gated_recurrence(none, leaf, off, torch.zeros(2, 0, device="cuda"), want_last=True)
+    assert h.shape == (5, 0) and last.shape == (2, 0) and not torch.autograd.grad(h.sum() + last.sum(), leaf)[0].any()
+    # only the last states are used, and h of steps that nothing depends on
+    x2 = torch.randn(5, 4, device="cuda", requires_grad=True)
+    _, last = dc.episodes.gated_recurrence(x2, 0.5, off, want_last=True)
+    dx, = torch.autograd.grad(last.sum(), x2)
+    assert torch.equal(dx[:, 0].cpu(), torch.tensor([0.25, 0.5, 1.0, 0.5, 1.0]))
+
+
 def test_recurrence_gradcheck(dc):
     off = ragged([3, 0, 5, 1])
     for kind in ("full", "step"):
@@ -511,6 +539,16 @@ def test_captured_and_replayed(dc):
             dc.tables.lookup(static["rows"], ids)
     torch.cuda.synchronize()
     assert bits.shape == (5, 3)
+    leaf = static["rows"].detach().requires_grad_()
+    eager = dc.episodes.gated_recurrence(leaf, 0.5, torch.tensor([0, 40], device="cuda"), validate=False)
+    grad = torch.ones_like(eager)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="outside of the graph"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            static["rows"].mul(1.0)
+            dc.episodes._Recurrence.backward(eager.grad_fn, grad)
+    torch.cuda.synchronize()
 
 
 def test_offsets_beyond_32_bits(dc):
