@@ -13,19 +13,9 @@ __global__ __launch_bounds__(256) void rec_walk_kernel(const int64_t* off, int64
     for (int64_t i = r; i < blocks; i += all) ticket[i * REC_TICKET] = 0;
     for (int64_t i = r; i < clear16; i += all) clear[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
     if (r >= N || !off) return;
-    const int64_t t = reverse ? N - 1 - r : r;
-    int64_t lo = 0, hi = E + 1;                            // the first offset above t
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (off[mid] <= t) lo = mid + 1; else hi = mid;
-    }
-    const bool out = lo == 0 || lo > E;
-    const int64_t e = out ? 0 : lo - 1;
-    int f = REC_OUT;
-    if (!out) {
-        const bool first = t == off[e], last = t == off[e + 1] - 1;
-        f = ((reverse ? last : first) ? REC_START : 0) | ((reverse ? first : last) ? REC_END : 0);
-    }
+    int64_t e;
+    const int f = rec_find(off, E, N, reverse, r, e);
+    const bool out = f & REC_OUT;
     flag[r] = (uint8_t)f;
     ep[r] = (int32_t)e;
     // (held inside the walk whatever the offsets say: a tile waits for tiles between itself and these)
@@ -128,7 +118,7 @@ void launch_recurrence_forward(const dcarl_recurrence_t& r, void* states, void* 
     const RecPlan p = rec_plan(r.N, r.D, r.type, r.gate_kind);
     char* ws = static_cast<char*>(workspace);
     char* plan = states ? static_cast<char*>(states) : ws + p.ws_plan;
-    rec_launch_walk(r, p, r.ep_off, plan, ws, st);
+    if (p.tiles > 1) rec_launch_walk(r, p, r.ep_off, plan, ws, st);
     with_type(r.type, [&](auto t) {
         using T = decltype(t);
         RecWalk<T> a = rec_walk<T>(r, p, plan, ws);

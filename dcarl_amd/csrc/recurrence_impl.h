@@ -90,6 +90,40 @@ __device__ __forceinline__ int64_t rec_ep_end(const int64_t* off, int64_t e, int
     return s < 0 ? 0 : s > N ? N : s;
 }
 
+// flags and episode of step r of the walk
+__device__ __forceinline__ int rec_find(const int64_t* off, int64_t E, int64_t N, int reverse, int64_t r, int64_t& e) {
+    const int64_t t = reverse ? N - 1 - r : r;
+    int64_t lo = 0, hi = E + 1;                            // the first offset above t
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (off[mid] <= t) lo = mid + 1; else hi = mid;
+    }
+    const bool out = lo == 0 || lo > E;
+    e = out ? 0 : lo - 1;
+    if (out) return REC_OUT;
+    const bool first = t == off[e], last = t == off[e + 1] - 1;
+    return ((reverse ? last : first) ? REC_START : 0) | ((reverse ? first : last) ? REC_END : 0);
+}
+
+// A call of one tile (one step of every live episode, short batches) finds its flags itself, in LDS, and saves the launch that finds them for longer ones.
+template <int TILE> struct RecOwn {
+    uint64_t flag[TILE / 8 + 1];
+    int32_t ep[TILE];
+};
+template <typename T, int TILE> __device__ __forceinline__ void rec_own(const RecWalk<T>& a, RecOwn<TILE>& own) {
+    if (a.tiles != 1) return;
+    uint8_t* flag = reinterpret_cast<uint8_t*>(own.flag);
+    for (int r = threadIdx.x; r < (int)a.N; r += REC_THREADS) {
+        int64_t e;
+        flag[r] = (uint8_t)rec_find(a.ep_off, a.E, a.N, a.reverse, r, e);
+        own.ep[r] = (int32_t)e;
+    }
+    __syncthreads();
+}
+template <typename T, int TILE> __device__ __forceinline__ int64_t rec_ep(const RecWalk<T>& a, const RecOwn<TILE>& own, int64_t r) {
+    return a.tiles == 1 ? own.ep[r] : a.ep[r];
+}
+
 // one thread's steps of a tile
 template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
     using Acc = typename SeqType<T>::Acc;
@@ -99,18 +133,21 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
     uint64_t fl;
     int n;                                                 // steps that exist
     // lr: the thread's first step within the tile; at(k): where its k-th lies among the tile's rows in memory
-    __device__ __forceinline__ void load(const RecWalk<T>& a, const RecSpan& w, int tile_rows, int lr, uint32_t cb) {
+    template <int TILE> __device__ __forceinline__ void load(const RecWalk<T>& a, const RecSpan& w, const RecOwn<TILE>& own, int lr, uint32_t cb) {
         const int left = w.rows - lr;
         n = left < 0 ? 0 : left > K ? K : left;
         fl = 0;
-        if (n > 0) __builtin_memcpy(&fl, a.flag + w.row0 + lr, K);       // the array has K bytes of room behind it
+        if (n > 0) {                                       // (both arrays have K bytes of room behind them)
+            if (a.tiles == 1) __builtin_memcpy(&fl, reinterpret_cast<const uint8_t*>(own.flag) + lr, K);
+            else __builtin_memcpy(&fl, a.flag + w.row0 + lr, K);
+        }
         if (n < K) fl = n <= 0 ? 0 : fl & ((1ull << (8 * n)) - 1);
         const T *xb = a.x + w.low * (int64_t)a.ldx, *gb = a.g ? a.g + w.low * (int64_t)a.ldg : nullptr;
         const T* db = BACK ? a.dh + w.low * (int64_t)a.lddh : nullptr;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int l = lr + k < w.rows ? lr + k : w.rows - 1;         // steps that do not exist repeat the last
-            const uint32_t at = (uint32_t)(a.reverse ? tile_rows - 1 - l : l);
+            const uint32_t at = (uint32_t)(a.reverse ? TILE - 1 - l : l);
             x[k] = rec_load<T, VEC>(xb, at * a.ldx + cb);
             if constexpr (GK == 2) g[k] = rec_load<T, VEC>(gb, at * a.ldg + cb);
             else if (a.g) gs[k] = rec_load<T, 1>(gb, at * a.ldg).v[0];
@@ -204,8 +241,8 @@ __device__ __forceinline__ void rec_carry(const RecMap<Acc, VEC>& m, const RecSh
 }
 
 // the thread's steps as one map, forward in time
-template <typename T, int C, int VEC, int GK, bool BACK>
-__device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecTile<T, C, VEC, GK, BACK>& t, int64_t r0, uint32_t cb,
+template <typename T, int C, int VEC, int GK, bool BACK, int TILE>
+__device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecOwn<TILE>& own, const RecTile<T, C, VEC, GK, BACK>& t, int64_t r0, uint32_t cb,
                                                 RecMap<typename SeqType<T>::Acc, VEC>& m) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>;
@@ -229,7 +266,7 @@ __device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecTi
         if (f & REC_START) {
             m.cut = true;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) m.B[v] = a.h0 ? (Acc)widen(a.h0[a.ep[r0 + k] * a.ldh0 + cb + v]) : Acc(0);
+            for (int v = 0; v < VEC; ++v) m.B[v] = a.h0 ? (Acc)widen(a.h0[rec_ep(a, own, r0 + k) * a.ldh0 + cb + v]) : Acc(0);
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -240,8 +277,8 @@ __device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecTi
     }
 }
 // ... and backward: c -> g (dh + c), from behind; an episode's last step takes dlast instead of what comes from behind it
-template <typename T, int C, int VEC, int GK>
-__device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecTile<T, C, VEC, GK, true>& t, int64_t r0, uint32_t cb,
+template <typename T, int C, int VEC, int GK, int TILE>
+__device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecOwn<TILE>& own, const RecTile<T, C, VEC, GK, true>& t, int64_t r0, uint32_t cb,
                                                  RecMap<typename SeqType<T>::Acc, VEC>& m) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>;
@@ -254,7 +291,7 @@ __device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecT
         if (f & REC_END) {
             m.cut = true;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) m.B[v] = a.dlast ? (Acc)widen(a.dlast[a.ep[r0 + k] * a.D + cb + v]) : Acc(0);
+            for (int v = 0; v < VEC; ++v) m.B[v] = a.dlast ? (Acc)widen(a.dlast[rec_ep(a, own, r0 + k) * a.D + cb + v]) : Acc(0);
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -436,6 +473,7 @@ __global__ __launch_bounds__(REC_THREADS, 4) void rec_forward_kernel(RecWalk<T> 
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share, reach;
+    __shared__ RecOwn<TILE> own;
     __shared__ Acc reached[C * VEC];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
     if (blockIdx.x >= a.tiles * a.blocks) {                                 // the states that empty episodes end with
@@ -454,9 +492,10 @@ __global__ __launch_bounds__(REC_THREADS, 4) void rec_forward_kernel(RecWalk<T> 
     const int lr = (wv * (64 / C) + lane / C) * K;
     const int64_t r0 = w.row0 + lr;
     RecTile<T, C, VEC, GK, false> t;
-    t.load(a, w, TILE, lr, cb);
+    rec_own(a, own);
+    t.load(a, w, own, lr, cb);
     RecMap<Acc, VEC> m;
-    rec_map_forward(a, t, r0, cb, m);
+    rec_map_forward(a, own, t, r0, cb, m);
     rec_scan_wave<Acc, C, VEC, 1>(m, share, lane, wv);
     __syncthreads();
     const bool first = wv == 0 && lane < C && mine;        // the threads that publish
@@ -481,7 +520,7 @@ __global__ __launch_bounds__(REC_THREADS, 4) void rec_forward_kernel(RecWalk<T> 
             if (k >= t.n) continue;
             if (t.flag(k) & REC_START) {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[a.ep[r0 + k] * a.ldh0 + cb + v]) : Acc(0);
+                for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[rec_ep(a, own, r0 + k) * a.ldh0 + cb + v]) : Acc(0);
             }
         }
         RecRaw<T, VEC> o;
@@ -496,7 +535,7 @@ __global__ __launch_bounds__(REC_THREADS, 4) void rec_forward_kernel(RecWalk<T> 
         }
         if (mine) {
             rec_store(hb, (uint32_t)(a.reverse ? TILE - 1 - lr - k : lr + k) * (uint32_t)a.D + cb, o, a.past);
-            if (a.last && !plain && (t.flag(k) & REC_END)) __builtin_memcpy(a.last + a.ep[r0 + k] * a.D + cb, &o, sizeof(o));
+            if (a.last && !plain && (t.flag(k) & REC_END)) __builtin_memcpy(a.last + rec_ep(a, own, r0 + k) * a.D + cb, &o, sizeof(o));
         }
     }
 }
@@ -506,6 +545,7 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __i
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share_b, share_f, reach;
+    __shared__ RecOwn<TILE> own;
     __shared__ Acc reached[C * VEC];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane % C;
     if (blockIdx.x >= a.tiles * a.blocks) {                                // an empty episode hands its dlast through
@@ -524,14 +564,15 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __i
     const int lr = (wv * (64 / C) + lane / C) * K;
     const int64_t r0 = w.row0 + lr;
     RecTile<T, C, VEC, GK, true> t;
-    t.load(a, w, TILE, lr, cb);
+    rec_own(a, own);
+    t.load(a, w, own, lr, cb);
     Acc state[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) state[v] = a.state[tile * a.D + cb + v];
     RecMap<Acc, VEC> mb, mf;
-    rec_map_backward(a, t, r0, cb, mb);
+    rec_map_backward(a, own, t, r0, cb, mb);
     rec_scan_wave<Acc, C, VEC, -1>(mb, share_b, lane, wv);
-    rec_map_forward(a, t, r0, cb, mf);
+    rec_map_forward(a, own, t, r0, cb, mf);
     rec_scan_wave<Acc, C, VEC, 1>(mf, share_f, lane, wv);
     __syncthreads();
     const bool first = wv == 0 && lane < C && mine;
@@ -551,7 +592,7 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __i
     for (int k = 0; k < K; ++k) {                          // the states before each step once more, in 32 bits
         if (k < t.n && (t.flag(k) & REC_START)) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[a.ep[r0 + k] * a.ldh0 + cb + v]) : Acc(0);
+            for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[rec_ep(a, own, r0 + k) * a.ldh0 + cb + v]) : Acc(0);
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -568,7 +609,7 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __i
         const int f = t.flag(k);
         if (f & REC_END) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) back[v] = a.dlast ? (Acc)widen(a.dlast[a.ep[r0 + k] * a.D + cb + v]) : Acc(0);
+            for (int v = 0; v < VEC; ++v) back[v] = a.dlast ? (Acc)widen(a.dlast[rec_ep(a, own, r0 + k) * a.D + cb + v]) : Acc(0);
         }
         RecRaw<T, VEC> ox, og;
 #pragma unroll
@@ -591,7 +632,7 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __i
                 RecRaw<T, VEC> o0;
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) o0.v[v] = narrow<T>(back[v]);
-                __builtin_memcpy(a.dh0 + a.ep[r0 + k] * a.D + cb, &o0, sizeof(o0));
+                __builtin_memcpy(a.dh0 + rec_ep(a, own, r0 + k) * a.D + cb, &o0, sizeof(o0));
             }
         }
     }
