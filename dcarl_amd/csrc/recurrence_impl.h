@@ -120,7 +120,7 @@ template <typename T, int TILE> __device__ __forceinline__ void rec_own(const Re
     }
     __syncthreads();
 }
-template <typename T, int TILE> __device__ __forceinline__ int64_t rec_ep(const RecWalk<T>& a, const RecOwn<TILE>& own, int64_t r) {
+template <typename T, int TILE> __device__ __forceinline__ int32_t rec_ep(const RecWalk<T>& a, const RecOwn<TILE>& own, int64_t r) {
     return a.tiles == 1 ? own.ep[r] : a.ep[r];
 }
 
@@ -132,8 +132,7 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
     T gs[GK == 2 ? 1 : K];
     uint64_t fl;
     int n;                                                 // steps that exist
-    // lr: the thread's first step within the tile; at(k): where its k-th lies among the tile's rows in memory
-    template <int TILE> __device__ __forceinline__ void load(const RecWalk<T>& a, const RecSpan& w, const RecOwn<TILE>& own, int lr, uint32_t cb) {
+    template <int TILE> __device__ __forceinline__ void flags(const RecWalk<T>& a, const RecSpan& w, const RecOwn<TILE>& own, int lr) {
         const int left = w.rows - lr;
         n = left < 0 ? 0 : left > K ? K : left;
         fl = 0;
@@ -142,6 +141,9 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
             else __builtin_memcpy(&fl, a.flag + w.row0 + lr, K);
         }
         if (n < K) fl = n <= 0 ? 0 : fl & ((1ull << (8 * n)) - 1);
+    }
+    // lr: the thread's first step within the tile; at(k): where its k-th lies among the tile's rows in memory
+    template <int TILE> __device__ __forceinline__ void load(const RecWalk<T>& a, const RecSpan& w, int lr, uint32_t cb) {
         const T *xb = a.x + w.low * (int64_t)a.ldx, *gb = a.g ? a.g + w.low * (int64_t)a.ldg : nullptr;
         const T* db = BACK ? a.dh + w.low * (int64_t)a.lddh : nullptr;
 #pragma unroll
@@ -160,6 +162,24 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
         else return a.g ? widen(gs[k]) : a.gval;
     }
 };
+
+// Rows of `base` for those of the thread's steps k0 .. k0 + REC_EDGES - 1 that carry `bit`, zeros for the others; all on the way together (one after
+// the other, the rows of one step of 48 episodes took 15 us, like this 9; all K at once spill).
+template <typename T> constexpr int REC_EDGES = sizeof(T) == 2 ? 4 : 2;
+template <typename T, int VEC> struct RecEdges { RecRaw<T, VEC> v[REC_EDGES<T>]; };
+template <typename T, int C, int VEC, int GK, bool BACK, int TILE>
+__device__ __forceinline__ void rec_edges(const RecWalk<T>& a, const RecOwn<TILE>& own, const RecTile<T, C, VEC, GK, BACK>& t, int64_t r0, uint32_t cb,
+                                          const T* base, int64_t ld, int bit, int k0, RecEdges<T, VEC>& o) {
+    int32_t e[REC_EDGES<T>];
+#pragma unroll
+    for (int k = 0; k < REC_EDGES<T>; ++k) e[k] = base && k0 + k < t.n && (t.flag(k0 + k) & bit) ? rec_ep(a, own, r0 + k0 + k) : -1;
+#pragma unroll
+    for (int k = 0; k < REC_EDGES<T>; ++k) {
+        if (base) __builtin_memcpy(&o.v[k], base + (int64_t)(e[k] < 0 ? 0 : e[k]) * ld + cb, sizeof(o.v[k]));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.v[k].v[i] = e[k] < 0 ? narrow<T>(0.0f) : o.v[k].v[i];
+    }
+}
 
 // (A, B) of a run of steps for VEC channels; `cut`: an episode starts inside, nothing from before comes through
 template <typename Acc, int VEC> struct RecMap {
@@ -258,15 +278,19 @@ __device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecOw
             }
         return;
     }
+    RecEdges<T, VEC> h0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
+        if constexpr (!BACK)                               // (the backward pass has no registers to spare for them)
+            if (k % REC_EDGES<T> == 0) rec_edges(a, own, t, r0, cb, a.h0, a.ldh0, REC_START, k, h0);
         if (k >= t.n) continue;
         const int f = t.flag(k);
         if (f & REC_OUT) { m.cut = true; continue; }
         if (f & REC_START) {
             m.cut = true;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) m.B[v] = a.h0 ? (Acc)widen(a.h0[rec_ep(a, own, r0 + k) * a.ldh0 + cb + v]) : Acc(0);
+            for (int v = 0; v < VEC; ++v)
+                m.B[v] = !BACK ? (Acc)widen(h0.v[k % REC_EDGES<T>].v[v]) : a.h0 ? (Acc)widen(a.h0[rec_ep(a, own, r0 + k) * a.ldh0 + cb + v]) : Acc(0);
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
@@ -492,8 +516,9 @@ __global__ __launch_bounds__(REC_THREADS, 4) void rec_forward_kernel(RecWalk<T> 
     const int lr = (wv * (64 / C) + lane / C) * K;
     const int64_t r0 = w.row0 + lr;
     RecTile<T, C, VEC, GK, false> t;
+    t.template load<TILE>(a, w, lr, cb);                   // (on the way while a call of one tile finds its flags)
     rec_own(a, own);
-    t.load(a, w, own, lr, cb);
+    t.flags(a, w, own, lr);
     RecMap<Acc, VEC> m;
     rec_map_forward(a, own, t, r0, cb, m);
     rec_scan_wave<Acc, C, VEC, 1>(m, share, lane, wv);
@@ -514,13 +539,15 @@ __global__ __launch_bounds__(REC_THREADS, 4) void rec_forward_kernel(RecWalk<T> 
     rec_carry<Acc, C, VEC, 1>(m, share, lane, wv, carry, s);
     const bool plain = __all(t.fl == 0 && t.n == K);
     T* hb = a.h + w.low * a.D;
+    RecEdges<T, VEC> h0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         if (!plain) {
+            if (k % REC_EDGES<T> == 0) rec_edges(a, own, t, r0, cb, a.h0, a.ldh0, REC_START, k, h0);
             if (k >= t.n) continue;
             if (t.flag(k) & REC_START) {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) s[v] = a.h0 ? (Acc)widen(a.h0[rec_ep(a, own, r0 + k) * a.ldh0 + cb + v]) : Acc(0);
+                for (int v = 0; v < VEC; ++v) s[v] = widen(h0.v[k % REC_EDGES<T>].v[v]);
             }
         }
         RecRaw<T, VEC> o;
@@ -564,8 +591,9 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __i
     const int lr = (wv * (64 / C) + lane / C) * K;
     const int64_t r0 = w.row0 + lr;
     RecTile<T, C, VEC, GK, true> t;
+    t.template load<TILE>(a, w, lr, cb);                   // (on the way while a call of one tile finds its flags)
     rec_own(a, own);
-    t.load(a, w, own, lr, cb);
+    t.flags(a, w, own, lr);
     Acc state[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) state[v] = a.state[tile * a.D + cb + v];
