@@ -493,7 +493,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
 }
 
 template <typename T, int C, int VEC, int GK>
-__global__ __launch_bounds__(REC_THREADS, 4) void rec_forward_kernel(RecWalk<T> a) {
+__global__ __launch_bounds__(REC_THREADS, GK == 2 && __is_same(T, float) ? 3 : 4) void rec_forward_kernel(RecWalk<T> a) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share, reach;
