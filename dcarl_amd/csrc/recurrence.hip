@@ -54,7 +54,7 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
     p.tiles = (N + p.tile - 1) / p.tile;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t here = at; at += up16(bytes); return here; };
-    p.flag = take(N + 8); p.ep = take(4 * N); p.from = take(4 * p.tiles); p.till = take(4 * p.tiles);
+    p.flag = take(N + 16); p.ep = take(4 * N); p.from = take(4 * p.tiles); p.till = take(4 * p.tiles);
     p.plan_bytes = at;
     p.state = take(p.tiles * D * acc);
     p.states_bytes = at;

@@ -107,7 +107,7 @@ __device__ __forceinline__ int rec_find(const int64_t* off, int64_t E, int64_t N
 
 // A call of one tile (one step of every live episode, short batches) finds its flags itself, in LDS, and saves the launch that finds them for longer ones.
 template <int TILE> struct RecOwn {
-    uint64_t flag[TILE / 8 + 1];
+    uint64_t flag[TILE / 8 + 2];
     int32_t ep[TILE];
 };
 template <typename T, int TILE> __device__ __forceinline__ void rec_own(const RecWalk<T>& a, RecOwn<TILE>& own) {
@@ -130,17 +130,46 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
     static constexpr int K = REC_K<T>;
     RecRaw<T, VEC> x[K], g[GK == 2 ? K : 1], dh[BACK ? K : 1];
     T gs[GK == 2 ? 1 : K];
-    uint64_t fl;
+    uint64_t fl[(K + 7) / 8];                              // a byte each
     int n;                                                 // steps that exist
     template <int TILE> __device__ __forceinline__ void flags(const RecWalk<T>& a, const RecSpan& w, const RecOwn<TILE>& own, int lr) {
         const int left = w.rows - lr;
         n = left < 0 ? 0 : left > K ? K : left;
-        fl = 0;
+#pragma unroll
+        for (int i = 0; i < (K + 7) / 8; ++i) fl[i] = 0;
         if (n > 0) {                                       // (both arrays have K bytes of room behind them)
-            if (a.tiles == 1) __builtin_memcpy(&fl, reinterpret_cast<const uint8_t*>(own.flag) + lr, K);
-            else __builtin_memcpy(&fl, a.flag + w.row0 + lr, K);
+            if (a.tiles == 1) __builtin_memcpy(fl, reinterpret_cast<const uint8_t*>(own.flag) + lr, K);
+            else __builtin_memcpy(fl, a.flag + w.row0 + lr, K);
         }
-        if (n < K) fl = n <= 0 ? 0 : fl & ((1ull << (8 * n)) - 1);
+#pragma unroll
+        for (int i = 0; i < (K + 7) / 8; ++i) {
+            const int have = n - 8 * i;
+            if (have < 8) fl[i] = have <= 0 ? 0 : fl[i] & ((1ull << (8 * have)) - 1);
+        }
+    }
+    // The second walk over the steps widens the 16-bit operands again: without this the compiler keeps the widened ones of the first, twice the registers.
+    __device__ __forceinline__ void again() {
+        if constexpr (sizeof(T) == 2 && VEC == 4) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                hide(x[k]);
+                if constexpr (GK == 2) hide(g[k]);
+                if constexpr (BACK) hide(dh[k]);
+            }
+        }
+    }
+    __device__ __forceinline__ static void hide(RecRaw<T, VEC>& r) {
+        uint64_t u;
+        __builtin_memcpy(&u, &r, sizeof(u));
+        asm volatile("" : "+v"(u));
+        __builtin_memcpy(&r, &u, sizeof(u));
+    }
+    // whether all of the thread's steps exist and none is an episode's edge
+    __device__ __forceinline__ bool inner() const {
+        uint64_t any = 0;
+#pragma unroll
+        for (int i = 0; i < (K + 7) / 8; ++i) any |= fl[i];
+        return any == 0 && n == K;
     }
     // lr: the thread's first step within the tile; at(k): where its k-th lies among the tile's rows in memory
     template <int TILE> __device__ __forceinline__ void load(const RecWalk<T>& a, const RecSpan& w, int lr, uint32_t cb) {
@@ -156,7 +185,7 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
             if constexpr (BACK) dh[k] = rec_load<T, VEC>(db, at * a.lddh + cb);
         }
     }
-    __device__ __forceinline__ int flag(int k) const { return (int)(fl >> (8 * k)) & 7; }
+    __device__ __forceinline__ int flag(int k) const { return (int)(fl[k / 8] >> (8 * (k % 8))) & 7; }
     __device__ __forceinline__ Acc gate(const RecWalk<T>& a, int k, int v) const {
         if constexpr (GK == 2) return widen(g[k].v[v]);
         else return a.g ? widen(gs[k]) : a.gval;
@@ -267,7 +296,7 @@ __device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecOw
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>;
     m.one();
-    if (__all(t.fl == 0 && t.n == K)) {
+    if (__all(t.inner())) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -326,6 +355,9 @@ __device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecO
     }
 }
 
+// wavefronts per SIMD: what each instance's registers allow without a spill
+template <typename T, int GK> constexpr int REC_WAVES_FORWARD = __is_same(T, float) && GK == 2 ? 3 : 4;
+template <typename T, int GK> constexpr int REC_WAVES_BACKWARD = __is_same(T, float) && GK == 2 ? 2 : 3;
 template <int C, typename T> constexpr int REC_TILE = REC_WAVES * (64 / C) * REC_K<T>;
 
 // ---- between workgroups -----------------------------------------------------------------------------------------------------------------
@@ -493,7 +525,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
 }
 
 template <typename T, int C, int VEC, int GK>
-__global__ __launch_bounds__(REC_THREADS, GK == 2 && __is_same(T, float) ? 3 : 4) void rec_forward_kernel(RecWalk<T> a) {
+__global__ __launch_bounds__(REC_THREADS, (REC_WAVES_FORWARD<T, GK>)) void rec_forward_kernel(RecWalk<T> a) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share, reach;
@@ -537,7 +569,8 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && __is_same(T, float) ? 3 : 4
     if (a.state && first)
         for (int v = 0; v < VEC; ++v) a.state[tile * a.D + cb + v] = carry[v];
     rec_carry<Acc, C, VEC, 1>(m, share, lane, wv, carry, s);
-    const bool plain = __all(t.fl == 0 && t.n == K);
+    t.again();
+    const bool plain = __all(t.inner());
     T* hb = a.h + w.low * a.D;
     RecEdges<T, VEC> h0;
 #pragma unroll
@@ -568,7 +601,7 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && __is_same(T, float) ? 3 : 4
 }
 
 template <typename T, int C, int VEC, int GK>
-__global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __is_same(T, f16)) ? 2 : 3) void rec_backward_kernel(RecWalk<T> a) {
+__global__ __launch_bounds__(REC_THREADS, (REC_WAVES_BACKWARD<T, GK>)) void rec_backward_kernel(RecWalk<T> a) {
     using Acc = typename SeqType<T>::Acc;
     constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share_b, share_f, reach;
@@ -616,6 +649,7 @@ __global__ __launch_bounds__(REC_THREADS, GK == 2 && (__is_same(T, float) || __i
     }
     rec_carry<Acc, C, VEC, -1>(mb, share_b, lane, wv, carry, back);
     rec_carry<Acc, C, VEC, 1>(mf, share_f, lane, wv, state, s);
+    t.again();
 #pragma unroll
     for (int k = 0; k < K; ++k) {                          // the states before each step once more, in 32 bits
         if (k < t.n && (t.flag(k) & REC_START)) {
