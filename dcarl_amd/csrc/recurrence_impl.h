@@ -52,7 +52,9 @@ template <typename T> struct RecWalk {
 };
 
 // K consecutive steps of VEC channels per thread (16-byte loads of f32, 8-byte ones of 16-bit types)
-template <typename T> constexpr int REC_K = sizeof(T) == 8 ? 4 : 8;
+// One channel alone: 16 (8) steps, side by side in memory, in 16-byte loads -- fewer tiles to hand out and to chain (4e6 steps of one f32 channel: 79 us with
+// 8 steps, 52 with 16).
+template <typename T, int C> constexpr int REC_K = C == 1 ? (sizeof(T) == 8 ? 8 : 16) : sizeof(T) == 8 ? 4 : 8;
 template <typename T> constexpr int REC_VEC = sizeof(T) == 8 ? 2 : 4;
 
 template <typename T, int VEC> struct RecRaw { T v[VEC]; };
@@ -74,6 +76,27 @@ template <typename T, int VEC> __device__ __forceinline__ void rec_store(T* base
     else if constexpr (sizeof(r) == 8) __builtin_nontemporal_store(__builtin_bit_cast(rec_u2, r), reinterpret_cast<rec_u2*>(p));
 }
 
+// One channel: a thread's K results side by side, `o` in walking order, those from n on do not exist.
+template <typename T, int K> __device__ __forceinline__ void rec_store_row(T* base, int lr, int n, int tile, int reverse, const T (&o)[K], bool past) {
+    if (n == K) {
+        RecRaw<T, K> v;
+#pragma unroll
+        for (int k = 0; k < K; ++k) v.v[k] = o[reverse ? K - 1 - k : k];
+        constexpr int W = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < K; i += W) {
+            RecRaw<T, W> q;
+#pragma unroll
+            for (int k = 0; k < W; ++k) q.v[k] = v.v[i + k];
+            rec_store(base, (uint32_t)(reverse ? tile - lr - K : lr) + i, q, past);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (k < n) base[reverse ? tile - 1 - lr - k : lr + k] = o[k];
+    }
+}
+
 // a workgroup's tile: the steps row0 .. row0 + rows - 1 of the walk, the first of its rows in memory
 struct RecSpan {
     int64_t tile, row0, low;
@@ -90,20 +113,28 @@ __device__ __forceinline__ int64_t rec_ep_end(const int64_t* off, int64_t e, int
     return s < 0 ? 0 : s > N ? N : s;
 }
 
-// flags and episode of step r of the walk
-__device__ __forceinline__ int rec_find(const int64_t* off, int64_t E, int64_t N, int reverse, int64_t r, int64_t& e) {
-    const int64_t t = reverse ? N - 1 - r : r;
-    int64_t lo = 0, hi = E + 1;                            // the first offset above t
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (off[mid] <= t) lo = mid + 1; else hi = mid;
+// the episode around a step, kept while the steps asked for lie in it
+struct RecFind {
+    int64_t lo = 0, hi = 0, e = -1;                        // steps lo .. hi - 1 of the stream; e < 0: they belong to none
+    // flags of step r of the walk
+    __device__ __forceinline__ int at(const int64_t* off, int64_t E, int64_t N, int reverse, int64_t r) {
+        const int64_t t = reverse ? N - 1 - r : r;
+        if (t < lo || t >= hi) {
+            int64_t a = 0, b = E + 1;                      // the first offset above t
+            while (a < b) {
+                const int64_t mid = (a + b) >> 1;
+                if (off[mid] <= t) a = mid + 1; else b = mid;
+            }
+            const bool out = a == 0 || a > E;
+            e = out ? -1 : a - 1;
+            lo = a == 0 ? 0 : off[a - 1];
+            hi = a > E ? N : off[a];
+        }
+        if (e < 0) return REC_OUT;
+        const bool first = t == lo, last = t == hi - 1;
+        return ((reverse ? last : first) ? REC_START : 0) | ((reverse ? first : last) ? REC_END : 0);
     }
-    const bool out = lo == 0 || lo > E;
-    e = out ? 0 : lo - 1;
-    if (out) return REC_OUT;
-    const bool first = t == off[e], last = t == off[e + 1] - 1;
-    return ((reverse ? last : first) ? REC_START : 0) | ((reverse ? first : last) ? REC_END : 0);
-}
+};
 
 // A call of one tile (one step of every live episode, short batches) finds its flags itself, in LDS, and saves the launch that finds them for longer ones.
 template <int TILE> struct RecOwn {
@@ -114,9 +145,9 @@ template <typename T, int TILE> __device__ __forceinline__ void rec_own(const Re
     if (a.tiles != 1) return;
     uint8_t* flag = reinterpret_cast<uint8_t*>(own.flag);
     for (int r = threadIdx.x; r < (int)a.N; r += REC_THREADS) {
-        int64_t e;
-        flag[r] = (uint8_t)rec_find(a.ep_off, a.E, a.N, a.reverse, r, e);
-        own.ep[r] = (int32_t)e;
+        RecFind f;
+        flag[r] = (uint8_t)f.at(a.ep_off, a.E, a.N, a.reverse, r);
+        own.ep[r] = (int32_t)f.e;
     }
     __syncthreads();
 }
@@ -127,11 +158,17 @@ template <typename T, int TILE> __device__ __forceinline__ int32_t rec_ep(const 
 // one thread's steps of a tile
 template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
     using Acc = typename SeqType<T>::Acc;
-    static constexpr int K = REC_K<T>;
+    static constexpr int K = REC_K<T, C>;
     RecRaw<T, VEC> x[K], g[GK == 2 ? K : 1], dh[BACK ? K : 1];
     T gs[GK == 2 ? 1 : K];
     uint64_t fl[(K + 7) / 8];                              // a byte each
     int n;                                                 // steps that exist
+    // K steps of one channel, side by side in memory
+    __device__ __forceinline__ static void row(const T* base, uint32_t at, int reverse, RecRaw<T, 1> (&o)[K]) {
+        const RecRaw<T, K> v = rec_load<T, K>(base, at);
+#pragma unroll
+        for (int k = 0; k < K; ++k) o[k].v[0] = reverse ? v.v[K - 1 - k] : v.v[k];
+    }
     template <int TILE> __device__ __forceinline__ void flags(const RecWalk<T>& a, const RecSpan& w, const RecOwn<TILE>& own, int lr) {
         const int left = w.rows - lr;
         n = left < 0 ? 0 : left > K ? K : left;
@@ -175,6 +212,21 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
     template <int TILE> __device__ __forceinline__ void load(const RecWalk<T>& a, const RecSpan& w, int lr, uint32_t cb) {
         const T *xb = a.x + w.low * (int64_t)a.ldx, *gb = a.g ? a.g + w.low * (int64_t)a.ldg : nullptr;
         const T* db = BACK ? a.dh + w.low * (int64_t)a.lddh : nullptr;
+        if constexpr (C == 1 && VEC == 1) {
+            if (a.ldx == 1 && (!a.g || a.ldg == 1) && (!BACK || a.lddh == 1) && lr + K <= w.rows) {
+                const uint32_t at = (uint32_t)(a.reverse ? TILE - lr - K : lr);
+                row(xb, at, a.reverse, x);
+                if constexpr (GK == 2) row(gb, at, a.reverse, g);
+                else if (a.g) {
+                    RecRaw<T, 1> v[K];
+                    row(gb, at, a.reverse, v);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) gs[k] = v[k].v[0];
+                }
+                if constexpr (BACK) row(db, at, a.reverse, dh);
+                return;
+            }
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int l = lr + k < w.rows ? lr + k : w.rows - 1;         // steps that do not exist repeat the last
@@ -294,7 +346,7 @@ template <typename T, int C, int VEC, int GK, bool BACK, int TILE>
 __device__ __forceinline__ void rec_map_forward(const RecWalk<T>& a, const RecOwn<TILE>& own, const RecTile<T, C, VEC, GK, BACK>& t, int64_t r0, uint32_t cb,
                                                 RecMap<typename SeqType<T>::Acc, VEC>& m) {
     using Acc = typename SeqType<T>::Acc;
-    constexpr int K = REC_K<T>;
+    constexpr int K = REC_K<T, C>;
     m.one();
     if (__all(t.inner())) {
 #pragma unroll
@@ -334,7 +386,7 @@ template <typename T, int C, int VEC, int GK, int TILE>
 __device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecOwn<TILE>& own, const RecTile<T, C, VEC, GK, true>& t, int64_t r0, uint32_t cb,
                                                  RecMap<typename SeqType<T>::Acc, VEC>& m) {
     using Acc = typename SeqType<T>::Acc;
-    constexpr int K = REC_K<T>;
+    constexpr int K = REC_K<T, C>;
     m.one();
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
@@ -358,7 +410,7 @@ __device__ __forceinline__ void rec_map_backward(const RecWalk<T>& a, const RecO
 // wavefronts per SIMD: what each instance's registers allow without a spill
 template <typename T, int GK> constexpr int REC_WAVES_FORWARD = __is_same(T, float) && GK == 2 ? 3 : 4;
 template <typename T, int GK> constexpr int REC_WAVES_BACKWARD = __is_same(T, float) && GK == 2 ? 2 : 3;
-template <int C, typename T> constexpr int REC_TILE = REC_WAVES * (64 / C) * REC_K<T>;
+template <int C, typename T> constexpr int REC_TILE = REC_WAVES * (64 / C) * REC_K<T, C>;
 
 // ---- between workgroups -----------------------------------------------------------------------------------------------------------------
 // a published value as a word that is never the cleared pattern (all ones, a NaN): every NaN is published as the quiet one
@@ -527,7 +579,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
 template <typename T, int C, int VEC, int GK>
 __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_FORWARD<T, GK>)) void rec_forward_kernel(RecWalk<T> a) {
     using Acc = typename SeqType<T>::Acc;
-    constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
+    constexpr int K = REC_K<T, C>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share, reach;
     __shared__ RecOwn<TILE> own;
     __shared__ Acc reached[C * VEC];
@@ -573,6 +625,7 @@ __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_FORWARD<T, GK>)) void rec_f
     const bool plain = __all(t.inner());
     T* hb = a.h + w.low * a.D;
     RecEdges<T, VEC> h0;
+    T line[C == 1 ? K : 1];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         if (!plain) {
@@ -593,17 +646,19 @@ __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_FORWARD<T, GK>)) void rec_f
 #pragma unroll
             for (int v = 0; v < VEC; ++v) { s[v] = 0; o.v[v] = narrow<T>(0.0f); }
         }
+        if constexpr (C == 1) line[k] = o.v[0];
         if (mine) {
-            rec_store(hb, (uint32_t)(a.reverse ? TILE - 1 - lr - k : lr + k) * (uint32_t)a.D + cb, o, a.past);
+            if constexpr (C > 1) rec_store(hb, (uint32_t)(a.reverse ? TILE - 1 - lr - k : lr + k) * (uint32_t)a.D + cb, o, a.past);
             if (a.last && !plain && (t.flag(k) & REC_END)) __builtin_memcpy(a.last + rec_ep(a, own, r0 + k) * a.D + cb, &o, sizeof(o));
         }
     }
+    if constexpr (C == 1) rec_store_row<T, K>(hb, lr, t.n, TILE, a.reverse, line, a.past);
 }
 
 template <typename T, int C, int VEC, int GK>
 __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_BACKWARD<T, GK>)) void rec_backward_kernel(RecWalk<T> a) {
     using Acc = typename SeqType<T>::Acc;
-    constexpr int K = REC_K<T>, TILE = REC_TILE<C, T>;
+    constexpr int K = REC_K<T, C>, TILE = REC_TILE<C, T>;
     __shared__ RecShare<Acc, C, VEC> share_b, share_f, reach;
     __shared__ RecOwn<TILE> own;
     __shared__ Acc reached[C * VEC];
@@ -663,6 +718,7 @@ __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_BACKWARD<T, GK>)) void rec_
         }
     }
     Acc sum[K];
+    T line_x[C == 1 ? K : 1], line_g[C == 1 ? K : 1];
     T *dxb = a.dx + w.low * a.D, *dgb = a.dg + (GK == 2 ? w.low * a.D : w.low);
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
@@ -686,10 +742,11 @@ __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_BACKWARD<T, GK>)) void rec_
 #pragma unroll
             for (int v = 0; v < VEC; ++v) { ox.v[v] = og.v[v] = narrow<T>(0.0f); back[v] = 0; }
         }
+        if constexpr (C == 1) { line_x[k] = ox.v[0]; line_g[k] = og.v[0]; }
         if (mine) {
             const uint32_t at = (uint32_t)(a.reverse ? TILE - 1 - lr - k : lr + k) * (uint32_t)a.D + cb;
-            if (a.dx) rec_store(dxb, at, ox, a.past);
-            if (GK == 2 && a.dg) rec_store(dgb, at, og, a.past);
+            if (C > 1 && a.dx) rec_store(dxb, at, ox, a.past);
+            if (C > 1 && GK == 2 && a.dg) rec_store(dgb, at, og, a.past);
             if (a.dh0 && (f & REC_START)) {
                 RecRaw<T, VEC> o0;
 #pragma unroll
@@ -697,6 +754,10 @@ __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_BACKWARD<T, GK>)) void rec_
                 __builtin_memcpy(a.dh0 + rec_ep(a, own, r0 + k) * a.D + cb, &o0, sizeof(o0));
             }
         }
+    }
+    if constexpr (C == 1) {
+        if (a.dx) rec_store_row<T, K>(dxb, lr, t.n, TILE, a.reverse, line_x, a.past);
+        if (GK == 2 && a.dg) rec_store_row<T, K>(dgb, lr, t.n, TILE, a.reverse, line_g, a.past);
     }
     if constexpr (GK == 1) {
         if (a.dg) {
