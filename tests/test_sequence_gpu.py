@@ -139,6 +139,46 @@ def test_recurrence_many_steps_in_parts(dc):
             check_recurrence(dc, x, gate, off, h0, dh, dl, reverse, t)
 
 
+@pytest.mark.parametrize("D, t", [(1, torch.float32), (1, torch.float64), (1, torch.bfloat16), (3, torch.float32), (20, torch.float32), (18, torch.float64), (70, torch.bfloat16), (130, torch.float16), (9, torch.float32)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_recurrence_whole_numbers_across_tiles_are_exact(dc, D, t, reverse):
+    """Gates of +1 and -1 and small whole numbers: nothing fades, so what passes between tiles and groups of tiles has to be right, and every sum is a
+    whole number that f32 holds, in any order of joining: the results are the definition's, rounded once to the type."""
+    gen = torch.Generator().manual_seed(D)
+    off = ragged([1, 700, 0, 23000, 130, 2048, 4000])                     # 23000 steps: tens of tiles for every width, more than four groups of them
+    N, E = off[-1], len(off) - 1
+    x, dh = (torch.randint(-1, 2, (N, D), generator=gen).to(t) for _ in range(2))
+    h0, dl = (torch.randint(-3, 4, (E, D), generator=gen).to(t) for _ in range(2))
+    for kind in ("full", "step"):
+        gate = (torch.randint(0, 2, (N, D) if kind == "full" else (N,), generator=gen) * 2 - 1).to(t)
+        leaf = [v.cuda().requires_grad_() for v in (x, gate, h0)]
+        h, last = dc.episodes.gated_recurrence(leaf[0], leaf[1], off, leaf[2], reverse=reverse, want_last=True)
+        grads = torch.autograd.grad([h, last], leaf, [dh.cuda(), dl.cuda()])
+        w_h, prev, w_last = so.recurrence(n64(x), n64(gate).reshape(N, -1), off, n64(h0), reverse)
+        wx, wg, w0 = so.recurrence_gradients(n64(dh), n64(gate).reshape(N, -1), prev, off, n64(dl), reverse)
+        wg = wg if kind == "full" else wg.sum(1)
+        assert max(np.abs(v).max() for v in (w_h, wx, wg)) < 2 ** 24      # (f16 holds 65504: what lies beyond is infinite in both)
+        for got, want, what in zip([h, last, *grads], [w_h, w_last, wx, wg, w0], ["h", "last", "dx", "dgate", "dh0"]):
+            assert torch.equal(got.detach().cpu(), torch.from_numpy(want).to(t)), (kind, what)
+
+
+def test_recurrence_side_by_side_on_two_streams(dc):
+    """Two long calls at once, each waiting for its own tiles only."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    off = torch.tensor([0, 60000, 60001, 131072], device="cuda")
+    args = [(torch.randn(131072, D, device="cuda", generator=gen), torch.rand(131072, D, device="cuda", generator=gen) * 0.1 + 0.899) for D in (192, 5)]
+    want = [dc.episodes.gated_recurrence(x, g, off, validate=False) for x, g in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for k, (x, g) in enumerate(args):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(dc.episodes.gated_recurrence(x, g, off, validate=False))
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, a) for w, many in zip(want, got) for a in many)
+
+
 def test_recurrence_rows_behind_and_no_h0(dc):
     off = [0, 6, 40]
     x, gate, _, dh, dl = inputs(90, 20, 2, torch.float32, "full", 3)
