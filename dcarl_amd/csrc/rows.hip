@@ -340,7 +340,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
     for (int r = 0; r < rows && s0 + r < S; ++r) {         // the long ones, the whole workgroup at each: partial sums of their chunks
         const int64_t b = begin[s0 + r], e = begin[s0 + r + 1];
         if (e - b <= RW_CHUNK) continue;
-        const bool very = e - b > RW_CHUNK * RW_SUPER;
+        const bool very = super && e - b > RW_CHUNK * RW_SUPER;
         const int64_t places = very ? RW_CHUNK * RW_SUPER : RW_CHUNK;
         const Acc* from_part = very ? super : part;
         const int64_t c0 = b / places, m = (e - 1) / places - c0 + 1;
@@ -424,7 +424,9 @@ void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* i
         if (N > RW_CHUNK)
             hipLaunchKernelGGL((rows_chunk_kernel<T, V()>), dim3((unsigned)((N + RW_CHUNK - 1) / RW_CHUNK), across), dim3(RW_THREADS), 0, st, k_in,
                                at(p.begin), p_in, (const T*)dout, ldd, N, S, D, lanes, part);
-        if (N > RW_CHUNK * RW_SUPER)
+        // up to 16384 ids the sums take their chunks one by one (256 at most): a launch less
+        if (N <= 8 * RW_CHUNK * RW_SUPER) super = nullptr;
+        else
             hipLaunchKernelGGL((rows_super_kernel<Acc, V()>), dim3((unsigned)((N + RW_CHUNK * RW_SUPER - 1) / (RW_CHUNK * RW_SUPER)), across),
                                dim3(RW_THREADS), 0, st, k_in, at(p.begin), N, S, D, lanes, part, super);
         // Four rows per group of threads where that leaves every CU eight workgroups, one otherwise: 50000 rows of 2 KB 22.6 (four) and 36.9 us (one),
