@@ -110,6 +110,23 @@ __device__ __forceinline__ uint32_t scan256(uint32_t v, uint32_t (&tot)[4]) {
     return v;
 }
 
+// Where this lane's item goes: its digit's next place (place[digit], this wavefront's own) and its rank among the wavefront's items of that digit.
+__device__ __forceinline__ uint32_t digit_place(uint32_t dig, bool live, int lane, uint32_t* place) {
+    unsigned long long same = __ballot(live);
+#pragma unroll
+    for (int j = 0; j < RS_BITS; ++j) {
+        const unsigned long long bit = __ballot((dig >> j) & 1);
+        same &= (dig >> j) & 1 ? bit : ~bit;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    uint32_t to = 0;
+    if (live) to = place[dig];
+    __builtin_amdgcn_wave_barrier();           // every lane has read its digit's place before the first lane of a group moves it on
+    if (live && rank == 0) place[dig] = to + (uint32_t)__popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    return to + rank;
+}
+
 // hist[block][digit]
 __global__ __launch_bounds__(256) void rows_hist_kernel(const void* ids, int wide, const uint32_t* key, int64_t S, int64_t N, int shift, uint32_t* hist) {
     __shared__ uint32_t h[RS_BINS];
@@ -181,23 +198,71 @@ __global__ __launch_bounds__(256) void rows_scatter_kernel(const void* ids, int 
     for (int r = 0; r < RS_ROUNDS; ++r) {
         const bool live = b + r * 64 < N;
         const uint32_t dig = (k[r] >> shift) & (RS_BINS - 1);
-        unsigned long long same = __ballot(live);
-#pragma unroll
-        for (int j = 0; j < RS_BITS; ++j) {
-            const unsigned long long bit = __ballot((dig >> j) & 1);
-            same &= (dig >> j) & 1 ? bit : ~bit;
-        }
-        const int rank = __popcll(same & ((1ull << lane) - 1));
-        uint32_t to = 0;
-        if (live) to = cnt[wv][dig];
-        __builtin_amdgcn_wave_barrier();       // every lane has read its digit's place before the first lane of a group moves it on
-        if (live && rank == 0) cnt[wv][dig] = to + (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
+        const uint32_t to = digit_place(dig, live, lane, cnt[wv]);
         if (live) {
-            key_out[to + rank] = k[r];
-            pos_out[to + rank] = ps[r];
+            key_out[to] = k[r];
+            pos_out[to] = ps[r];
         }
     }
+}
+
+// Up to RS_SMALL ids: every pass in one workgroup, keys and places in LDS between them -- one launch in place of two a pass (a gradient of 256 ids 23.7 -> 19.0 us,
+// of 4096 27.5 -> 22.2).
+constexpr int RS_SMALL = 4096, RS_SMALL_THREADS = 1024, RS_SMALL_ROUNDS = RS_SMALL / RS_SMALL_THREADS, RS_SMALL_WAVES = RS_SMALL_THREADS / 64;
+__global__ __launch_bounds__(RS_SMALL_THREADS) void rows_sort_small_kernel(const void* ids, int wide, int64_t S, int N, int passes, uint32_t* key_out, uint32_t* pos_out) {
+    __shared__ uint32_t key[RS_SMALL], pos[RS_SMALL];
+    __shared__ uint32_t cnt[RS_SMALL_WAVES][RS_BINS];
+    __shared__ uint32_t tot[4];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int b = wv * (64 * RS_SMALL_ROUNDS) + lane;
+    uint32_t k[RS_SMALL_ROUNDS], ps[RS_SMALL_ROUNDS];
+#pragma unroll
+    for (int r = 0; r < RS_SMALL_ROUNDS; ++r) {
+        const int n = b + r * 64;
+        k[r] = n < N ? row_key(ids, wide, nullptr, S, n) : 0xffffffffu;
+        ps[r] = (uint32_t)n;
+    }
+    for (int p = 0; p < passes; ++p) {
+        const int shift = p * RS_BITS;
+        for (int i = tid; i < RS_SMALL_WAVES * RS_BINS; i += RS_SMALL_THREADS) (&cnt[0][0])[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RS_SMALL_ROUNDS; ++r)
+            if (b + r * 64 < N) atomicAdd(&cnt[wv][(k[r] >> shift) & (RS_BINS - 1)], 1u);
+        __syncthreads();
+        uint32_t all = 0;                      // inclusive over the digits, in the first four wavefronts
+        if (tid < RS_BINS) {
+            for (int w = 0; w < RS_SMALL_WAVES; ++w) all += cnt[w][tid];
+        }
+        uint32_t in = all;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(in, o);
+            if (lane >= o) in += up;
+        }
+        if (wv < 4 && lane == 63) tot[wv] = in;
+        __syncthreads();
+        if (tid < RS_BINS) {
+            for (int w = 0; w < wv; ++w) in += tot[w];
+            uint32_t at = in - all;
+            for (int w = 0; w < RS_SMALL_WAVES; ++w) { const uint32_t c = cnt[w][tid]; cnt[w][tid] = at; at += c; }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RS_SMALL_ROUNDS; ++r) {
+            const bool live = b + r * 64 < N;
+            const uint32_t dig = (k[r] >> shift) & (RS_BINS - 1);
+            const uint32_t to = digit_place(dig, live, lane, cnt[wv]);
+            if (live) { key[to] = k[r]; pos[to] = ps[r]; }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RS_SMALL_ROUNDS; ++r)
+            if (b + r * 64 < N) { k[r] = key[b + r * 64]; ps[r] = pos[b + r * 64]; }
+    }
+#pragma unroll
+    for (int r = 0; r < RS_SMALL_ROUNDS; ++r)
+        if (b + r * 64 < N) { key_out[b + r * 64] = k[r]; pos_out[b + r * 64] = ps[r]; }
 }
 
 // begin[s] = first place of the sorted keys that is not below s, for s = 0 .. S
@@ -406,7 +471,11 @@ void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* i
     char* w = static_cast<char*>(ws);
     auto at = [&](int64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
     uint32_t *k_in = nullptr, *p_in = nullptr, *k_out = at(p.key0), *p_out = at(p.pos0);
-    for (int i = 0; i < p.passes && N > 0; ++i) {
+    if (N > 0 && N <= RS_SMALL) {
+        k_in = k_out; p_in = p_out;
+        hipLaunchKernelGGL(rows_sort_small_kernel, dim3(1), dim3(RS_SMALL_THREADS), 0, st, ids, id_bytes == 8, S, (int)N, p.passes, k_in, p_in);
+    }
+    for (int i = 0; i < p.passes && N > RS_SMALL; ++i) {
         const bool direct = p.nblk <= RS_DIRECT;
         hipLaunchKernelGGL(rows_hist_kernel, dim3(p.nblk), dim3(256), 0, st, ids, id_bytes == 8, k_in, S, N, i * RS_BITS, at(p.hist));
         if (!direct) hipLaunchKernelGGL(rows_scan_kernel, dim3(RS_BINS), dim3(256), 0, st, at(p.hist), p.nblk, at(p.total));

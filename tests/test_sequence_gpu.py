@@ -326,7 +326,7 @@ def test_lookup_and_gradient(dc, t, N, S, D):
         assert not grad[torch.tensor(n == 0, device="cuda")].any()
 
 
-@pytest.mark.parametrize("N, S", [(1, 1), (63, 9), (4096, 4096), (16384, 300), (16385, 300), (70001, 65536), (200000, 300000), (130000, 17)])
+@pytest.mark.parametrize("N, S", [(1, 1), (63, 9), (3000, 300000), (4095, 1 << 24), (4096, 4096), (4097, 300), (16384, 300), (16385, 300), (70001, 65536), (200000, 300000), (130000, 17)])
 def test_gradient_of_whole_numbers_is_exact(dc, N, S):
     gen = torch.Generator(device="cuda").manual_seed(N)
     ids = torch.randint(-1, S, (N,), generator=gen, device="cuda")
