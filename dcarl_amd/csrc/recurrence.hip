@@ -120,7 +120,7 @@ void launch_recurrence_forward(const dcarl_recurrence_t& r, void* states, void* 
     const RecPlan p = rec_plan(r.N, r.D, r.type, r.gate_kind);
     char* ws = static_cast<char*>(workspace);
     char* plan = states ? static_cast<char*>(states) : ws + p.ws_plan;
-    if (p.tiles > 1) rec_launch_walk(r, p, r.ep_off, r.h0 || last, plan, ws, st);
+    if (p.tiles > 1) rec_launch_walk(r, p, r.ep_off, r.h0 || last || states, plan, ws, st);     // (a backward pass may ask for dh0 or bring a dlast)
     with_type(r.type, [&](auto t) {
         using T = decltype(t);
         RecWalk<T> a = rec_walk<T>(r, p, plan, ws);

