@@ -188,7 +188,8 @@ template <typename T, int C, int VEC, int GK, bool BACK> struct RecTile {
             if (have < 8) fl[i] = have <= 0 ? 0 : fl[i] & ((1ull << (8 * have)) - 1);
         }
     }
-    // The second walk over the steps widens the 16-bit operands again: without this the compiler keeps the widened ones of the first, twice the registers.
+    // The second walk over the steps widens the 16-bit operands again: without this the compiler keeps the widened ones of the first, in twice the
+    // registers (f16 backward, 65536 steps of 2048 channels: 427 us, like this 343).
     __device__ __forceinline__ void again() {
         if constexpr (sizeof(T) == 2 && VEC == 4) {
 #pragma unroll
