@@ -1069,7 +1069,7 @@ static int check_recurrence(const char* who, const dcarl_recurrence_t* r) {
     if (r->D > far || r->ldx < 0 || r->ldx > (r->D ? far : r->ldx) || r->ldg < 0 || r->ldg > (r->D ? far : r->ldg))
         return fail(DCARL_EINVAL, "%s: D=%lld, ldx=%lld or ldg=%lld outside [0,%lld]", who, (long long)r->D, (long long)r->ldx, (long long)r->ldg, (long long)far);
     if (int rc = check_ld(who, "ldh0", r->ldh0)) return rc;
-    if (r->E && !r->ep_off) return fail(DCARL_EINVAL, "%s: ep_off is NULL", who);
+    if ((r->E || r->N) && r->D && !r->ep_off) return fail(DCARL_EINVAL, "%s: ep_off is NULL", who);       // (no episode is one offset)
     if (r->N && r->D && (!r->x || (r->gate_kind && !r->gate))) return fail(DCARL_EINVAL, "%s: x / gate is NULL", who);
     return DCARL_OK;
 }

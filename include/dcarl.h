@@ -622,7 +622,7 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
 #define DCARL_BF16 2
 #define DCARL_F16 3
 /* Gated linear recurrence along ragged episodes, per channel d:   h[t] = g[t] * h[t-1] + x[t]
- *   episode e = steps [ep_off[e], ep_off[e+1]) (device, ep_off[0] == 0, rising, ep_off[E] <= N), h before its first step = h0[e] or 0.
+ *   episode e = steps [ep_off[e], ep_off[e+1]) (device, E + 1 offsets, ep_off[0] == 0, rising, ep_off[E] <= N), h before its first step = h0[e] or 0.
  *   reverse != 0 mirrors time: h[t] = g[t] * h[t+1] + x[t], an episode starts at its last step (discounted returns: x = rewards,
  *   g = gamma, D = 1).  x [N][D] with ldx elements between steps (channels contiguous; any alignment of the type;
  *   ldx, ldg and lddh of up to 2^17 elements, or of D, always fit);

@@ -212,3 +212,14 @@ def test_c_abi_refusals():
                      (dict(repetition_value=float("nan")), "not positive"), (dict(B=-1), "out of range"), (dict(ld_bias=-1), "ld_bias")):
         assert sc(**kw) == -1 and text in err(), kw
     assert sc(B=0) == 0 and lib.dcarl_adjust_scores(None, one, 40, null) == -1
+
+
+def test_c_abi_steps_without_offsets_are_refused():
+    if torch.cuda.is_available():
+        pytest.skip("fake addresses: only where nothing can run")
+    lib = load_library()
+    one, null = C.c_void_p(16), C.c_void_p(None)
+    for N in (4, 5000):                                       # no episode is one offset, not none
+        r = C.byref(_lib.CRecurrence(N=N, D=3, E=0, ep_off=0, x=16, ldx=3, gate=16, ldg=3, gate_kind=2, type=1))
+        for rc in (lib.dcarl_recurrence_forward(r, null, one, one, null, null), lib.dcarl_recurrence_backward(r, one, one, one, 3, null, one, one, null, null)):
+            assert rc == -1 and "ep_off is NULL" in lib.dcarl_last_error().decode()
