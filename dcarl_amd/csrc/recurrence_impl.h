@@ -267,6 +267,12 @@ __device__ __forceinline__ void rec_edges(const RecWalk<T>& a, const RecOwn<TILE
     }
 }
 
+// The map (A, B) at s.  At zero it is B whatever A is: over many steps the product of gates above 1 overflows, and a state of zero stays what the steps make of it.
+template <typename Acc> __device__ __forceinline__ Acc rec_apply(Acc A, Acc s, Acc B) {
+    const Acc r = fma(A, s, B);
+    return s == Acc(0) ? B : r;
+}
+
 // (A, B) of a run of steps for VEC channels; `cut`: an episode starts inside, nothing from before comes through
 template <typename Acc, int VEC> struct RecMap {
     Acc A[VEC], B[VEC];
@@ -280,7 +286,7 @@ template <typename Acc, int VEC> struct RecMap {
     __device__ __forceinline__ void after(const RecMap& f) {
         if (cut) return;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) { B[v] = fma(A[v], f.B[v], B[v]); A[v] *= f.A[v]; }
+        for (int v = 0; v < VEC; ++v) { B[v] = rec_apply(A[v], f.B[v], B[v]); A[v] *= f.A[v]; }
         cut = f.cut;
     }
 };
@@ -333,14 +339,14 @@ __device__ __forceinline__ void rec_carry(const RecMap<Acc, VEC>& m, const RecSh
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const Acc b = sh.B[w][c * VEC + v];
-            carry[v] = cut ? b : fma(sh.A[w][c * VEC + v], carry[v], b);
+            carry[v] = cut ? b : rec_apply(sh.A[w][c * VEC + v], carry[v], b);
         }
     }
     if constexpr (G > 1) {
         const RecMap<Acc, VEC> f = rec_from_lane(m, (lane - DIR * C) & 63);
         if (DIR > 0 ? grp > 0 : grp < G - 1) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) in[v] = f.cut ? f.B[v] : fma(f.A[v], in[v], f.B[v]);
+            for (int v = 0; v < VEC; ++v) in[v] = f.cut ? f.B[v] : rec_apply(f.A[v], in[v], f.B[v]);
         }
     }
 }
@@ -567,17 +573,17 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
                 for (int v = 0; v < VEC; ++v) st[v] = 0;
                 if (chain) rec_get_states<VEC>([&](int v) { return a.through + at(far, v); }, st);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) reached[c * VEC + v] = q.cut ? q.B[v] : fma(q.A[v], st[v], q.B[v]);
+                for (int v = 0; v < VEC; ++v) reached[c * VEC + v] = q.cut ? q.B[v] : rec_apply(q.A[v], st[v], q.B[v]);
             }
         }
         __syncthreads();
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) carry[v] = from < 0 ? Acc(0) : m.cut ? m.B[v] : fma(m.A[v], outside ? reached[c * VEC + v] : Acc(0), m.B[v]);
+    for (int v = 0; v < VEC; ++v) carry[v] = from < 0 ? Acc(0) : m.cut ? m.B[v] : rec_apply(m.A[v], outside ? reached[c * VEC + v] : Acc(0), m.B[v]);
     if (closes && first)                                   // what reaches the next group
 #pragma unroll
         for (int v = 0; v < VEC; ++v)
-            rec_put_state(a.through + at(group + DIR, v), total.cut ? total.B[v] : fma(total.A[v], carry[v], total.B[v]));
+            rec_put_state(a.through + at(group + DIR, v), total.cut ? total.B[v] : rec_apply(total.A[v], carry[v], total.B[v]));
 }
 
 template <typename T, int C, int VEC, int GK>

@@ -151,9 +151,12 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
 
     x: (N, D) steps, or (N,) for one channel; float64, float32, bfloat16 or float16 (sums in f32; f64 for float64; each result rounded once).
     gate: (N, D) like x, (N,) shared by the channels of a step, or a number.  ep_off: (E+1,) int offsets of the episodes as in
-    ``episode_returns``; steps behind ``ep_off[E]`` belong to none: they are not read, the results are zero there.
+    ``episode_returns``; steps behind ``ep_off[E]`` belong to none: what they hold counts nowhere, the results are zero there.
     h0: (E, D) (or (E,)) states before the first steps; one step of E live episodes is N == E with every length 1.
     reverse: mirrored, ``h[t] = gate[t] * h[t+1] + x[t]`` from the end of each episode.
+    Products of consecutive gates are formed by themselves, in the type of the sums: gates of magnitude up to 1 are right over any length; where a product of
+    larger ones leaves that type's range, states that are not zero read inf or NaN, also where later gates would bring them back, and an
+    infinite state may read NaN further on.
     want_last: also the (E, D) states that the episodes end with (``h0`` or zero for an empty one).
     validate: check ep_off's values; where it lies on the GPU this waits for it.  ``validate=False`` never waits and is what a captured call
     needs; offsets that do not rise from 0 to at most N then give unspecified results (and no access out of range).

@@ -622,3 +622,28 @@ def test_scores_beyond_32_bits(dc):
     off[-1] = 2
     z = dc.candidates.adjust(s, torch.tensor([V - 1, 4], device="cuda"), off, presence=1.0, out=s)
     assert z[-1, V - 1] == -1 and z[-1, 4] == -1 and int((z[-1] != 0).sum()) == 2 and not z[0].any() and not z[1100].any()
+
+
+@pytest.mark.parametrize("D", [1, 5, 64])
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_recurrence_gates_above_one_leave_zeros_alone(dc, t, D):
+    """The product of the gates overflows long before the first value arrives; nothing is rounded: powers of two alone."""
+    lengths = [300, 5000, 70000]
+    off = ragged(lengths)
+    N = off[-1]
+    x, dh = torch.zeros(N, D), torch.zeros(N, D)
+    for b, e in zip(off, off[1:]):
+        x[e - 4], x[e - 2] = 1.0, 2.0
+        dh[b + 1], dh[b + 3] = 1.0, 2.0
+    h = torch.zeros(N, D)
+    dx = torch.zeros(N, D)
+    for b, e in zip(off, off[1:]):
+        h[e - 4:e] = torch.tensor([1.0, 4.0, 18.0, 72.0])[:, None]
+        dx[b:b + 4] = torch.tensor([132.0, 33.0, 8.0, 2.0])[:, None]
+    leaf = [x.to("cuda", t).requires_grad_(), torch.full((N, D), 4.0, device="cuda", dtype=t, requires_grad=True)]
+    got = dc.episodes.gated_recurrence(*leaf, off)
+    assert torch.equal(got.detach().cpu().float(), h)
+    gx, gg = torch.autograd.grad(got, leaf, dh.to("cuda", t))
+    assert torch.equal(gx.cpu().float(), dx) and not gg.any()
+    back = dc.episodes.gated_recurrence(x.flip(0).to("cuda", t), 4.0, [N - v for v in reversed(off)], reverse=True)
+    assert torch.equal(back.cpu().float(), h.flip(0))
