@@ -647,3 +647,20 @@ def test_recurrence_gates_above_one_leave_zeros_alone(dc, t, D):
     assert torch.equal(gx.cpu().float(), dx) and not gg.any()
     back = dc.episodes.gated_recurrence(x.flip(0).to("cuda", t), 4.0, [N - v for v in reversed(off)], reverse=True)
     assert torch.equal(back.cpu().float(), h.flip(0))
+
+
+def test_adjust_extreme_repetition(dc):
+    """r whose inverse overflows f32 or is subnormal: still z / r, of two roundings at most (2^-24 each; results here are normal)."""
+    r = torch.tensor([2.0 ** -149, 5 * 2.0 ** -149, 2.0 ** -128, 2.0 ** 126, 3 * 2.0 ** 126, 2.0 ** 125, 1.75 * 2.0 ** 127], dtype=torch.float32)
+    z = torch.tensor([2.0 ** -30, 3 * 2.0 ** -30, 7 * 2.0 ** -30, 7.0, 11.0, 13.0, 23.0], dtype=torch.float32).repeat(7, 1)
+    z[3:] = z[3:] * 2.0 ** 40
+    z[:3, 3:] = 2.0 ** -28
+    ids, off = torch.arange(7, device="cuda").repeat(7), torch.arange(8, device="cuda") * 7
+    got = dc.candidates.adjust(z.cuda(), ids, off, repetition=r.cuda())
+    want = z.double() / r.double()[:, None]
+    assert want.min() > 2.0 ** -126 and want.max() < 2.0 ** 127 * 1.9
+    check(got, want.numpy(), 2 * 2.0 ** -24 * want.numpy(), "z / r")
+    got = dc.candidates.adjust(torch.tensor([[5.0, math.inf, -1.0]], device="cuda"), torch.arange(3, device="cuda"), torch.tensor([0, 3], device="cuda"), repetition=math.inf)
+    assert got[0, 0] == 0 and got[0, 1].isnan() and got[0, 2] == -math.inf
+    one = dc.candidates.adjust(z[4:5].cuda(), ids[:7], off[:2], repetition=float(r[4]))      # a number for all rows
+    check(one, want[4:5].numpy(), 2 * 2.0 ** -24 * want[4:5].numpy(), "z / r")
