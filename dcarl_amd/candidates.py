@@ -64,6 +64,16 @@ def _half_over(scores, out) -> bool:
     return True
 
 
+def _end(t) -> int:
+    """The address behind a tensor's last element."""
+    return t.data_ptr() + (1 + sum((n - 1) * step for n, step in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _over(t, out) -> bool:
+    """Whether an operand that all of a row's workgroups read shares memory with out."""
+    return t is not None and t.device == out.device and t.numel() > 0 and out.numel() > 0 and t.data_ptr() < _end(out) and out.data_ptr() < _end(t)
+
+
 def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, frequency=0.0, presence=0.0, bias=None, allowed=None, out=None,
            validate: bool = False):
     """For each of B rows of V scores:  z = score;  taken before: z = z / r if z > 0 else z * r;  z -= f * n + p where n > 0;
@@ -74,7 +84,7 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
     entries at a history's front were handed to the policy and not chosen by it: ``n`` counts the others, "taken before" looks at all.
     repetition (> 0), frequency, presence: r, f, p, a number or a float32 tensor (B,).  bias: float32 (V,) or (B, V).
     allowed: int32 words of ``pack_allowed``, (ceil(V/32),) or (B, ceil(V/32)); a row that allows nothing is -inf throughout.
-    out: where the result goes; ``out=scores`` adjusts in place.  validate: check taken_off's values (waits for them when they are on
+    out: where the result goes; ``out=scores`` adjusts in place, and out lies over no other operand.  validate: check taken_off's values (waits for them when they are on
     the GPU); without it, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one are refused."""
     if not isinstance(scores, torch.Tensor) or scores.dtype not in SCORE_TYPES:
         raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
@@ -106,6 +116,11 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
             raise ValueError("out requires a gradient")
         if _half_over(scores, out):
             raise ValueError("out lies partly over scores: it is scores itself or apart from it")
+        for name, t in (("taken", taken), ("taken_off", off), ("given", given), ("repetition", rep), ("frequency", freq), ("presence", pres), ("allowed", allowed)):
+            if _over(t, out):
+                raise ValueError(f"out lies over {name}")
+        if bias is not None and (_half_over(bias, out) if bias.dim() == 2 and bias.dtype == out.dtype else _over(bias, out)):
+            raise ValueError("out lies partly over bias: it is bias itself or apart from it")
     dev = _seq.on_device(("scores", scores), ("taken", taken), ("taken_off", off), ("given", given), ("repetition", rep), ("frequency", freq),
                          ("presence", pres), ("bias", bias), ("allowed", allowed), ("out", out))
     return _seq.run_on(dev, _adjust, scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias, ld_bias, allowed, ld_allowed, out)

@@ -223,3 +223,19 @@ def test_c_abi_steps_without_offsets_are_refused():
         r = C.byref(_lib.CRecurrence(N=N, D=3, E=0, ep_off=0, x=16, ldx=3, gate=16, ldg=3, gate_kind=2, type=1))
         for rc in (lib.dcarl_recurrence_forward(r, null, one, one, null, null), lib.dcarl_recurrence_backward(r, one, one, one, 3, null, one, one, null, null)):
             assert rc == -1 and "ep_off is NULL" in lib.dcarl_last_error().decode()
+
+
+def test_adjust_refuses_out_over_what_a_row_reads():
+    from dcarl_amd import candidates
+    s, n = torch.zeros(2, 32), 2 * 32
+    buf = torch.zeros(3 * n)
+    out = buf[:n].view(2, 32)
+    for kw in (dict(bias=buf[n - 1:n + 31]), dict(bias=buf[:32]), dict(bias=buf[32:96].view(2, 32)), dict(bias=buf[:32].expand(2, 32)), dict(frequency=buf[10:12]),
+               dict(presence=buf[62:64]), dict(given=buf.view(torch.int32)[:2]), dict(allowed=buf.view(torch.int32)[63:64]),
+               dict(taken=buf.view(torch.int32)[60:70], taken_off=[0, 1, 2]), dict(taken=torch.zeros(4, dtype=torch.int32), taken_off=buf.view(torch.int64)[30:33])):
+        with pytest.raises(ValueError, match="out lies"):
+            candidates.adjust(s, out=out, **kw)
+    wide = torch.zeros(2, 70)
+    for kw in (dict(bias=buf[n:n + 32]), dict(bias=out), dict(bias=wide[:, 33:65], out=wide[:, :32]), dict(presence=buf[64:66])):
+        with pytest.raises(_lib.DcarlError, match="no CPU path"):         # (past the checks)
+            candidates.adjust(s, **{"out": out, **kw})
