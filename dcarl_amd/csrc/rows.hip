@@ -113,6 +113,13 @@ __device__ __forceinline__ uint32_t scan256(uint32_t v, uint32_t (&tot)[4]) {
     return v;
 }
 
+// LDS accesses of a wavefront's lanes stay on their side of this (the hardware keeps their order; it holds the compiler to it)
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Where this lane's item goes: its digit's next place (place[digit], this wavefront's own) and its rank among the wavefront's items of that digit.
 __device__ __forceinline__ uint32_t digit_place(uint32_t dig, bool live, int lane, uint32_t* place) {
     unsigned long long same = __ballot(live);
@@ -124,9 +131,9 @@ __device__ __forceinline__ uint32_t digit_place(uint32_t dig, bool live, int lan
     const int rank = __popcll(same & ((1ull << lane) - 1));
     uint32_t to = 0;
     if (live) to = place[dig];
-    __builtin_amdgcn_wave_barrier();           // every lane has read its digit's place before the first lane of a group moves it on
+    wave_order();                              // every lane has read its digit's place before the first lane of a group moves it on
     if (live && rank == 0) place[dig] = to + (uint32_t)__popcll(same);
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
     return to + rank;
 }
 
