@@ -382,10 +382,10 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
     using Acc = typename SeqType<T>::Acc;
     __shared__ Acc lds[RW_THREADS * VEC];
     const RowLane l = row_lane<VEC>(lanes, D);
-    auto put = [&](int64_t s, const Acc(&sum)[VEC]) {
+    auto put = [&](int64_t s, const Acc(&sum)[VEC], Acc by) {
         RowVec<T, VEC> o;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o.v[i] = narrow<T>(sum[i] * (Acc)scale);
+        for (int i = 0; i < VEC; ++i) o.v[i] = narrow<T>(sum[i] * by);
         row_store(grad + s * D + l.cb, o);
     };
     const int64_t s0 = (int64_t)blockIdx.x * l.R * ROWS;
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
         for (int i = 0; i < VEC; ++i) sum[i] = 0;
         const uint32_t b = b4[j];
         rows_add<T, VEC>(sum, e4[j] - b, [&](int64_t i) { return dout + (int64_t)pos[b + i] * ldd + l.cb; });
-        put(s, sum);
+        put(s, sum, e4[j] > b ? (Acc)scale : Acc(0));        // (no id: zero, whatever the scale)
     }
     if (!__syncthreads_or(is_long)) return;
     for (int r = 0; r < rows && s0 + r < S; ++r) {         // the long ones, the whole workgroup at each: partial sums of their chunks
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
         if (l.live && from < to)
             rows_add<Acc, VEC>(sum, to - from, [&](int64_t i) { return from_part + ((c0 + from + i) * 2 + ((c0 + from + i) * places < b)) * D + l.cb; });
         rows_join<VEC>(sum, lds, l, lanes);
-        if (l.live && l.r == 0) put(s0 + r, sum);
+        if (l.live && l.r == 0) put(s0 + r, sum, (Acc)scale);
     }
 }
 

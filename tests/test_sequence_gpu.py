@@ -664,3 +664,13 @@ def test_adjust_extreme_repetition(dc):
     assert got[0, 0] == 0 and got[0, 1].isnan() and got[0, 2] == -math.inf
     one = dc.candidates.adjust(z[4:5].cuda(), ids[:7], off[:2], repetition=float(r[4]))      # a number for all rows
     check(one, want[4:5].numpy(), 2 * 2.0 ** -24 * want[4:5].numpy(), "z / r")
+
+
+@pytest.mark.parametrize("scale", [math.inf, math.nan, -0.0])
+def test_gradient_rows_without_an_id_are_zero_whatever_the_scale(dc, scale):
+    ids = torch.tensor([3, -1, 3, 9], device="cuda")
+    grad = dc.tables.lookup_gradient(torch.ones(4, 5, device="cuda"), ids, 300, scale)
+    named = torch.zeros(300, dtype=torch.bool, device="cuda")
+    named[[3, 9]] = True
+    assert not grad[~named].any()
+    assert torch.equal(grad[named].cpu(), torch.tensor([[2.0], [1.0]]).expand(2, 5) * scale) or math.isnan(scale) and grad[named].isnan().all()
