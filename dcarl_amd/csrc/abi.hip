@@ -89,6 +89,7 @@ int launch_census_table(const double*, int, int, const DevParams&, unsigned long
 template <typename T>
 int launch_census_trace(const T*, const uint8_t*, const int64_t*, const int32_t*, int, int, const DevParams&, unsigned long long*, hipStream_t);
 int64_t recurrence_max_ld(int64_t, int);
+int64_t recurrence_workgroups(int64_t, int64_t, int64_t, int);
 int64_t recurrence_workspace_bytes(int64_t, int64_t, int64_t, int, int);
 int64_t recurrence_states_bytes(int64_t, int64_t, int64_t, int, int);
 void launch_recurrence_forward(const dcarl_recurrence_t&, void*, void*, void*, void*, hipStream_t);
@@ -1049,7 +1050,7 @@ int32_t dcarl_index_states_f64(const double* obs, int64_t N, int32_t D, const do
 // ---- sequence operators ------------------------------------------------------------------------------------------------
 constexpr int64_t SEQ_MAX = (int64_t)1 << 31;          // steps, channels, episodes, rows, ids of one call
 constexpr int64_t SEQ_MAX_WIDE = (int64_t)1 << 23;     // channels of a table row: 65535 blocks of 256 threads and more
-constexpr int64_t SEQ_MAX_ELEMENTS = (int64_t)1 << 40; // of one operand: a launch's workgroups stay below 2^31
+constexpr int64_t SEQ_MAX_ELEMENTS = (int64_t)1 << 40; // of one operand
 
 static int check_seq(const char* who, int32_t type, int64_t n, int64_t d, int64_t e) {
     if (type < DCARL_F64 || type > DCARL_F16) return fail(DCARL_EINVAL, "%s: type=%d is none of DCARL_F64/F32/BF16/F16", who, type);
@@ -1068,6 +1069,8 @@ static int check_recurrence(const char* who, const dcarl_recurrence_t* r) {
     const int64_t far = r->D ? dcarl::recurrence_max_ld(r->D, r->type) : 0;
     if (r->D > far || r->ldx < 0 || r->ldx > (r->D ? far : r->ldx) || r->ldg < 0 || r->ldg > (r->D ? far : r->ldg))
         return fail(DCARL_EINVAL, "%s: D=%lld, ldx=%lld or ldg=%lld outside [0,%lld]", who, (long long)r->D, (long long)r->ldx, (long long)r->ldg, (long long)far);
+    if (r->D && dcarl::recurrence_workgroups(r->N, r->D, r->E, r->type) >= (1 << 24))             // of 256 threads: a launch holds fewer than 2^32
+        return fail(DCARL_EINVAL, "%s: N=%lld steps of D=%lld channels are more than one call takes", who, (long long)r->N, (long long)r->D);
     if (int rc = check_ld(who, "ldh0", r->ldh0)) return rc;
     if ((r->E || r->N) && r->D && !r->ep_off) return fail(DCARL_EINVAL, "%s: ep_off is NULL", who);       // (no episode is one offset)
     if (r->N && r->D && (!r->x || (r->gate_kind && !r->gate))) return fail(DCARL_EINVAL, "%s: x / gate is NULL", who);

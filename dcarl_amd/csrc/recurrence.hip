@@ -73,6 +73,11 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
 int64_t recurrence_max_ld(int64_t D, int type) {
     return ((int64_t)1 << 31) / rec_plan(1, D, type, 2).tile / (type == DCARL_F64 ? 8 : type == DCARL_F32 ? 4 : 2);
 }
+// workgroups of a call's largest launch
+int64_t recurrence_workgroups(int64_t N, int64_t D, int64_t E, int type) {
+    const RecPlan p = rec_plan(N, D, type, 2);
+    return p.tiles * p.blocks + rec_empty_blocks(true, E);
+}
 int64_t recurrence_workspace_bytes(int64_t N, int64_t D, int64_t, int type, int gate_kind) { return D ? rec_plan(N, D, type, gate_kind).ws_bytes : 0; }
 int64_t recurrence_states_bytes(int64_t N, int64_t D, int64_t, int type, int gate_kind) { return D ? rec_plan(N, D, type, gate_kind).states_bytes : 0; }
 

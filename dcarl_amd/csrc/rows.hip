@@ -320,6 +320,11 @@ template <int VEC, typename Acc> __device__ __forceinline__ void rows_join(Acc (
             for (int k = 0; k < VEC; ++k) sum[k] += lds[(r * lanes + l.c) * VEC + k];
 }
 
+// A launch holds fewer than 2^32 threads along x: workgroups beyond ROW_FOLD go along z.
+constexpr int64_t ROW_FOLD = 1 << 22;
+__device__ __forceinline__ int64_t row_block() { return blockIdx.x + (int64_t)blockIdx.z * gridDim.x; }
+static dim3 row_grid(int64_t n, unsigned across) { return dim3((unsigned)(n < ROW_FOLD ? n : ROW_FOLD), across, (unsigned)((n + ROW_FOLD - 1) / ROW_FOLD)); }
+
 // The sums of the long runs (more than RW_CHUNK places) over one chunk of RW_CHUNK sorted places.  At most two long runs meet a chunk: the one
 // of its first place (part[chunk][0]) and the one of its last (part[chunk][1]).  The workgroup's groups take a quarter, a third ... of the places each.
 template <typename T, int VEC>
@@ -328,7 +333,8 @@ __global__ __launch_bounds__(RW_THREADS) void rows_chunk_kernel(const uint32_t* 
     using Acc = typename SeqType<T>::Acc;
     __shared__ Acc lds[RW_THREADS * VEC];
     const RowLane l = row_lane<VEC>(lanes, D);
-    const int64_t b = (int64_t)blockIdx.x * RW_CHUNK, e = b + RW_CHUNK < N ? b + RW_CHUNK : N;
+    const int64_t chunk = row_block(), b = chunk * RW_CHUNK, e = b + RW_CHUNK < N ? b + RW_CHUNK : N;
+    if (b >= N) return;
     const uint32_t first = key[b], last = key[e - 1];
     for (int slot = 0; slot < 2; ++slot) {
         const uint32_t k = slot ? last : first;
@@ -343,7 +349,7 @@ __global__ __launch_bounds__(RW_THREADS) void rows_chunk_kernel(const uint32_t* 
         if (l.live && from < to) rows_add<T, VEC>(sum, to - from, [&](int64_t i) { return dout + (int64_t)pos[from + i] * ldd + l.cb; });
         rows_join<VEC>(sum, lds, l, lanes);
         if (l.live && l.r == 0)
-            for (int i = 0; i < VEC; ++i) part[((int64_t)blockIdx.x * 2 + slot) * D + l.cb + i] = sum[i];
+            for (int i = 0; i < VEC; ++i) part[(chunk * 2 + slot) * D + l.cb + i] = sum[i];
     }
 }
 
@@ -388,7 +394,8 @@ __global__ __launch_bounds__(RW_THREADS) void rows_sum_kernel(const uint32_t* be
         for (int i = 0; i < VEC; ++i) o.v[i] = narrow<T>(sum[i] * by);
         row_store(grad + s * D + l.cb, o);
     };
-    const int64_t s0 = (int64_t)blockIdx.x * l.R * ROWS;
+    const int64_t s0 = row_block() * l.R * ROWS;
+    if (s0 >= S) return;
     const int rows = l.R * ROWS;
     Acc sum[VEC];
     uint32_t b4[ROWS], e4[ROWS];
@@ -501,7 +508,7 @@ void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* i
         Acc *part = reinterpret_cast<Acc*>(w + p.part), *super = reinterpret_cast<Acc*>(w + p.super);
         const int64_t R = RW_THREADS / lanes;
         if (N > RW_CHUNK)
-            hipLaunchKernelGGL((rows_chunk_kernel<T, V()>), dim3((unsigned)((N + RW_CHUNK - 1) / RW_CHUNK), across), dim3(RW_THREADS), 0, st, k_in,
+            hipLaunchKernelGGL((rows_chunk_kernel<T, V()>), row_grid((N + RW_CHUNK - 1) / RW_CHUNK, across), dim3(RW_THREADS), 0, st, k_in,
                                at(p.begin), p_in, (const T*)dout, ldd, N, S, D, lanes, part);
         // up to 16384 ids the sums take their chunks one by one (256 at most): a launch less
         if (N <= 8 * RW_CHUNK * RW_SUPER) super = nullptr;
@@ -512,7 +519,7 @@ void launch_rows_gradient(int type, const void* dout, int64_t ldd, const void* i
         // 8000 rows of 1 KB 43 and 27.
         auto go = [&](auto rows) {
             const int64_t each = R * rows();
-            hipLaunchKernelGGL((rows_sum_kernel<T, V(), rows()>), dim3((unsigned)((S + each - 1) / each), across), dim3(RW_THREADS), 0, st,
+            hipLaunchKernelGGL((rows_sum_kernel<T, V(), rows()>), row_grid((S + each - 1) / each, across), dim3(RW_THREADS), 0, st,
                                at(p.begin), p_in, (const T*)dout, ldd, S, D, lanes, scale, part, super, (T*)grad);
         };
         if (S / (R * RW_ROWS) * across >= 2048) go(std::integral_constant<int, RW_ROWS>{});

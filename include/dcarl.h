@@ -627,7 +627,9 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
  *   g = gamma, D = 1).  x [N][D] with ldx elements between steps (channels contiguous; any alignment of the type;
  *   ldx, ldg and lddh of up to 2^17 elements, or of D, always fit);
  *   gate_kind 0: g = gate_value; 1: gate [N], element stride ldg, shared by the channels; 2: gate [N][D], ldg elements between steps.
- *   Steps behind the last episode are read by nothing; the outputs hold zeros there.
+ *   What steps behind the last episode hold counts nowhere; the outputs hold zeros there.  |g| <= 1 is right over any length; where the product of
+ *   consecutive larger gates overflows the type of the sums, a state that is not zero reads inf or NaN from there on.
+ *   Calls of 2^24 workgroups (2^37 elements of wide 16-bit rows; 2^31 steps of 17 channels) are refused.
  * dcarl_recurrence_forward: h [N][D] contiguous; last (nullable) [E][D] = the state each episode ends with, h0[e] (or 0) for an empty one;
  *   states (nullable): dcarl_recurrence_states_bytes bytes the backward call wants (16-byte aligned).
  * dcarl_recurrence_backward, from the same arguments, the forward call's states, dh [N][D] (lddh elements between steps) and dlast (nullable)

@@ -239,3 +239,14 @@ def test_adjust_refuses_out_over_what_a_row_reads():
     for kw in (dict(bias=buf[n:n + 32]), dict(bias=out), dict(bias=wide[:, 33:65], out=wide[:, :32]), dict(presence=buf[64:66])):
         with pytest.raises(_lib.DcarlError, match="no CPU path"):         # (past the checks)
             candidates.adjust(s, **{"out": out, **kw})
+
+
+def test_c_abi_recurrence_beyond_a_launch_is_refused():
+    if torch.cuda.is_available():
+        pytest.skip("fake addresses: only where nothing can run")
+    lib = load_library()
+    one, null = C.c_void_p(16), C.c_void_p(None)
+    for N, D, t in (((1 << 31) - 2, 17, 3), (1 << 25, 16400, 2)):
+        r = C.byref(_lib.CRecurrence(N=N, D=D, E=1, ep_off=16, x=16, ldx=D, gate=16, ldg=1, gate_kind=1, type=t))
+        for rc in (lib.dcarl_recurrence_forward(r, null, one, one, null, null), lib.dcarl_recurrence_backward(r, one, one, one, D, null, one, one, null, null)):
+            assert rc == -1 and "more than one call takes" in lib.dcarl_last_error().decode()

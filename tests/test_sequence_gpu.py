@@ -674,3 +674,22 @@ def test_gradient_rows_without_an_id_are_zero_whatever_the_scale(dc, scale):
     named[[3, 9]] = True
     assert not grad[~named].any()
     assert torch.equal(grad[named].cpu(), torch.tensor([[2.0], [1.0]]).expand(2, 5) * scale) or math.isnan(scale) and grad[named].isnan().all()
+
+
+def test_gradient_of_more_chunks_and_rows_than_one_grid_axis_takes(dc):
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 80 GB")
+    N = (1 << 28) + 1000                                                  # chunks of 64 ids
+    ids = torch.arange(N, device="cuda", dtype=torch.int32) % 3
+    dout = torch.zeros(N, 1, device="cuda", dtype=torch.float16)
+    places = torch.cat([torch.randint(0, N, (900,), generator=torch.Generator().manual_seed(1)), torch.arange(N - 300, N)]).unique()
+    dout[places.cuda()] = 1.0
+    grad = dc.tables.lookup_gradient(dout, ids, 3, validate=False)
+    assert torch.equal(grad.flatten().cpu().long(), torch.bincount(places % 3))
+    del ids, dout
+    S, D = (1 << 24) + 77, 1032                                           # a workgroup takes four rows of this width
+    ids = torch.tensor([0, S - 1, (1 << 24) - 1, 1 << 24, 12345, S - 1], device="cuda")
+    dout = torch.arange(6, device="cuda", dtype=torch.float16)[:, None].expand(6, D) + 1
+    grad = dc.tables.lookup_gradient(dout, ids, S)
+    assert torch.equal(grad[ids].cpu(), torch.tensor([1.0, 8, 3, 4, 5, 8], dtype=torch.float16)[:, None].expand(6, D))
+    assert sum(int((grad[a:a + (1 << 21)] != 0).any(1).sum()) for a in range(0, S, 1 << 21)) == 5
