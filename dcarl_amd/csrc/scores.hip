@@ -121,8 +121,8 @@ __global__ __launch_bounds__(THREADS) void scores_kernel(const T* in, T* out, Sc
         const float r = a.rep ? a.rep[b] : a.rep0, f = a.freq ? a.freq[b] : a.freq0, p0 = a.pres ? a.pres[b] : a.pres0;
         // z / r as z * (1 / r): one rounding of 2^-24 more, and no division for each of the candidates; but for an r whose inverse f32 does not hold, or holds
         // with fewer bits (below 2^-126)
-        const float inverse = 1.0f / r, size = __builtin_fabsf(inverse);
-        const bool divides = !(size >= 0x1p-126f && size < __builtin_inff());
+        const float inverse = 1.0f / r;
+        const bool divides = !__builtin_isnormal(inverse);
 #pragma unroll
         for (int p = 0; p < PIECES; ++p) {
             const int i = (p * THREADS + (int)threadIdx.x) * VEC;
