@@ -693,3 +693,17 @@ def test_gradient_of_more_chunks_and_rows_than_one_grid_axis_takes(dc):
     grad = dc.tables.lookup_gradient(dout, ids, S)
     assert torch.equal(grad[ids].cpu(), torch.tensor([1.0, 8, 3, 4, 5, 8], dtype=torch.float16)[:, None].expand(6, D))
     assert sum(int((grad[a:a + (1 << 21)] != 0).any(1).sum()) for a in range(0, S, 1 << 21)) == 5
+
+
+@pytest.mark.parametrize("kind", ["full", "step", "number"])
+@pytest.mark.parametrize("t, D", [(torch.float64, 1), (torch.float64, 7), (torch.float32, 3), (torch.float32, 65), (torch.bfloat16, 4), (torch.bfloat16, 770), (torch.float16, 2), (torch.float16, 33)])
+def test_recurrence_of_about_a_step_each(dc, t, D, kind):
+    """Few steps of many episodes: all of them, some, two or three steps, all in one episode; rows behind the last."""
+    for i, (lengths, behind) in enumerate((([1], 0), ([1] * 48, 0), ([0, 1, 0, 0, 2, 1, 0], 3), ([2] * 20 + [1, 0], 0), ([0] * 63 + [64], 0), ([100] + [0] * 63 + [28], 0), ([0] * 5, 9), ([1] * 300, 0))):
+        off = ragged(lengths)
+        x, gate, h0, dh, dl = inputs(off[-1] + behind, D, len(lengths), t, kind, i)
+        if behind:
+            x[off[-1]:] = math.nan
+            dh[off[-1]:] = math.nan
+        for reverse in (False, True):
+            check_recurrence(dc, x, gate, off, h0 if i != 3 else None, dh, dl, reverse, t)
