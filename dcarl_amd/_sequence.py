@@ -19,16 +19,17 @@ def type_code(name: str, t: torch.Tensor, allowed=TYPES) -> int:
 
 def on_device(*named) -> torch.device:
     """The one GPU that all of the (name, tensor or None) live on; raises where one lives elsewhere (there is no CPU path)."""
-    dev = None
+    first = None
     for name, t in named:
         if t is None:
             continue
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise _lib.DcarlError(f"{name} is on {t.device}: the operator has no CPU path")
-        if dev is not None and t.device != dev[1].device:
-            raise ValueError(f"{name} is on {t.device}, {dev[0]} on {dev[1].device}")
-        dev = dev or (name, t)
-    return dev[1].device
+        if first is None:
+            first, index = (name, t), t.get_device()
+        elif t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, {first[0]} on {first[1].device}")
+    return first[1].device
 
 
 def run_on(device: torch.device, call, *args):
@@ -50,6 +51,11 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 def at(t):
     """The address of a tensor, None where there is none."""
     return None if t is None else t.data_ptr()
+
+
+def like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, type and device (empty_like by itself keeps the order of a transposed one's strides)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def wants_gradient(*tensors) -> bool:

@@ -130,7 +130,7 @@ def _adjust(scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias
     B, V = scores.shape
     dev = scores.device
     s, ld = _seq.rows_of(scores)
-    z = torch.empty(B, V, dtype=s.dtype, device=dev) if out is None else out
+    z = _seq.like(s) if out is None else out
     given = None if given is None else given.contiguous()
     at = _seq.at
     a = _lib.CScores(at(s), B, V, ld, at(taken), at(off), 0 if taken is None else taken.numel(), at(given), at(rep), at(freq), at(pres), at(bias),

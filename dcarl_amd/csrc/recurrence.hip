@@ -120,7 +120,7 @@ RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
     p.through = take(p.tiles > 1 ? (p.tiles / REC_GROUP + 1) * p.wide * acc : 0);
     p.clear_bytes = at;
     p.ticket = take(p.tiles > 1 ? 4 * REC_TICKET * p.blocks : 0);
-    p.ws_plan = take(p.plan_bytes);
+    p.ws_plan = take(p.tiles > 1 ? p.plan_bytes : 0);
     p.dgp = take(gate_kind == 1 && p.blocks > 1 ? p.blocks * N * acc : 0);
     p.ws_bytes = at;
     return p;
@@ -145,6 +145,7 @@ template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, co
     a.g = r.gate_kind ? static_cast<const T*>(r.gate) : nullptr; a.ldg = (uint32_t)r.ldg;
     a.h0 = static_cast<const T*>(r.h0); a.ldh0 = r.ldh0;
     a.gval = (Acc)r.gate_value;
+    if (p.tiles <= 1) return a;                            // finds its flags itself, waits for nothing
     a.flag = reinterpret_cast<uint8_t*>(plan + p.flag);
     a.ep = reinterpret_cast<int32_t*>(plan + p.ep);
     a.ticket = reinterpret_cast<uint32_t*>(ws + p.ticket);

@@ -94,13 +94,13 @@ def _recurrence_args(x, gate, ep_off, h0, gate_value, reverse):
 
 
 def _bytes(n, dev):
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=dev)
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
 def _recurrence_forward(x, gate, ep_off, h0, gate_value, reverse, want_last, want_states):
     lib, dev = _lib.load(), x.device
     a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    h = _seq.like(x)
     last = torch.empty(a.E, a.D, dtype=x.dtype, device=dev) if want_last else None
     sizes = (a.N, a.D, a.E, a.type, a.gate_kind)
     states = _bytes(lib.dcarl_recurrence_states_bytes(*sizes), dev) if want_states else None
@@ -115,9 +115,9 @@ def _recurrence_backward(x, gate, ep_off, h0, gate_value, reverse, states, dh, d
     a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
     dh, lddh = _seq.rows_of(dh, _FAR)
     dlast = None if dlast is None else dlast.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
-    dgate = torch.empty(gate.shape, dtype=x.dtype, device=dev) if want[1] else None
-    dh0 = torch.empty(h0.shape, dtype=x.dtype, device=dev) if want[2] else None
+    dx = _seq.like(x) if want[0] else None
+    dgate = _seq.like(gate) if want[1] else None
+    dh0 = _seq.like(h0) if want[2] else None
     ws = _bytes(lib.dcarl_recurrence_workspace_bytes(a.N, a.D, a.E, a.type, a.gate_kind), dev)
     _lib.check(lib.dcarl_recurrence_backward(C.byref(a), _seq.at(states), _seq.at(ws), _seq.at(dh), lddh, _seq.at(dlast), _seq.at(dx),
                                              _seq.at(dgate), _seq.at(dh0), _seq.stream(dev)), "dcarl_recurrence_backward")
@@ -186,7 +186,7 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
             raise ValueError(f"h0 {tuple(h0.shape)} does not hold a state like x {tuple(x.shape)} for every episode")
         E = h0.shape[0]
     off = _seq.offsets("ep_off", ep_off, N, E, validate)
-    dev = _seq.on_device(("x", x), ("gate", gate), ("h0", h0), ("ep_off", off if off.device.type == "cuda" else None))
+    dev = _seq.on_device(("x", x), ("gate", gate), ("h0", h0), ("ep_off", off if off.is_cuda else None))
     if off.device != dev:
         if _seq.capturing():
             raise ValueError("ep_off must lie on the GPU while a graph is captured")

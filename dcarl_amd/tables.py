@@ -66,7 +66,7 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
     if table.dim() != 2:
         raise ValueError(f"table must be (S, D), not {tuple(table.shape)}")
     ids = _check_ids(ids, table.shape[0], validate)
-    dev = _seq.on_device(("table", table), ("ids", ids if ids.device.type == "cuda" else None))
+    dev = _seq.on_device(("table", table), ("ids", ids if ids.is_cuda else None))
     if ids.device != dev:
         if _seq.capturing():
             raise ValueError("ids must lie on the GPU while a graph is captured")
@@ -85,7 +85,7 @@ def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: boo
     ids = _check_ids(ids, n_rows, validate)
     if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"dout {tuple(dout.shape)} has no row for each of the ids {tuple(ids.shape)}")
-    dev = _seq.on_device(("dout", dout), ("ids", ids if ids.device.type == "cuda" else None))
+    dev = _seq.on_device(("dout", dout), ("ids", ids if ids.is_cuda else None))
     if ids.device != dev:
         if _seq.capturing():
             raise ValueError("ids must lie on the GPU while a graph is captured")
