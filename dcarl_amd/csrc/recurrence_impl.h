@@ -140,7 +140,7 @@ struct RecFind {
     }
 };
 
-// A call of one tile (one step of every live episode, short batches) finds its flags itself, in LDS, and saves the launch that finds them for longer ones.
+// A call of one tile (short batches) finds its flags itself, in LDS, and saves the launch that finds them for longer ones.
 template <int TILE> struct RecOwn {
     uint64_t flag[TILE / 8 + 2];
     int32_t ep[TILE];
