@@ -47,11 +47,14 @@ class _Lookup(torch.autograd.Function):
     def forward(ctx, table, ids, scale):
         ctx.save_for_backward(ids)
         ctx.rest = table.shape[0], scale
+        ctx.captured = _seq.capturing()
         return _seq.run_on(table.device, _gather, table, ids, scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        if not ctx.captured and _seq.capturing():
+            raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
         return _seq.run_on(dout.device, _gradient, dout, ctx.saved_tensors[0], *ctx.rest), None, None
 
 
@@ -61,7 +64,9 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
     table: (S, D) float64, float32, bfloat16 or float16 on the GPU, rows at any distance; ids: int32 or int64.
     The gradient of the table is dense, of the table's type: per id the sum over the batch in ascending order, held in f32 (f64), scaled and
     rounded once; rows no id names are zero.  validate: raise IndexError for ids outside [-1, S), which waits for them; with
-    ``validate=False`` nothing waits (a captured call needs it) and such ids count as -1."""
+    ``validate=False`` nothing waits (a captured call needs it) and such ids count as -1.
+    A backward pass is captured into a graph as that of ``episodes.gated_recurrence`` is: with its forward pass, through ``torch.autograd.grad`` on
+    leaves of the graph's own, or by ``lookup_gradient``."""
     _seq.type_code("table", table)
     if table.dim() != 2:
         raise ValueError(f"table must be (S, D), not {tuple(table.shape)}")

@@ -707,3 +707,73 @@ def test_recurrence_of_about_a_step_each(dc, t, D, kind):
             dh[off[-1]:] = math.nan
         for reverse in (False, True):
             check_recurrence(dc, x, gate, off, h0 if i != 3 else None, dh, dl, reverse, t)
+
+
+def test_lookup_and_its_gradient_captured(dc):
+    table = torch.randn(70, 40, device="cuda")
+    ids = torch.randint(-1, 70, (9000,), device="cuda")
+    w = torch.randn(9000, 40, device="cuda")
+
+    def step():
+        leaf = table.detach().requires_grad_()
+        rows = dc.tables.lookup(leaf, ids, 0.5, validate=False)
+        return rows.detach(), torch.autograd.grad(rows, leaf, w)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        table.normal_()
+        w.normal_()
+        ids.copy_(torch.randint(-1, 70, ids.shape, device="cuda"))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    eager = dc.tables.lookup(table.detach().requires_grad_(), ids, validate=False)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="outside of the graph"):
+        other = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(other):
+            table.mul(1.0)
+            dc.tables._Lookup.backward(eager.grad_fn, w)
+    torch.cuda.synchronize()
+
+
+def test_steps_of_live_episodes_captured(dc):
+    """Serving: a row per live episode, a step of each, scores and what may be answered, in one graph that keeps its states in place."""
+    E, S, D, V = 30, 50, 24, 70
+    gen = torch.Generator().manual_seed(2)
+    table, out = torch.randn(S, D, generator=gen).cuda(), torch.randn(D, V, generator=gen).cuda()
+    ids, taken = torch.zeros(E, dtype=torch.int64, device="cuda"), torch.zeros(E, dtype=torch.int64, device="cuda")
+    one = torch.arange(E + 1, device="cuda")
+    gate = torch.rand(E, D, generator=gen).cuda()
+    state = torch.zeros(E, D, device="cuda")
+    z = torch.zeros(E, V, device="cuda")
+
+    def step(state):
+        h = dc.episodes.gated_recurrence(dc.tables.lookup(table, ids, validate=False), gate, one, state, validate=False)
+        dc.candidates.adjust(h @ out, taken, one, presence=0.5, out=z)
+        return h
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(state)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        state.copy_(step(state))
+    state.zero_()
+    want = torch.zeros_like(state)
+    for _ in range(5):
+        ids.copy_(torch.randint(-1, S, (E,), generator=gen))
+        taken.copy_(torch.randint(0, V, (E,), generator=gen))
+        graph.replay()
+        got = z.clone()
+        want = step(want)
+        torch.cuda.synchronize()
+        assert torch.equal(state, want) and torch.equal(got, z)
