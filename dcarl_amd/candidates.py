@@ -84,7 +84,8 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
     entries at a history's front were handed to the policy and not chosen by it: ``n`` counts the others, "taken before" looks at all.
     repetition (> 0), frequency, presence: r, f, p, a number or a float32 tensor (B,).  bias: float32 (V,) or (B, V).
     allowed: int32 words of ``pack_allowed``, (ceil(V/32),) or (B, ceil(V/32)); a row that allows nothing is -inf throughout.
-    out: where the result goes; ``out=scores`` adjusts in place, and out lies over no other operand.  validate: check taken_off's values (waits for them when they are on
+    out: where the result goes; ``out=scores`` adjusts in place, and out lies over no other operand.  Autograd sees that write as it sees torch's own
+    in-place ones: a gradient that needs what out held before raises.  validate: check taken_off's values (waits for them when they are on
     the GPU); without it, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one are refused."""
     if not isinstance(scores, torch.Tensor) or scores.dtype not in SCORE_TYPES:
         raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
@@ -137,4 +138,6 @@ def _adjust(scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias
                      ld_bias, at(allowed), ld_allowed, rep0 if rep is None else 1.0, freq0, pres0, _seq.TYPES[s.dtype],
                      4 if taken is None else taken.element_size(), 0)
     _lib.check(_lib.load().dcarl_adjust_scores(C.byref(a), at(z), z.stride(0), _seq.stream(dev)), "dcarl_adjust_scores")
+    if out is not None:
+        torch.autograd.graph.increment_version(out)          # written through its address: autograd sees what it saved there change
     return z

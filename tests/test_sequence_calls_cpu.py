@@ -1,0 +1,85 @@
+"""What the sequence operators hand to their kernels and leave behind, seen on the CPU: the launch is replaced by one that computes a marked result in
+the same memory."""
+import os
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, REPO)
+from dcarl_amd import _lib, _sequence, candidates, episodes, tables  # noqa: E402
+
+OFF = torch.tensor([0, 2, 5])
+
+
+def f32(address, n):
+    import ctypes
+    return np.ctypeslib.as_array((ctypes.c_float * n).from_address(address)) if n else np.zeros(0, np.float32)
+
+
+class Launches:
+    """f32 operands alone: adjust adds 100, the recurrence 1000, its gradient is 7 dh; rows by numpy."""
+    calls = 0
+
+    def dcarl_recurrence_states_bytes(self, *sizes):
+        return 64
+
+    dcarl_recurrence_workspace_bytes = dcarl_rows_workspace_bytes = dcarl_recurrence_states_bytes
+
+    def dcarl_adjust_scores(self, a, out, ld, stream):
+        self.calls += 1
+        self.args = a = a._obj
+        for b in range(a.B):
+            f32(out + 4 * b * ld, a.V)[:] = f32(a.scores + 4 * b * a.ld_scores, a.V) + 100
+        return 0
+
+    def dcarl_recurrence_forward(self, a, states, ws, h, last, stream):
+        self.calls += 1
+        self.args = a = a._obj
+        f32(h, a.N * a.D)[:] = np.concatenate([f32(a.x + 4 * n * a.ldx, a.D) for n in range(a.N)]) + 1000
+        return 0
+
+    def dcarl_recurrence_backward(self, a, states, ws, dh, lddh, dlast, dx, dgate, dh0, stream):
+        self.calls += 1
+        a = a._obj
+        f32(dx, a.N * a.D)[:] = 7 * np.concatenate([f32(dh + 4 * n * lddh, a.D) for n in range(a.N)])
+        return 0
+
+    def dcarl_rows_gather(self, table, type_, ld, S, ids, width, N, D, scale, out, stream):
+        self.calls += 1
+        f32(out, N * D)[:] = scale * np.concatenate([f32(table + 4 * n * ld, D) for n in range(N)])
+        return 0
+
+    def dcarl_rows_gradient(self, dout, type_, ldd, ids, width, N, D, S, scale, ws, grad, stream):
+        self.calls += 1
+        f32(grad, S * D)[:] = np.concatenate([f32(dout + 4 * n * ldd, D) for n in range(S)])
+        return 0
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    lib = Launches()
+    monkeypatch.setattr(_lib, "load", lambda *a: lib)
+    monkeypatch.setattr(_lib, "check", lambda *a: None)
+    monkeypatch.setattr(_sequence, "on_device", lambda *named: torch.device("cpu"))
+    monkeypatch.setattr(_sequence, "run_on", lambda device, call, *args: call(*args))
+    monkeypatch.setattr(_sequence, "stream", lambda device: 0)
+    return lib
+
+
+def test_adjust_into_a_saved_tensor_is_seen_by_autograd(launches):
+    for into in (lambda p: dict(out=p.detach()), lambda p: dict(out=p.detach()[:, :2], cut=2), lambda p: dict(out=p.detach(), apart=True)):
+        kw = into(p := torch.zeros(3, 4, requires_grad=True).exp())           # exp keeps its result for its gradient
+        scores = torch.zeros(3, 4) if kw.pop("apart", False) else p.detach()[:, :kw.pop("cut", 4)]
+        candidates.adjust(scores, **kw)
+        assert launches.calls and float(p.detach()[0, 0]) >= 100
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            p.sum().backward()
+    fresh = torch.zeros(3, 4)
+    candidates.adjust(fresh)
+    assert fresh._version == 0                                               # nothing is written there
+    with torch.inference_mode():
+        kept = torch.zeros(3, 4)
+        assert candidates.adjust(kept, out=kept) is kept
