@@ -3,6 +3,7 @@ checks of ids and offsets, the device a call runs on."""
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from . import _lib
 
@@ -60,6 +61,14 @@ def like(t: torch.Tensor) -> torch.Tensor:
 
 def wants_gradient(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def no_tangent(*tensors) -> None:
+    """Refuses operands that carry a tangent: the operators have no forward-mode gradient, and a launch would drop it in silence."""
+    if getattr(_forward, "_current_level", 0) < 0:           # outside of every dual_level there are none
+        return
+    if any(isinstance(t, torch.Tensor) and _forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("the operator has no forward-mode gradient: an operand carries a tangent")
 
 
 def rows_of(t: torch.Tensor, far: int = 1 << 62):

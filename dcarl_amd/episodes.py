@@ -140,6 +140,7 @@ class _Recurrence(torch.autograd.Function):
     def backward(ctx, dh, dlast=None):
         if not ctx.captured and _seq.capturing():
             raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
+        _seq.no_tangent(dh, dlast)
         x, gate, h0, ep_off, states = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dgate, dh0 = _seq.run_on(x.device, _recurrence_backward, x, gate, ep_off, h0, *ctx.rest, states, dh, dlast, need[:3])
@@ -161,7 +162,8 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
     validate: check ep_off's values; where it lies on the GPU this waits for it.  ``validate=False`` never waits and is what a captured call
     needs; offsets that do not rise from 0 to at most N then give unspecified results (and no access out of range).
 
-    Everything runs on the tensors' device and its current stream; nothing is kept between calls.  The gradient has no gradient of its own.
+    Everything runs on the tensors' device and its current stream; nothing is kept between calls.  The gradient has no gradient of its own, and there is
+    none in forward mode: operands that carry a tangent are refused.
     A backward pass can be captured into a graph together with its forward pass, through ``torch.autograd.grad``; by itself, of a forward pass
     that ran outside, it is refused.  (``Tensor.backward`` inside a capture while an eager graph of the same leaves is alive makes autograd wait
     for the eager stream, which ends the process: capture with leaves of their own, as ``torch.autograd.grad`` on detached tensors has.)"""
@@ -178,6 +180,7 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
             raise ValueError(f"gate {tuple(gate.shape)} fits neither x {tuple(x.shape)} nor its {N} steps")
     else:
         value, gate = float(gate), None
+    _seq.no_tangent(x, gate, h0)
     E = None
     if h0 is not None:
         if _seq.type_code("h0", h0) != code:

@@ -55,6 +55,7 @@ class _Lookup(torch.autograd.Function):
     def backward(ctx, dout):
         if not ctx.captured and _seq.capturing():
             raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
+        _seq.no_tangent(dout)
         return _seq.run_on(dout.device, _gradient, dout, ctx.saved_tensors[0], *ctx.rest), None, None
 
 
@@ -63,13 +64,14 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
 
     table: (S, D) float64, float32, bfloat16 or float16 on the GPU, rows at any distance; ids: int32 or int64.
     The gradient of the table is dense, of the table's type: per id the sum over the batch in ascending order, held in f32 (f64), scaled and
-    rounded once; rows no id names are zero.  validate: raise IndexError for ids outside [-1, S), which waits for them; with
+    rounded once; rows no id names are zero.  A table that carries a tangent is refused (no forward mode).  validate: raise IndexError for ids outside [-1, S), which waits for them; with
     ``validate=False`` nothing waits (a captured call needs it) and such ids count as -1.
     A backward pass is captured into a graph as that of ``episodes.gated_recurrence`` is: with its forward pass, through ``torch.autograd.grad`` on
     leaves of the graph's own, or by ``lookup_gradient``."""
     _seq.type_code("table", table)
     if table.dim() != 2:
         raise ValueError(f"table must be (S, D), not {tuple(table.shape)}")
+    _seq.no_tangent(table)
     ids = _check_ids(ids, table.shape[0], validate)
     dev = _seq.on_device(("table", table), ("ids", ids if ids.is_cuda else None))
     if ids.device != dev:
@@ -84,6 +86,7 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
 def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: bool = True):
     """The gradient of ``lookup``'s table by itself: (n_rows, D) with row s = scale * the sum of ``dout`` (ids' shape, D) over ids == s."""
     _seq.type_code("dout", dout)
+    _seq.no_tangent(dout)
     n_rows = int(n_rows)
     if n_rows < 0:
         raise ValueError(f"n_rows = {n_rows} is negative")

@@ -83,3 +83,39 @@ def test_adjust_into_a_saved_tensor_is_seen_by_autograd(launches):
     with torch.inference_mode():
         kept = torch.zeros(3, 4)
         assert candidates.adjust(kept, out=kept) is kept
+
+
+def test_tangents_are_refused_not_dropped(launches):
+    x, h0, table, dout = torch.ones(5, 3), torch.ones(2, 3), torch.ones(4, 3), torch.ones(2, 3)
+    gate, per_row = torch.ones(5, 3), torch.ones(5)
+    need = torch.ones(5, 3, requires_grad=True)
+    back = episodes.gated_recurrence(need, 0.5, OFF)
+    rows_need = torch.ones(4, 3, requires_grad=True)
+    rows_back = tables.lookup(rows_need, [0, 1])
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))      # noqa: E731
+        before = launches.calls
+        for call in (lambda: episodes.gated_recurrence(dual(x), 0.5, OFF),
+                     lambda: episodes.gated_recurrence(dual(x).requires_grad_(), 0.5, OFF),
+                     lambda: episodes.gated_recurrence(x, dual(gate), OFF),
+                     lambda: episodes.gated_recurrence(x, dual(gate)[:, 0], OFF),
+                     lambda: episodes.gated_recurrence(x, 0.5, OFF, dual(h0)),
+                     lambda: episodes.gated_recurrence(need, gate, OFF, dual(h0)),
+                     lambda: episodes.gated_recurrence(dual(x)[:, 0], 0.5, OFF, reverse=True),
+                     lambda: torch.autograd.grad(back, need, dual(x)),
+                     lambda: tables.lookup(dual(table), [0, 1]),
+                     lambda: tables.lookup_gradient(dual(dout), [0, 1], 4),
+                     lambda: torch.autograd.grad(rows_back, rows_need, dual(dout)),
+                     lambda: candidates.adjust(dual(x)),
+                     lambda: candidates.adjust(x, bias=dual(x)),
+                     lambda: candidates.adjust(x, bias=dual(x)[0]),
+                     lambda: candidates.adjust(x, repetition=dual(per_row)),
+                     lambda: candidates.adjust(x, frequency=dual(per_row)),
+                     lambda: candidates.adjust(x, presence=dual(per_row)),
+                     lambda: candidates.adjust(x, out=dual(x.clone()))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        assert launches.calls == before
+        episodes.gated_recurrence(x, 0.5, OFF)                               # no tangent: an ordinary call inside the level too
+        assert launches.calls == before + 1
+    episodes.gated_recurrence(x, 0.5, OFF)
