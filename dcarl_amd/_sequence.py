@@ -71,6 +71,16 @@ def no_tangent(*tensors) -> None:
         raise ValueError("the operator has no forward-mode gradient: an operand carries a tangent")
 
 
+_proxies = getattr(torch._C, "_TorchDispatchModeKey", None) and torch._C._TorchDispatchModeKey.PROXY
+
+
+def no_trace(launched: bool = True) -> None:
+    """Refuses to be traced: a launch through addresses leaves no node behind, so the record would hold the allocation of the result alone and
+    replay whatever lies there.  An autograd function (launched False) is a node of torch.jit's own and runs again on replay; to make_fx it is none."""
+    if _proxies is not None and torch._C._get_dispatch_mode(_proxies) is not None or launched and torch._C._get_tracing_state() is not None:
+        raise ValueError("the operator cannot be traced: the trace would not hold its launch (capture a graph instead)")
+
+
 def rows_of(t: torch.Tensor, far: int = 1 << 62):
     """(tensor, elements between its rows) of a 2-D operand whose channels are contiguous; a copy where they are not.  Rows may lie
     anywhere at a non-negative distance (slices, one row expanded to many) of up to `far` elements, or of their own width."""

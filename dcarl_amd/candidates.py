@@ -86,13 +86,15 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
     allowed: int32 words of ``pack_allowed``, (ceil(V/32),) or (B, ceil(V/32)); a row that allows nothing is -inf throughout.
     out: where the result goes; ``out=scores`` adjusts in place, and out lies over no other operand.  Autograd sees that write as it sees torch's own
     in-place ones: a gradient that needs what out held before raises.  validate: check taken_off's values (waits for them when they are on
-    the GPU); without it, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one, or carry a tangent, are refused."""
+    the GPU); without it, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one, or carry a tangent, are refused, and so is a
+    call under torch.jit.trace or make_fx, whose record would not hold it."""
     if not isinstance(scores, torch.Tensor) or scores.dtype not in SCORE_TYPES:
         raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
     if scores.dim() != 2:
         raise ValueError(f"scores must be (B, V), not {tuple(scores.shape)}")
     if _seq.wants_gradient(scores, *(t for t in (repetition, frequency, presence, bias) if isinstance(t, torch.Tensor))):
         raise ValueError("adjust has no gradient: detach the scores, strengths and biases")
+    _seq.no_trace()
     _seq.no_tangent(scores, repetition, frequency, presence, bias, out)
     B, V = scores.shape
     if (taken is None) != (taken_off is None):

@@ -141,6 +141,7 @@ class _Recurrence(torch.autograd.Function):
         if not ctx.captured and _seq.capturing():
             raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
         _seq.no_tangent(dh, dlast)
+        _seq.no_trace()
         x, gate, h0, ep_off, states = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dgate, dh0 = _seq.run_on(x.device, _recurrence_backward, x, gate, ep_off, h0, *ctx.rest, states, dh, dlast, need[:3])
@@ -166,7 +167,8 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
     none in forward mode: operands that carry a tangent are refused.
     A backward pass can be captured into a graph together with its forward pass, through ``torch.autograd.grad``; by itself, of a forward pass
     that ran outside, it is refused.  (``Tensor.backward`` inside a capture while an eager graph of the same leaves is alive makes autograd wait
-    for the eager stream, which ends the process: capture with leaves of their own, as ``torch.autograd.grad`` on detached tensors has.)"""
+    for the eager stream, which ends the process: capture with leaves of their own, as ``torch.autograd.grad`` on detached tensors has.)
+    A call that torch.jit.trace or make_fx would record without its launch is refused."""
     code = _seq.type_code("x", x)
     flat = x.dim() == 1
     if x.dim() not in (1, 2):
@@ -198,7 +200,9 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
         x, h0 = x.unsqueeze(1), None if h0 is None else h0.unsqueeze(1)
     if gate is not None and gate.dim() == 1 and x.shape[1] == 1:
         gate = gate.unsqueeze(1)                              # one channel: shared or not is the same
-    if _seq.wants_gradient(x, gate, h0):
+    gradient = _seq.wants_gradient(x, gate, h0)
+    _seq.no_trace(not gradient)
+    if gradient:
         out = _Recurrence.apply(x, gate, h0, off, value, bool(reverse), bool(want_last))
     else:
         h, last, _ = _seq.run_on(dev, _recurrence_forward, x, gate, off, h0, value, bool(reverse), bool(want_last), False)

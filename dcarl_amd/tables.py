@@ -56,6 +56,7 @@ class _Lookup(torch.autograd.Function):
         if not ctx.captured and _seq.capturing():
             raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
         _seq.no_tangent(dout)
+        _seq.no_trace()
         return _seq.run_on(dout.device, _gradient, dout, ctx.saved_tensors[0], *ctx.rest), None, None
 
 
@@ -67,7 +68,7 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
     rounded once; rows no id names are zero.  A table that carries a tangent is refused (no forward mode).  validate: raise IndexError for ids outside [-1, S), which waits for them; with
     ``validate=False`` nothing waits (a captured call needs it) and such ids count as -1.
     A backward pass is captured into a graph as that of ``episodes.gated_recurrence`` is: with its forward pass, through ``torch.autograd.grad`` on
-    leaves of the graph's own, or by ``lookup_gradient``."""
+    leaves of the graph's own, or by ``lookup_gradient``.  A call that torch.jit.trace or make_fx would record without its launch is refused."""
     _seq.type_code("table", table)
     if table.dim() != 2:
         raise ValueError(f"table must be (S, D), not {tuple(table.shape)}")
@@ -78,7 +79,9 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
         if _seq.capturing():
             raise ValueError("ids must lie on the GPU while a graph is captured")
         ids = ids.to(dev)
-    if _seq.wants_gradient(table):
+    gradient = _seq.wants_gradient(table)
+    _seq.no_trace(not gradient)
+    if gradient:
         return _Lookup.apply(table, ids, float(scale))
     return _seq.run_on(dev, _gather, table, ids, float(scale))
 
@@ -87,6 +90,7 @@ def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: boo
     """The gradient of ``lookup``'s table by itself: (n_rows, D) with row s = scale * the sum of ``dout`` (ids' shape, D) over ids == s."""
     _seq.type_code("dout", dout)
     _seq.no_tangent(dout)
+    _seq.no_trace()
     n_rows = int(n_rows)
     if n_rows < 0:
         raise ValueError(f"n_rows = {n_rows} is negative")

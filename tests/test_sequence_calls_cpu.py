@@ -119,3 +119,29 @@ def test_tangents_are_refused_not_dropped(launches):
         episodes.gated_recurrence(x, 0.5, OFF)                               # no tangent: an ordinary call inside the level too
         assert launches.calls == before + 1
     episodes.gated_recurrence(x, 0.5, OFF)
+
+
+def make_fx(f, *args):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    return make_fx(f)(*args)
+
+
+def test_a_trace_that_would_hold_no_launch_is_refused(launches):
+    x, ids = torch.arange(15.0).view(5, 3), torch.tensor([0, 1])
+    calls = (lambda x: episodes.gated_recurrence(x, 0.5, OFF, validate=False), lambda x: episodes.gated_recurrence(x[:, 0], 0.5, OFF, validate=False, want_last=True)[0],
+             lambda x: tables.lookup(x, ids, validate=False), lambda x: tables.lookup_gradient(x[:2], ids, 4, validate=False), lambda x: candidates.adjust(x),
+             lambda x: candidates.adjust(torch.zeros(5, 3), bias=x))
+    for call in calls:
+        with pytest.raises(ValueError, match="trace"):
+            torch.jit.trace(call, x, check_trace=False)
+        with pytest.raises(ValueError, match="trace"):
+            make_fx(call, x)
+        call(x)
+    for call in calls[:3]:
+        with pytest.raises(ValueError, match="trace"):                       # with gradients too: the launch is in no such record
+            make_fx(call, x.clone().requires_grad_())
+    # what runs the operators again on replay is a record of them: torch.jit.trace through the autograd function, torch.compile around them
+    f = torch.jit.trace(calls[0], x.clone().requires_grad_(), check_trace=False)
+    assert torch.equal(f(x + 1), x + 1001)
+    y = (x + 2).requires_grad_()
+    assert torch.equal(f(y), x + 1002) and torch.equal(torch.autograd.grad(f(y).sum(), y)[0], torch.full((5, 3), 7.0))
