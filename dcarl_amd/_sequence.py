@@ -50,8 +50,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda in
 
 
 def at(t):
-    """The address of a tensor, None where there is none."""
-    return None if t is None else t.data_ptr()
+    """The address of a tensor, None where there is none.  A wrapper that has elements and no address (functionalize's, a tangent's lazy zeros) is no
+    absent operand."""
+    if t is None:
+        return None
+    p = t.data_ptr()
+    if not p and t.numel():
+        raise ValueError(f"an operand {tuple(t.shape)} has no memory behind it that a kernel could read")
+    return p
 
 
 def like(t: torch.Tensor) -> torch.Tensor:

@@ -88,8 +88,8 @@ def _recurrence_args(x, gate, ep_off, h0, gate_value, reverse):
     if h0 is not None:
         h0, ldh0 = _seq.rows_of(h0)
     N, D = x.shape
-    a = _lib.CRecurrence(N, D, ep_off.numel() - 1, ep_off.data_ptr(), x.data_ptr(), ldx, 0 if gate is None else gate.data_ptr(), ldg,
-                         0 if h0 is None else h0.data_ptr(), ldh0, gate_value, kind, int(reverse), _seq.TYPES[x.dtype], 0)
+    a = _lib.CRecurrence(N, D, ep_off.numel() - 1, _seq.at(ep_off), _seq.at(x), ldx, _seq.at(gate), ldg,
+                         _seq.at(h0), ldh0, gate_value, kind, int(reverse), _seq.TYPES[x.dtype], 0)
     return a, (x, gate, h0)                                   # the tensors: alive until the launch
 
 

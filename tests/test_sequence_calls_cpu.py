@@ -145,3 +145,20 @@ def test_a_trace_that_would_hold_no_launch_is_refused(launches):
     assert torch.equal(f(x + 1), x + 1001)
     y = (x + 2).requires_grad_()
     assert torch.equal(f(y), x + 1002) and torch.equal(torch.autograd.grad(f(y).sum(), y)[0], torch.full((5, 3), 7.0))
+
+
+def test_operands_without_memory_are_refused_not_left_out(launches):
+    """Wrappers that have a shape but no address: an optional operand of that kind must not count as absent."""
+    x, h0, bias, allowed = torch.ones(5, 3), torch.ones(2, 3), torch.ones(3), torch.ones(1, dtype=torch.int32)
+    functional = torch.func.functionalize
+    for call, arg in ((lambda b: candidates.adjust(x, bias=b), bias), (lambda b: candidates.adjust(x, bias=b), torch.ones(5, 3)), (lambda b: candidates.adjust(x, allowed=b), allowed),
+                      (lambda b: candidates.adjust(x, given=b), torch.ones(5, dtype=torch.int32)), (lambda b: candidates.adjust(x, repetition=b), torch.ones(5)),
+                      (lambda b: candidates.adjust(x, b, torch.zeros(6, dtype=torch.int64)), torch.ones(2, dtype=torch.int64)),
+                      (lambda b: candidates.adjust(x, torch.ones(2, dtype=torch.int64), b), torch.zeros(6, dtype=torch.int64)), (candidates.adjust, x),
+                      (lambda b: episodes.gated_recurrence(x, 0.5, OFF, b), h0), (lambda b: episodes.gated_recurrence(x, b, OFF, h0), torch.ones(5)),
+                      (lambda b: episodes.gated_recurrence(b, 0.5, OFF, h0), x), (lambda b: tables.lookup(b, [0, 1]), x), (lambda b: tables.lookup_gradient(b, [0, 1], 2), torch.ones(2, 3))):
+        before = launches.calls
+        with pytest.raises(ValueError, match="no memory"):
+            functional(call)(arg)
+        assert launches.calls == before
+        call(arg)
