@@ -87,9 +87,15 @@ def no_trace(launched: bool = True) -> None:
         raise ValueError("the operator cannot be traced: the trace would not hold its launch (capture a graph instead)")
 
 
+def plain(t):
+    """A tensor whose memory holds its values: a lazily negated view (the imaginary part of a conjugate) is written out."""
+    return t.resolve_neg() if t is not None and t.is_neg() else t
+
+
 def rows_of(t: torch.Tensor, far: int = 1 << 62):
     """(tensor, elements between its rows) of a 2-D operand whose channels are contiguous; a copy where they are not.  Rows may lie
     anywhere at a non-negative distance (slices, one row expanded to many) of up to `far` elements, or of their own width."""
+    t = plain(t)
     step, one = t.stride()
     if one != 1 and t.shape[1] > 1 or step < 0 or step > far and step > t.shape[1]:
         t = t.contiguous()
@@ -106,7 +112,7 @@ def whole_numbers(name: str, t) -> torch.Tensor:
         t = torch.as_tensor(t)
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
-    return t
+    return plain(t)
 
 
 def offsets(name: str, off, n: int, segments, validate: bool) -> torch.Tensor:

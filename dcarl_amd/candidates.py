@@ -27,7 +27,7 @@ def _strength(name, v, B):
     if isinstance(v, torch.Tensor):
         if v.dtype != torch.float32 or tuple(v.shape) != (B,):
             raise ValueError(f"{name} must be a number or a float32 tensor ({B},), not {v.dtype} {tuple(v.shape)}")
-        return v.contiguous(), 0.0
+        return _seq.plain(v).contiguous(), 0.0
     v = float(v)
     if v != v or (name == "repetition" and not v > 0.0):
         raise ValueError(f"{name} = {v}" + (" is not positive" if name == "repetition" else ""))
@@ -40,7 +40,7 @@ def _per_row(name, t, B, width, dtype):
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
     if tuple(t.shape) == (width,):
-        return t.contiguous(), 0
+        return _seq.plain(t).contiguous(), 0
     if tuple(t.shape) != (B, width):
         raise ValueError(f"{name} {tuple(t.shape)} is neither ({width},) nor ({B}, {width})")
     return _seq.rows_of(t)
@@ -116,6 +116,8 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
             raise ValueError(f"out must be a {scores.dtype} tensor {tuple(scores.shape)}")
         if V > 1 and out.stride(1) != 1 or B > 1 and out.stride(0) < V:
             raise ValueError("out must have contiguous rows that do not overlap")
+        if out.is_neg():
+            raise ValueError("out is a lazily negated view")
         if out.requires_grad:
             raise ValueError("out requires a gradient")
         if _half_over(scores, out):
@@ -135,7 +137,7 @@ def _adjust(scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias
     dev = scores.device
     s, ld = _seq.rows_of(scores)
     z = _seq.like(s) if out is None else out
-    given = None if given is None else given.contiguous()
+    given = None if given is None else _seq.plain(given).contiguous()
     at = _seq.at
     a = _lib.CScores(at(s), B, V, ld, at(taken), at(off), 0 if taken is None else taken.numel(), at(given), at(rep), at(freq), at(pres), at(bias),
                      ld_bias, at(allowed), ld_allowed, rep0 if rep is None else 1.0, freq0, pres0, _seq.TYPES[s.dtype],

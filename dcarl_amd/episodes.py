@@ -83,6 +83,7 @@ def _recurrence_args(x, gate, ep_off, h0, gate_value, reverse):
     if kind == 2:
         gate, ldg = _seq.rows_of(gate, _FAR)
     elif kind == 1:
+        gate = _seq.plain(gate)
         gate, ldg = (gate, gate.stride(0)) if 0 <= gate.stride(0) <= _FAR else (gate.contiguous(), 1)
     ldh0 = 0
     if h0 is not None:
@@ -114,7 +115,7 @@ def _recurrence_backward(x, gate, ep_off, h0, gate_value, reverse, states, dh, d
     lib, dev = _lib.load(), x.device
     a, keep = _recurrence_args(x, gate, ep_off, h0, gate_value, reverse)
     dh, lddh = _seq.rows_of(dh, _FAR)
-    dlast = None if dlast is None else dlast.contiguous()
+    dlast = None if dlast is None else _seq.plain(dlast).contiguous()
     dx = _seq.like(x) if want[0] else None
     dgate = _seq.like(gate) if want[1] else None
     dh0 = _seq.like(h0) if want[2] else None

@@ -1,5 +1,6 @@
 """What the sequence operators hand to their kernels and leave behind, seen on the CPU: the launch is replaced by one that computes a marked result in
 the same memory."""
+import ctypes
 import os
 import sys
 
@@ -15,13 +16,17 @@ OFF = torch.tensor([0, 2, 5])
 
 
 def f32(address, n):
-    import ctypes
     return np.ctypeslib.as_array((ctypes.c_float * n).from_address(address)) if n else np.zeros(0, np.float32)
 
 
 class Launches:
     """f32 operands alone: adjust adds 100, the recurrence 1000, its gradient is 7 dh; rows by numpy."""
     calls = 0
+
+    def seen(self, a):
+        """The first word of every operand, as it lies in memory during the launch."""
+        self.first = {k: f32(p, 1)[0] for k, t in a._fields_ if t is ctypes.c_void_p and (p := getattr(a, k))}
+        return a
 
     def dcarl_recurrence_states_bytes(self, *sizes):
         return 64
@@ -30,14 +35,14 @@ class Launches:
 
     def dcarl_adjust_scores(self, a, out, ld, stream):
         self.calls += 1
-        self.args = a = a._obj
+        a = self.seen(a._obj)
         for b in range(a.B):
             f32(out + 4 * b * ld, a.V)[:] = f32(a.scores + 4 * b * a.ld_scores, a.V) + 100
         return 0
 
     def dcarl_recurrence_forward(self, a, states, ws, h, last, stream):
         self.calls += 1
-        self.args = a = a._obj
+        a = self.seen(a._obj)
         f32(h, a.N * a.D)[:] = np.concatenate([f32(a.x + 4 * n * a.ldx, a.D) for n in range(a.N)]) + 1000
         return 0
 
@@ -162,3 +167,42 @@ def test_operands_without_memory_are_refused_not_left_out(launches):
             functional(call)(arg)
         assert launches.calls == before
         call(arg)
+
+
+def negated(t):
+    """t as a lazily negated view: what lies in memory has the other sign."""
+    n = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert n.is_neg() and torch.equal(n, t)
+    return n
+
+
+def test_lazily_negated_operands_have_their_sign(launches):
+    x, table = torch.randn(5, 3), torch.randn(4, 1)
+    for v in (x, x[:, :1], x[:, 0]):
+        assert torch.equal(episodes.gated_recurrence(negated(v), 0.5, OFF), v + 1000)
+        need = v.clone().requires_grad_()
+        h = episodes.gated_recurrence(need, 0.5, OFF)
+        assert torch.equal(torch.autograd.grad(h, need, negated(v))[0], 7 * v)
+        need = v.clone().requires_grad_()
+        h = episodes.gated_recurrence(torch._neg_view(need), 0.5, OFF)       # through the view's own gradient
+        assert torch.equal(h, 1000 - v) and torch.equal(torch.autograd.grad(h, need, torch.ones_like(h))[0], torch.full_like(v, -7))
+    for gate in (x, x[:, 0]):
+        episodes.gated_recurrence(x, negated(gate), OFF, negated(x[:2]))
+        assert launches.first["gate"] == gate.flatten()[0] and launches.first["h0"] == x[0, 0]
+    assert torch.equal(tables.lookup(negated(table), [0, 1]), table[:2]) and torch.equal(tables.lookup_gradient(negated(table), [0, 1, 2, 3], 2, validate=False), table[:2])
+    need = torch.randn(4, 1, requires_grad=True)
+    assert torch.equal(torch.autograd.grad(tables.lookup(need, [0, 1, 2, 3]), need, negated(table))[0], table)
+    ids = torch._neg_view(torch.tensor([-1, 0, -2], dtype=torch.int64))
+    assert ids.is_neg() and not _sequence.whole_numbers("ids", ids).is_neg()
+    for s in (x, x[:, :1]):
+        assert torch.equal(candidates.adjust(negated(s)), s + 100)
+    for name, v in (("bias", x), ("bias", x[0]), ("repetition", x[:, 0].abs()), ("frequency", x[:, 0]), ("presence", x[:, 0])):
+        candidates.adjust(x, **{name: negated(v)})
+        assert launches.first[name] == v.flatten()[0]
+    for name, v in (("given", torch.ones(5, dtype=torch.int32)), ("allowed", torch.ones(1, dtype=torch.int32))):
+        candidates.adjust(x, **{name: torch._neg_view(-v)})
+        assert launches.first[name].view(np.int32) == 1
+    before = launches.calls
+    with pytest.raises(ValueError, match="negated"):
+        candidates.adjust(x, out=torch._neg_view(torch.zeros(5, 3)))
+    assert launches.calls == before
