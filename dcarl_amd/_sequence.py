@@ -69,6 +69,15 @@ def wants_gradient(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def number(name: str, v) -> float:
+    """A strength, scale or discount; one that wants a gradient is refused, since none comes back to it."""
+    if isinstance(v, torch.Tensor):
+        if wants_gradient(v):
+            raise ValueError(f"{name} has no gradient: detach it")
+        no_tangent(v)
+    return float(v)
+
+
 def no_tangent(*tensors) -> None:
     """Refuses operands that carry a tangent: the operators have no forward-mode gradient, and a launch would drop it in silence."""
     if getattr(_forward, "_current_level", 0) < 0:           # outside of every dual_level there are none

@@ -217,8 +217,9 @@ def discounted_returns(rew, ep_off, gamma: float = 0.95, *, validate: bool = Tru
     """``R[t] = rew[t] + gamma * R[t+1]`` to the end of each episode: the cumulative-reward column for a discount, where ``nstep_backup``
     has the field recorder's ten-step rule.  rew: (N,) (or (N, D): D streams side by side), a tensor of a type of ``gated_recurrence`` or anything
     that becomes a float64 one; moved to the GPU where it lies elsewhere."""
+    gamma = _seq.number("gamma", gamma)
     if not isinstance(rew, torch.Tensor):
         rew = _dev64(rew, _lib.require_gpu())
     elif rew.device.type != "cuda":
         rew = rew.to(_lib.require_gpu())
-    return gated_recurrence(rew, float(gamma), ep_off, reverse=True, validate=validate)
+    return gated_recurrence(rew, gamma, ep_off, reverse=True, validate=validate)

@@ -73,6 +73,7 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
     if table.dim() != 2:
         raise ValueError(f"table must be (S, D), not {tuple(table.shape)}")
     _seq.no_tangent(table)
+    scale = _seq.number("scale", scale)
     ids = _check_ids(ids, table.shape[0], validate)
     dev = _seq.on_device(("table", table), ("ids", ids if ids.is_cuda else None))
     if ids.device != dev:
@@ -82,15 +83,19 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
     gradient = _seq.wants_gradient(table)
     _seq.no_trace(not gradient)
     if gradient:
-        return _Lookup.apply(table, ids, float(scale))
-    return _seq.run_on(dev, _gather, table, ids, float(scale))
+        return _Lookup.apply(table, ids, scale)
+    return _seq.run_on(dev, _gather, table, ids, scale)
 
 
 def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: bool = True):
-    """The gradient of ``lookup``'s table by itself: (n_rows, D) with row s = scale * the sum of ``dout`` (ids' shape, D) over ids == s."""
+    """The gradient of ``lookup``'s table by itself: (n_rows, D) with row s = scale * the sum of ``dout`` (ids' shape, D) over ids == s.
+    It has no gradient of its own: a dout that requires one is refused."""
     _seq.type_code("dout", dout)
     _seq.no_tangent(dout)
     _seq.no_trace()
+    if _seq.wants_gradient(dout):
+        raise ValueError("lookup_gradient has no gradient of its own: detach dout")
+    scale = _seq.number("scale", scale)
     n_rows = int(n_rows)
     if n_rows < 0:
         raise ValueError(f"n_rows = {n_rows} is negative")
@@ -102,4 +107,4 @@ def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: boo
         if _seq.capturing():
             raise ValueError("ids must lie on the GPU while a graph is captured")
         ids = ids.to(dev)
-    return _seq.run_on(dev, _gradient, dout, ids, n_rows, float(scale))
+    return _seq.run_on(dev, _gradient, dout, ids, n_rows, scale)

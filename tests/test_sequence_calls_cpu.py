@@ -206,3 +206,18 @@ def test_lazily_negated_operands_have_their_sign(launches):
     with pytest.raises(ValueError, match="negated"):
         candidates.adjust(x, out=torch._neg_view(torch.zeros(5, 3)))
     assert launches.calls == before
+
+
+def test_gradients_that_no_one_would_get_are_refused(launches):
+    dout = torch.ones(2, 3, requires_grad=True)
+    k = torch.tensor(0.5, requires_grad=True)
+    x, ids = torch.ones(4, 3), [0, 1]
+    for call in (lambda: tables.lookup_gradient(dout, ids, 4), lambda: tables.lookup_gradient(dout.detach(), ids, 4, k), lambda: tables.lookup(x, ids, k),
+                 lambda: tables.lookup(x.clone().requires_grad_(), ids, k), lambda: episodes.discounted_returns(x, [0, 4], k), lambda: episodes.gated_recurrence(x, 0.5 * k, [0, 4]),
+                 lambda: candidates.adjust(x, frequency=k)):
+        with pytest.raises(ValueError):
+            call()
+    assert launches.calls == 0
+    with torch.no_grad():
+        assert torch.equal(tables.lookup_gradient(dout, ids, 2), torch.ones(2, 3)) and torch.equal(tables.lookup(x, ids, k), torch.full((2, 3), 0.5))
+    assert torch.equal(tables.lookup(x, ids, k.detach()), torch.full((2, 3), 0.5))
