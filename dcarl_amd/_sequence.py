@@ -112,6 +112,20 @@ def rows_of(t: torch.Tensor, far: int = 1 << 62):
     return t, step
 
 
+def on_gpu(t):
+    """t where it lies on a GPU, else None: whole numbers may lie on the host too."""
+    return t if t is not None and t.is_cuda else None
+
+
+def from_host(name: str, t, device):
+    """Ids or offsets, moved to the call's device where they lie on the host."""
+    if t is None or t.device == device:
+        return t
+    if capturing():
+        raise ValueError(f"{name} must lie on the GPU while a graph is captured")
+    return t.to(device)
+
+
 def capturing() -> bool:
     return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
 

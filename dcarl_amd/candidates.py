@@ -79,14 +79,15 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
     """For each of B rows of V scores:  z = score;  taken before: z = z / r if z > 0 else z * r;  z -= f * n + p where n > 0;
     z += bias;  z = -inf where not allowed, whatever it was.  -> (B, V) of the scores' type, computed in f32, rounded once.
 
-    scores: (B, V) float32, bfloat16 or float16, rows at any distance.  taken: the rows' histories one after the other (int32 or int64 ids;
-    ids outside [0, V), such as -1, count nowhere), row b's is ``taken[taken_off[b]:taken_off[b+1]]``.  given: (B,) int32, how many
+    scores: (B, V) float32, bfloat16 or float16, rows at any distance.  taken: the rows' histories one after the other (int32 or int64 ids, moved
+    to the GPU where they lie on the host, as taken_off is; ids outside [0, V), such as -1, count nowhere), row b's is ``taken[taken_off[b]:taken_off[b+1]]``.  given: (B,) int32, how many
     entries at a history's front were handed to the policy and not chosen by it: ``n`` counts the others, "taken before" looks at all.
     repetition (> 0), frequency, presence: r, f, p, a number or a float32 tensor (B,).  bias: float32 (V,) or (B, V).
     allowed: int32 words of ``pack_allowed``, (ceil(V/32),) or (B, ceil(V/32)); a row that allows nothing is -inf throughout.
     out: where the result goes; ``out=scores`` adjusts in place, and out lies over no other operand.  Autograd sees that write as it sees torch's own
     in-place ones: a gradient that needs what out held before raises.  validate: check taken_off's values (waits for them when they are on
-    the GPU); without it, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one, or carry a tangent, are refused, and so is a
+    the GPU); without it, and by default since
+    this call stands in an answer's path, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one, or carry a tangent, are refused, and so is a
     call under torch.jit.trace or make_fx, whose record would not hold it."""
     if not isinstance(scores, torch.Tensor) or scores.dtype not in SCORE_TYPES:
         raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
@@ -127,8 +128,9 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
                 raise ValueError(f"out lies over {name}")
         if bias is not None and (_half_over(bias, out) if bias.dim() == 2 and bias.dtype == out.dtype else _over(bias, out)):
             raise ValueError("out lies partly over bias: it is bias itself or apart from it")
-    dev = _seq.on_device(("scores", scores), ("taken", taken), ("taken_off", off), ("given", given), ("repetition", rep), ("frequency", freq),
+    dev = _seq.on_device(("scores", scores), ("taken", _seq.on_gpu(taken)), ("taken_off", _seq.on_gpu(off)), ("given", given), ("repetition", rep), ("frequency", freq),
                          ("presence", pres), ("bias", bias), ("allowed", allowed), ("out", out))
+    taken, off = _seq.from_host("taken", taken, dev), _seq.from_host("taken_off", off, dev)
     return _seq.run_on(dev, _adjust, scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias, ld_bias, allowed, ld_allowed, out)
 
 

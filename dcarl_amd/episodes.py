@@ -192,11 +192,8 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
             raise ValueError(f"h0 {tuple(h0.shape)} does not hold a state like x {tuple(x.shape)} for every episode")
         E = h0.shape[0]
     off = _seq.offsets("ep_off", ep_off, N, E, validate)
-    dev = _seq.on_device(("x", x), ("gate", gate), ("h0", h0), ("ep_off", off if off.is_cuda else None))
-    if off.device != dev:
-        if _seq.capturing():
-            raise ValueError("ep_off must lie on the GPU while a graph is captured")
-        off = off.to(dev)
+    dev = _seq.on_device(("x", x), ("gate", gate), ("h0", h0), ("ep_off", _seq.on_gpu(off)))
+    off = _seq.from_host("ep_off", off, dev)
     if flat:
         x, h0 = x.unsqueeze(1), None if h0 is None else h0.unsqueeze(1)
     if gate is not None and gate.dim() == 1 and x.shape[1] == 1:

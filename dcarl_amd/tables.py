@@ -75,11 +75,8 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
     _seq.no_tangent(table)
     scale = _seq.number("scale", scale)
     ids = _check_ids(ids, table.shape[0], validate)
-    dev = _seq.on_device(("table", table), ("ids", ids if ids.is_cuda else None))
-    if ids.device != dev:
-        if _seq.capturing():
-            raise ValueError("ids must lie on the GPU while a graph is captured")
-        ids = ids.to(dev)
+    dev = _seq.on_device(("table", table), ("ids", _seq.on_gpu(ids)))
+    ids = _seq.from_host("ids", ids, dev)
     gradient = _seq.wants_gradient(table)
     _seq.no_trace(not gradient)
     if gradient:
@@ -102,9 +99,6 @@ def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: boo
     ids = _check_ids(ids, n_rows, validate)
     if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"dout {tuple(dout.shape)} has no row for each of the ids {tuple(ids.shape)}")
-    dev = _seq.on_device(("dout", dout), ("ids", ids if ids.is_cuda else None))
-    if ids.device != dev:
-        if _seq.capturing():
-            raise ValueError("ids must lie on the GPU while a graph is captured")
-        ids = ids.to(dev)
+    dev = _seq.on_device(("dout", dout), ("ids", _seq.on_gpu(ids)))
+    ids = _seq.from_host("ids", ids, dev)
     return _seq.run_on(dev, _gradient, dout, ids, n_rows, scale)

@@ -221,3 +221,18 @@ def test_gradients_that_no_one_would_get_are_refused(launches):
     with torch.no_grad():
         assert torch.equal(tables.lookup_gradient(dout, ids, 2), torch.ones(2, 3)) and torch.equal(tables.lookup(x, ids, k), torch.full((2, 3), 0.5))
     assert torch.equal(tables.lookup(x, ids, k.detach()), torch.full((2, 3), 0.5))
+
+
+def test_adjust_takes_histories_from_the_host(monkeypatch):
+    """As the other two take their ids and offsets: whole numbers on the host are moved to the scores' device."""
+    seen, moved = {}, []
+    monkeypatch.setattr(_sequence, "on_device", lambda *named: seen.update(named) or torch.device("meta"))
+    monkeypatch.setattr(_sequence, "run_on", lambda device, call, *args: moved.extend(args))
+    scores = torch.zeros(2, 5, device="meta")
+    candidates.adjust(scores, [1, 2, 4], [0, 1, 3])
+    assert seen["taken"] is None and seen["taken_off"] is None and seen["scores"] is scores
+    assert [t.device.type for t in moved if isinstance(t, torch.Tensor)] == ["meta"] * 3
+    monkeypatch.setattr(_sequence, "capturing", lambda: True)
+    for kw in (dict(taken=[1, 2, 4], taken_off=torch.zeros(3, dtype=torch.int64, device="meta")), dict(taken=torch.zeros(3, dtype=torch.int64, device="meta"), taken_off=[0, 1, 3])):
+        with pytest.raises(ValueError, match="captured"):
+            candidates.adjust(scores, **kw)
