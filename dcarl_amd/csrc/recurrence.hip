@@ -143,7 +143,7 @@ template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, co
     a.N = r.N; a.D = r.D; a.E = r.E; a.ep_off = r.ep_off; a.reverse = r.reverse; a.past = r.D * sizeof(T) % 128 == 0; a.tiles = p.tiles; a.blocks = p.blocks;
     a.x = static_cast<const T*>(r.x); a.ldx = (uint32_t)r.ldx;
     a.g = r.gate_kind ? static_cast<const T*>(r.gate) : nullptr; a.ldg = (uint32_t)r.ldg;
-    a.h0 = static_cast<const T*>(r.h0); a.ldh0 = r.ldh0;
+    a.h0 = r.E ? static_cast<const T*>(r.h0) : nullptr; a.ldh0 = r.ldh0;       // (without episodes it has no row, and row 0 is read for steps that start none)
     a.gval = (Acc)r.gate_value;
     if (p.tiles <= 1) return a;                            // finds its flags itself, waits for nothing
     a.flag = reinterpret_cast<uint8_t*>(plan + p.flag);

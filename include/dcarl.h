@@ -630,6 +630,7 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
  *   What steps behind the last episode hold counts nowhere; the outputs hold zeros there.  |g| <= 1 is right over any length; where the product of
  *   consecutive larger gates overflows the type of the sums, a state that is not zero reads inf or NaN from there on.
  *   Calls of 2^24 workgroups (2^37 elements of wide 16-bit rows; 2^31 steps of 17 channels) are refused.
+ *   E == 0: no step belongs to an episode, h0 is not looked at.
  * dcarl_recurrence_forward: h [N][D] contiguous; last (nullable) [E][D] = the state each episode ends with, h0[e] (or 0) for an empty one;
  *   states (nullable): dcarl_recurrence_states_bytes bytes the backward call wants (16-byte aligned).
  * dcarl_recurrence_backward, from the same arguments, the forward call's states, dh [N][D] (lddh elements between steps) and dlast (nullable)

@@ -49,3 +49,24 @@ def test_lazily_negated_operands(dc):
     assert torch.equal(dc.episodes.gated_recurrence(x, 0.5, off), want) and torch.equal(dc.episodes.gated_recurrence(x[:, 0], 0.5, off), want[:, 0])
     assert torch.equal(dc.tables.lookup(x, [3, 9, -1]), torch.cat([-z.imag[[3, 9]], torch.zeros(1, 1, device="cuda")]))
     assert torch.equal(dc.candidates.adjust(x), -z.imag)
+
+
+def recurrence(dc, x, gate, off, h0, E, reverse=0):
+    N, D = x.shape
+    return dc._lib.CRecurrence(N=N, D=D, E=E, ep_off=off.data_ptr(), x=x.data_ptr(), ldx=D, gate=gate.data_ptr(), ldg=D, h0=h0, ldh0=D, gate_kind=2, reverse=reverse, type=1)
+
+
+@pytest.mark.parametrize("N, D", [(40, 12), (3000, 12), (9000, 1)])
+def test_c_abi_states_without_episodes_are_not_looked_at(dc, N, D):
+    """No episode: h0 is an array of no rows, its address may be anything (here one row of NaN)."""
+    lib, stream = dc.load_library(), dc._lib.stream_ptr()
+    x, gate = torch.randn(N, D, device="cuda"), torch.rand(N, D, device="cuda")
+    off, nan = torch.zeros(1, dtype=torch.int64, device="cuda"), torch.full((1, D), math.nan, device="cuda")
+    r = recurrence(dc, x, gate, off, nan.data_ptr(), 0)
+    sizes = (N, D, 0, 1, 2)
+    states, ws = (torch.empty(f(*sizes) + 16, dtype=torch.uint8, device="cuda") for f in (lib.dcarl_recurrence_states_bytes, lib.dcarl_recurrence_workspace_bytes))
+    h, dx, dg = (torch.full((N, D), math.nan, device="cuda") for _ in range(3))
+    at = lambda t: C.c_void_p(t.data_ptr())      # noqa: E731
+    assert lib.dcarl_recurrence_forward(C.byref(r), at(states), at(ws), at(h), None, stream) == 0
+    assert lib.dcarl_recurrence_backward(C.byref(r), at(states), at(ws), at(x), D, None, at(dx), at(dg), None, stream) == 0
+    assert not h.any() and not dx.any() and not dg.any()
