@@ -218,10 +218,10 @@ void launch_recurrence_backward(const dcarl_recurrence_t& r, const void* states,
         RecWalk<T> a = rec_walk<T>(r, p, plan, ws);
         a.state = reinterpret_cast<Acc*>(plan + p.state);
         a.dh = static_cast<const T*>(dh); a.lddh = (uint32_t)lddh;
-        a.dlast = static_cast<const T*>(dlast);
+        a.dlast = r.E ? static_cast<const T*>(dlast) : nullptr;
         a.dx = static_cast<T*>(dx);
         a.dg = static_cast<T*>(dgate);
-        a.dh0 = static_cast<T*>(dh0);
+        a.dh0 = r.E ? static_cast<T*>(dh0) : nullptr;
         a.dgp = r.gate_kind == 1 && p.blocks > 1 ? reinterpret_cast<Acc*>(ws + p.dgp) : nullptr;
         rec_launch_backward<T>(a, r.gate_kind, p, st);
         if (a.dgp && a.dg)

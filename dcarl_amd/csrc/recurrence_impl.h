@@ -155,8 +155,11 @@ template <typename T, int TILE> __device__ __forceinline__ void rec_own(const Re
     }
     __syncthreads();
 }
+// (A backward pass reads what the forward one left, which may not have run yet where both are in graphs: an episode of that call, whatever lies there.)
 template <typename T, int TILE> __device__ __forceinline__ int32_t rec_ep(const RecWalk<T>& a, const RecOwn<TILE>& own, int64_t r) {
-    return a.tiles == 1 ? own.ep[r] : a.ep[r];
+    if (a.tiles == 1) return own.ep[r];
+    const int32_t e = a.ep[r];
+    return (uint32_t)e < (uint32_t)a.E ? e : 0;
 }
 
 // one thread's steps of a tile
@@ -682,7 +685,8 @@ __global__ __launch_bounds__(REC_THREADS, (REC_WAVES_BACKWARD<T, GK>)) void rec_
     }
     const RecSpan w = rec_span(a, TILE, true);             // from the end of time
     const int64_t tile = w.tile;
-    const int till = a.tiles > 1 ? a.till[tile] : -1;
+    int till = a.tiles > 1 ? a.till[tile] : -1;
+    if (till >= a.tiles) till = (int)a.tiles - 1;          // (as rec_ep: a tile that publishes, whatever lies there)
     const int64_t c0 = ((int64_t)w.blk * C + c) * VEC;
     const bool mine = c0 < a.D;
     const uint32_t cb = (uint32_t)(c0 < a.D - VEC ? c0 : a.D - VEC);

@@ -633,7 +633,7 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
  *   E == 0: no step belongs to an episode, h0 is not looked at.
  * dcarl_recurrence_forward: h [N][D] contiguous; last (nullable) [E][D] = the state each episode ends with, h0[e] (or 0) for an empty one;
  *   states (nullable): dcarl_recurrence_states_bytes bytes the backward call wants (16-byte aligned).
- * dcarl_recurrence_backward, from the same arguments, the forward call's states, dh [N][D] (lddh elements between steps) and dlast (nullable)
+ * dcarl_recurrence_backward, from the same arguments, the forward call's states (other contents: other values, no access out of range), dh [N][D] (lddh elements between steps) and dlast (nullable)
  *   [E][D]:  d[t] = dh[t] + g[t+1] d[t+1] inside the episode;  dx = d;  dgate[t] = d[t] * h[t-1] (gate_kind 1: summed over the channels);
  *   dh0[e] = g[s] d[s] (s: the first step; dlast[e] for an empty episode).  dx / dgate / dh0 nullable, contiguous; dgate must be NULL for
  *   gate_kind 0.  Both calls add up in a fixed order: run-to-run identical.  Workgroups wait for one another inside a launch, in an order that

@@ -70,3 +70,45 @@ def test_c_abi_states_without_episodes_are_not_looked_at(dc, N, D):
     assert lib.dcarl_recurrence_forward(C.byref(r), at(states), at(ws), at(h), None, stream) == 0
     assert lib.dcarl_recurrence_backward(C.byref(r), at(states), at(ws), at(x), D, None, at(dx), at(dg), None, stream) == 0
     assert not h.any() and not dx.any() and not dg.any()
+
+
+@pytest.mark.parametrize("N, D", [(9000, 12), (400_000, 1), (30_000, 70), (100, 5)])
+def test_c_abi_backward_of_states_that_no_forward_pass_wrote(dc, N, D):
+    """The values are anything, but only the call's own rows are written, and every wait ends: flags, episodes and tiles read from the states stay inside."""
+    lib, stream, E = dc.load_library(), dc._lib.stream_ptr(), 3
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    x, gate = torch.randn(N, D, device="cuda", generator=gen), torch.rand(N, D, device="cuda", generator=gen)
+    off = torch.tensor([0, N // 3, N // 2, N], device="cuda")
+    rows = torch.full((4, 5 * E, D), 7.0, device="cuda")                  # h0, dlast, dh0, dx's guard
+    at = lambda t: C.c_void_p(t.data_ptr())      # noqa: E731
+    r = recurrence(dc, x, gate, off, rows[0, 2 * E].data_ptr(), E)
+    sizes = (N, D, E, 1, 2)
+    states = torch.randint(0, 256, (lib.dcarl_recurrence_states_bytes(*sizes),), dtype=torch.uint8, device="cuda", generator=gen)
+    ws = torch.empty(lib.dcarl_recurrence_workspace_bytes(*sizes) + 16, dtype=torch.uint8, device="cuda")
+    out = torch.full((2, N + 2, D), 7.0, device="cuda")
+    for fill in (None, 0, 255, 127):
+        if fill is not None:
+            states.fill_(fill)
+        assert lib.dcarl_recurrence_backward(C.byref(r), at(states), at(ws), at(x), D, at(rows[1, 2 * E]), at(out[0, 1]), at(out[1, 1]), at(rows[2, 2 * E]), stream) == 0
+        torch.cuda.synchronize()
+        assert bool((out[:, [0, N + 1]] == 7).all()) and bool((rows[[0, 1, 3]] == 7).all()) and bool((rows[2, :2 * E] == 7).all()) and bool((rows[2, 3 * E:] == 7).all())
+
+
+def test_backward_of_a_captured_forward_pass_before_and_after_its_replay(dc):
+    N, off = 5000, torch.tensor([0, 1700, 1700, 5000], device="cuda")
+    x, gate, h0 = torch.randn(N, 9, device="cuda"), torch.rand(N, 9, device="cuda"), torch.randn(3, 9, device="cuda")
+    leaf = [v.clone().requires_grad_() for v in (x, gate, h0)]
+    want = torch.autograd.grad(dc.episodes.gated_recurrence(leaf[0], leaf[1], off, leaf[2]), leaf, torch.ones_like(x))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        dc.episodes.gated_recurrence(leaf[0], leaf[1], off, leaf[2], validate=False)
+    torch.cuda.current_stream().wait_stream(side)
+    mine = [v.detach().requires_grad_() for v in leaf]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = dc.episodes.gated_recurrence(mine[0], mine[1], off, mine[2], validate=False)
+    torch.autograd.grad(h, mine, torch.ones_like(x), retain_graph=True)    # of states not written yet: any values, no access out of range
+    torch.cuda.synchronize()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(h, mine, torch.ones_like(x)), want))
