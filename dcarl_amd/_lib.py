@@ -156,6 +156,8 @@ SIGNATURES = {
     "dcarl_recurrence_states_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32]),
     "dcarl_recurrence_forward": (_i32, [C.POINTER(CRecurrence), _vp, _vp, _vp, _vp, _vp]),
     "dcarl_recurrence_backward": (_i32, [C.POINTER(CRecurrence), _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "dcarl_recurrence_status": (_i32, [_vp]),
+    "dcarl_debug_recurrence_polls": (_i32, [_i32]),
     "dcarl_rows_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32]),
     "dcarl_rows_gather": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _i64, _i64, _f64, _vp, _vp]),
     "dcarl_rows_gradient": (_i32, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _f64, _vp, _vp, _vp]),

@@ -94,6 +94,8 @@ int64_t recurrence_workspace_bytes(int64_t, int64_t, int64_t, int, int);
 int64_t recurrence_states_bytes(int64_t, int64_t, int64_t, int, int);
 void launch_recurrence_forward(const dcarl_recurrence_t&, void*, void*, void*, void*, hipStream_t);
 void launch_recurrence_backward(const dcarl_recurrence_t&, const void*, void*, const void*, int64_t, const void*, void*, void*, void*, hipStream_t);
+int recurrence_status(hipStream_t);
+void recurrence_polls(int);
 int64_t rows_workspace_bytes(int64_t, int64_t, int64_t, int);
 void launch_rows_gather(int, const void*, int64_t, int64_t, const void*, int, int64_t, int64_t, double, void*, hipStream_t);
 void launch_rows_gradient(int, const void*, int64_t, const void*, int, int64_t, int64_t, int64_t, double, void*, void*, hipStream_t);
@@ -1109,6 +1111,19 @@ int32_t dcarl_recurrence_backward(const dcarl_recurrence_t* r, const void* state
     if (!aligned16(workspace) || !aligned16(states)) return fail(DCARL_EINVAL, "%s: workspace and states need 16-byte alignment", who);
     dcarl::launch_recurrence_backward(*r, states, workspace, dh, lddh, dlast, dx, dgate, dh0, static_cast<hipStream_t>(stream));
     return after_launch(who);
+}
+
+int32_t dcarl_recurrence_status(void* stream) {
+    const int v = dcarl::recurrence_status(static_cast<hipStream_t>(stream));
+    if (v < 0) return fail(DCARL_EDEVICE, "dcarl_recurrence_status: the stream or the fault words could not be read (a device fault?)");
+    if (v > 0) return fail(DCARL_ELAUNCH, "dcarl_recurrence: a workgroup's wait for another one was given up; results of the launches since the last "
+                                          "dcarl_recurrence_status() hold NaN behind it");
+    return DCARL_OK;
+}
+
+int32_t dcarl_debug_recurrence_polls(int32_t polls) {
+    dcarl::recurrence_polls(polls);
+    return DCARL_OK;
 }
 
 int64_t dcarl_rows_workspace_bytes(int64_t N, int64_t S, int64_t D, int32_t type) {

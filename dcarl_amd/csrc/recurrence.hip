@@ -1,4 +1,5 @@
 // The recurrence along episodes: the walk's flags, the plan of a call, the launches of the forward pass (kernels: recurrence_impl.h).
+#include <atomic>
 #include <type_traits>
 #include "recurrence_impl.h"
 
@@ -94,6 +95,14 @@ template <typename T> __global__ __launch_bounds__(256) void rec_share_kernel(co
     dg[reverse ? N - 1 - r : r] = narrow<T>(s);
 }
 
+static std::atomic<int> rec_polls{REC_POLLS};              // (a test hook lowers it)
+void recurrence_polls(int polls) { rec_polls = polls < 0 || polls > REC_POLLS ? REC_POLLS : polls; }
+int recurrence_status(hipStream_t st) {
+    if (hipStreamSynchronize(st) != hipSuccess) return -1;
+    const int f = rec_take(), b = recurrence_status_backward();
+    return f < 0 || b < 0 ? -1 : f | b;
+}
+
 static int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 
 RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind) {
@@ -140,7 +149,7 @@ int64_t recurrence_states_bytes(int64_t N, int64_t D, int64_t, int type, int gat
 template <typename T> static RecWalk<T> rec_walk(const dcarl_recurrence_t& r, const RecPlan& p, char* plan, char* ws) {
     using Acc = typename SeqType<T>::Acc;
     RecWalk<T> a{};
-    a.N = r.N; a.D = r.D; a.E = r.E; a.ep_off = r.ep_off; a.reverse = r.reverse; a.past = r.D * sizeof(T) % 128 == 0; a.tiles = p.tiles; a.blocks = p.blocks;
+    a.N = r.N; a.D = r.D; a.E = r.E; a.ep_off = r.ep_off; a.reverse = r.reverse; a.polls = rec_polls; a.past = r.D * sizeof(T) % 128 == 0; a.tiles = p.tiles; a.blocks = p.blocks;
     a.x = static_cast<const T*>(r.x); a.ldx = (uint32_t)r.ldx;
     a.g = r.gate_kind ? static_cast<const T*>(r.gate) : nullptr; a.ldg = (uint32_t)r.ldg;
     a.h0 = r.E ? static_cast<const T*>(r.h0) : nullptr; a.ldh0 = r.ldh0;       // (without episodes it has no row, and row 0 is read for steps that start none)

@@ -15,6 +15,8 @@ template <typename T> void rec_launch_backward(const RecWalk<T>& a, int gate_kin
     });
 }
 
+int recurrence_status_backward() { return rec_take(); }
+
 template void rec_launch_backward<double>(const RecWalk<double>&, int, const RecPlan&, hipStream_t);
 template void rec_launch_backward<float>(const RecWalk<float>&, int, const RecPlan&, hipStream_t);
 template void rec_launch_backward<bf16>(const RecWalk<bf16>&, int, const RecPlan&, hipStream_t);

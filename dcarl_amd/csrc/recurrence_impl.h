@@ -10,7 +10,8 @@
 //     between its episode's start and itself, tiles in its own group, whole groups before, and beyond REC_BACK groups the state published there.
 //     x and g are read once.
 // The waits end: a workgroup takes its tile by a ticket, in time order, so whatever it waits for belongs to workgroups that run already and
-// wait in turn only for earlier ones; a wait that takes REC_POLLS polls all the same gives up with NaN.  A published word is its own flag: the
+// wait in turn only for earlier ones; a wait that takes REC_POLLS polls all the same gives up with NaN
+// and says so (rec_gave_up).  A published word is its own flag: the
 // words are cleared to a pattern before the launch that no result has (rec_word), written and polled by relaxed atomics of device scope, and
 // nothing else passes between workgroups, so no fence is needed.
 // An episode's start is a flag, never a gate of zero: what lies before it is dropped, so a NaN there stays there.
@@ -32,7 +33,7 @@ template <typename T> struct RecWalk {
     using Acc = typename SeqType<T>::Acc;
     int64_t N, D, E;
     const int64_t* ep_off;
-    int reverse, past;
+    int reverse, past, polls;
     int64_t tiles;             // along the time axis
     uint32_t blocks;           // of channels
     const T *x, *g, *h0;
@@ -430,17 +431,30 @@ template <int C, typename T> constexpr int REC_TILE = REC_WAVES * (64 / C) * REC
 __device__ __forceinline__ uint32_t rec_word(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v); }
 __device__ __forceinline__ uint64_t rec_word(double v) { return v != v ? 0x7ff8000000000000ull : (uint64_t)__double_as_longlong(v); }
 template <typename W> __device__ __forceinline__ void rec_put(W* p, W w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// A wait of this unit's kernels was given up since the host last asked.  (A word per unit and device.)
+static __device__ uint32_t rec_gave_up = 0;
+static int rec_take() {                  // reads and clears it: 0 or 1, -1 where the device cannot be read
+    void* p = nullptr;
+    uint32_t v = 0;
+    const uint32_t none = 0;
+    if (hipGetSymbolAddress(&p, HIP_SYMBOL(rec_gave_up)) != hipSuccess || hipMemcpy(&v, p, sizeof(v), hipMemcpyDeviceToHost) != hipSuccess) return -1;
+    if (v && hipMemcpy(p, &none, sizeof(none), hipMemcpyHostToDevice) != hipSuccess) return -1;
+    return v != 0;
+}
 // n words, p(i) the address of the i-th, all in flight together
-template <int n, typename W, typename P> __device__ __forceinline__ void rec_poll(W (&w)[n], P&& p) {
+template <int n, typename W, typename P> __device__ __forceinline__ void rec_poll(W (&w)[n], int polls, P&& p) {
     bool all = false;
-    for (int tries = 0; !all && tries < REC_POLLS; ++tries) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) w[i] = ~(W)0;
+    for (int tries = 0; !all && tries < polls; ++tries) {
         if (tries) __builtin_amdgcn_s_sleep(1);
         all = true;
 #pragma unroll
         for (int i = 0; i < n; ++i) w[i] = __hip_atomic_load(p(i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
         for (int i = 0; i < n; ++i) all = all && w[i] != (W)~(W)0;
-    }                                                      // given up: all ones, a NaN
+    }
+    if (!all) __hip_atomic_store(&rec_gave_up, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);        // what is missing: all ones, a NaN
 }
 // a map of f32 is one 8-byte word, one of f64 two
 __device__ __forceinline__ void rec_put_map(float* p, float A, float B) {
@@ -451,29 +465,29 @@ __device__ __forceinline__ void rec_put_map(double* p, double A, double B) {
     rec_put(reinterpret_cast<uint64_t*>(p) + 1, rec_word(B));
 }
 // maps of VEC channels, p(v) where the v-th lies
-template <int VEC, typename P> __device__ __forceinline__ void rec_get_maps(P&& p, float (&A)[VEC], float (&B)[VEC]) {
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_maps(int polls, P&& p, float (&A)[VEC], float (&B)[VEC]) {
     uint64_t w[VEC];
-    rec_poll(w, [&](int v) { return reinterpret_cast<const uint64_t*>(p(v)); });
+    rec_poll(w, polls, [&](int v) { return reinterpret_cast<const uint64_t*>(p(v)); });
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { A[v] = __uint_as_float((uint32_t)w[v]); B[v] = __uint_as_float((uint32_t)(w[v] >> 32)); }
 }
-template <int VEC, typename P> __device__ __forceinline__ void rec_get_maps(P&& p, double (&A)[VEC], double (&B)[VEC]) {
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_maps(int polls, P&& p, double (&A)[VEC], double (&B)[VEC]) {
     uint64_t w[2 * VEC];
-    rec_poll(w, [&](int i) { return reinterpret_cast<const uint64_t*>(p(i / 2)) + i % 2; });
+    rec_poll(w, polls, [&](int i) { return reinterpret_cast<const uint64_t*>(p(i / 2)) + i % 2; });
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { A[v] = __longlong_as_double((long long)w[2 * v]); B[v] = __longlong_as_double((long long)w[2 * v + 1]); }
 }
 __device__ __forceinline__ void rec_put_state(float* p, float v) { rec_put(reinterpret_cast<uint32_t*>(p), rec_word(v)); }
 __device__ __forceinline__ void rec_put_state(double* p, double v) { rec_put(reinterpret_cast<uint64_t*>(p), rec_word(v)); }
-template <int VEC, typename P> __device__ __forceinline__ void rec_get_states(P&& p, float (&s)[VEC]) {
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_states(int polls, P&& p, float (&s)[VEC]) {
     uint32_t w[VEC];
-    rec_poll(w, [&](int v) { return reinterpret_cast<const uint32_t*>(p(v)); });
+    rec_poll(w, polls, [&](int v) { return reinterpret_cast<const uint32_t*>(p(v)); });
 #pragma unroll
     for (int v = 0; v < VEC; ++v) s[v] = __uint_as_float(w[v]);
 }
-template <int VEC, typename P> __device__ __forceinline__ void rec_get_states(P&& p, double (&s)[VEC]) {
+template <int VEC, typename P> __device__ __forceinline__ void rec_get_states(int polls, P&& p, double (&s)[VEC]) {
     uint64_t w[VEC];
-    rec_poll(w, [&](int v) { return reinterpret_cast<const uint64_t*>(p(v)); });
+    rec_poll(w, polls, [&](int v) { return reinterpret_cast<const uint64_t*>(p(v)); });
 #pragma unroll
     for (int v = 0; v < VEC; ++v) s[v] = __longlong_as_double((long long)w[v]);
 }
@@ -543,7 +557,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
     m.one();
     if (from >= 0) {                                       // (otherwise an episode starts with the tile: its map is all there is)
         if (j < REC_GROUP && mine && (DIR > 0 ? src < tile && src >= from : src > tile && src <= from)) {
-            rec_get_maps<VEC>([&](int v) { return a.map + at(src, v) * 2; }, m.A, m.B);
+            rec_get_maps<VEC>(a.polls, [&](int v) { return a.map + at(src, v) * 2; }, m.A, m.B);
             m.cut = src == from;
         }
         rec_scan_wave<Acc, C, VEC, DIR>(m, sh, lane, wv);
@@ -566,7 +580,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
             RecMap<Acc, VEC> q;
             q.one();
             if (mine && (DIR > 0 ? g < group : g <= (chain ? far : fg))) {
-                rec_get_maps<VEC>([&](int v) { return a.group + at(g, v) * 2; }, q.A, q.B);
+                rec_get_maps<VEC>(a.polls, [&](int v) { return a.group + at(g, v) * 2; }, q.A, q.B);
                 q.cut = g == fg;
             }
             rec_scan_groups<Acc, C, VEC, DIR>(q, lane);
@@ -574,7 +588,7 @@ __device__ __forceinline__ void rec_reach(const RecWalk<T>& a, int64_t tile, int
                 Acc st[VEC];
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) st[v] = 0;
-                if (chain) rec_get_states<VEC>([&](int v) { return a.through + at(far, v); }, st);
+                if (chain) rec_get_states<VEC>(a.polls, [&](int v) { return a.through + at(far, v); }, st);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) reached[c * VEC + v] = q.cut ? q.B[v] : rec_apply(q.A[v], st[v], q.B[v]);
             }
@@ -811,6 +825,7 @@ struct RecPlan {
 };
 RecPlan rec_plan(int64_t N, int64_t D, int type, int gate_kind);
 
+int recurrence_status_backward();
 template <typename T> void rec_launch_forward(const RecWalk<T>& a, int gate_kind, const RecPlan& p, hipStream_t st);
 template <typename T> void rec_launch_backward(const RecWalk<T>& a, int gate_kind, const RecPlan& p, hipStream_t st);
 

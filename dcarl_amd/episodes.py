@@ -210,6 +210,12 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
     return out
 
 
+def check_recurrence(stream=None) -> None:
+    """Waits for ``stream`` (a handle; default: the current one) and raises DcarlError if a recurrence on the current device gave up a wait between its
+    workgroups since the last check: NaN stands behind it then.  No launch has been seen to; every wait ends by the order of the launch."""
+    _lib.check(_lib.load().dcarl_recurrence_status(_lib.stream_ptr() if stream is None else C.c_void_p(stream)), "dcarl_recurrence_status")
+
+
 def discounted_returns(rew, ep_off, gamma: float = 0.95, *, validate: bool = True):
     """``R[t] = rew[t] + gamma * R[t+1]`` to the end of each episode: the cumulative-reward column for a discount, where ``nstep_backup``
     has the field recorder's ten-step rule.  rew: (N,) (or (N, D): D streams side by side), a tensor of a type of ``gated_recurrence`` or anything

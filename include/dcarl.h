@@ -13,7 +13,7 @@
  *   - every pointer is a DEVICE pointer unless marked [host]; the caller owns every buffer; the library allocates no device or
  *     host memory of its own and no RESULT depends on an earlier call.  What it does keep between calls, all of it diagnostic:
  *       * one device word (static, not allocated): the fault word of the multi-wave online kernel, set by a hand-over that never
- *         arrives, read and cleared by dcarl_trace_status();
+ *         arrives, read and cleared by dcarl_trace_status(); two more of the recurrence's waits, read and cleared by dcarl_recurrence_status();
  *       * per thread, the text of the last error (dcarl_last_error) and the name of the last kernel launched (dcarl_last_kernel);
  *       * per process, a 64-entry memo {workspace address -> N, S, A, flags, element width} of the latest dcarl_ingest_group_* calls,
  *         consulted by dcarl_ingest_pack_* only to REFUSE a pack call whose arguments differ from its group call;
@@ -174,7 +174,7 @@ int32_t dcarl_trace_resume_f64(const double* R, const uint8_t* act, const int64_
  * would cost every launch what only a corrupt table needs). */
 int32_t dcarl_count_nonfinite(const void* values, int32_t value_bytes, int64_t n, int64_t* count, void* stream);
 
-/* The ONE call of this library that synchronises: waits for `stream`, then reports whether a
+/* With dcarl_recurrence_status the only call of this library that synchronises: waits for `stream`, then reports whether a
  * dcarl_trace_* launch since the previous call gave up on a cross-wave hand-over (the multi-wave online kernel orders its
  * waves through LDS counters; a wave that waits ~3e10 cycles for a partner raises a fault word and ends instead of hanging
  * the GPU or killing the context).  DCARL_OK, or DCARL_ELAUNCH with a message in dcarl_last_error() — the outputs of those
@@ -637,7 +637,7 @@ int32_t dcarl_frenet_select(const double* traj, const double* glob, const int32_
  *   [E][D]:  d[t] = dh[t] + g[t+1] d[t+1] inside the episode;  dx = d;  dgate[t] = d[t] * h[t-1] (gate_kind 1: summed over the channels);
  *   dh0[e] = g[s] d[s] (s: the first step; dlast[e] for an empty episode).  dx / dgate / dh0 nullable, contiguous; dgate must be NULL for
  *   gate_kind 0.  Both calls add up in a fixed order: run-to-run identical.  Workgroups wait for one another inside a launch, in an order that
- *   ends; should a wait fail all the same it is given up and the outputs behind it are NaN.
+ *   ends; should a wait fail all the same it is given up, the outputs behind it are NaN and dcarl_recurrence_status reports it.
  * workspace: dcarl_recurrence_workspace_bytes bytes, 16-byte aligned, contents irrelevant before / after. */
 typedef struct dcarl_recurrence {
     int64_t N, D, E;
@@ -656,6 +656,11 @@ int64_t dcarl_recurrence_states_bytes(int64_t N, int64_t D, int64_t E, int32_t t
 int32_t dcarl_recurrence_forward(const dcarl_recurrence_t* r /* [host] */, void* states, void* workspace, void* h, void* last, void* stream);
 int32_t dcarl_recurrence_backward(const dcarl_recurrence_t* r /* [host] */, const void* states, void* workspace, const void* dh, int64_t lddh,
                                   const void* dlast, void* dx, void* dgate, void* dh0, void* stream);
+/* Waits for `stream`, then reports whether a dcarl_recurrence_* launch on the current device since the previous call gave up a wait: DCARL_OK, or DCARL_ELAUNCH
+ * with a message in dcarl_last_error().  Never observed outside the test below; a caller that hands results to the host may ask here first. */
+int32_t dcarl_recurrence_status(void* stream);
+/* Test hook: later launches of this process poll at most `polls` times per wait (0: every wait is given up at once; negative: the library's own bound). */
+int32_t dcarl_debug_recurrence_polls(int32_t polls);
 /* Rows of a table by id (ids of id_bytes 4 or 8, device): out[n] = scale * table[ids[n]], [N][D] contiguous; zeros for an id outside [0, S)
  *   (dcarl_sample_pairs hands out -1 for a visit it drops).  table [S][D], ld elements between rows.
  * dcarl_rows_gradient: grad [S][D] contiguous, every row written: scale * the sum of dout[n] (ldd elements between rows) over ids[n] == s, in

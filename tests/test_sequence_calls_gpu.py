@@ -112,3 +112,48 @@ def test_backward_of_a_captured_forward_pass_before_and_after_its_replay(dc):
     torch.cuda.synchronize()
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(h, mine, torch.ones_like(x)), want))
+
+
+@pytest.fixture
+def no_polls(dc):
+    """Every wait between workgroups is given up at its first poll, from here to the end of the test."""
+    lib = dc.load_library()
+    assert lib.dcarl_recurrence_status(dc._lib.stream_ptr()) == 0
+    lib.dcarl_debug_recurrence_polls(0)
+    try:
+        yield lib
+    finally:
+        lib.dcarl_debug_recurrence_polls(-1)
+        torch.cuda.synchronize()
+        lib.dcarl_recurrence_status(dc._lib.stream_ptr())
+
+
+@pytest.mark.parametrize("D, tile, t", [(9, 512, torch.float32), (9, 512, torch.bfloat16), (1, 4096, torch.float32), (1, 2048, torch.float64), (40, 128, torch.float16)])
+def test_waits_given_up_are_reported(dc, no_polls, D, tile, t):
+    off = [0, 3 * tile + 100, 20 * tile, 20 * tile, 22 * tile + 7]
+    N = off[-1]
+    episode = np.searchsorted(off, np.arange(N), side="right") - 1
+    starts, ends = np.array(off)[episode], np.array(off)[episode + 1] - 1
+    x, gate = torch.ones(N, D, device="cuda", dtype=t), torch.full((N, D), 0.5, device="cuda", dtype=t)
+    leaf = [x.requires_grad_(), gate.requires_grad_()]
+    no_polls.dcarl_debug_recurrence_polls(-1)
+    want = dc.episodes.gated_recurrence(*leaf, off)
+    grads = torch.autograd.grad(want, leaf, torch.ones_like(x), retain_graph=True)
+    dc.episodes.check_recurrence()                                        # nothing was given up
+    no_polls.dcarl_debug_recurrence_polls(0)
+    dc.episodes.gated_recurrence(x[:90].detach(), 0.5, [0, 90])          # one tile waits for nothing
+    dc.episodes.check_recurrence()
+    inside = torch.tensor(starts // tile == np.arange(N) // tile, device="cuda")           # the episode starts in the step's own tile: no wait
+    for _ in range(2):
+        got = dc.episodes.gated_recurrence(x.detach(), gate.detach(), off)
+        with pytest.raises(dc.DcarlError, match="given up"):
+            dc.episodes.check_recurrence()
+        dc.episodes.check_recurrence()                                    # asking clears it
+        assert torch.equal(got[inside], want[inside]) and bool(got[~inside].isnan().all())
+    inside = torch.tensor(ends // tile == np.arange(N) // tile, device="cuda")
+    for a, b in zip(torch.autograd.grad(want, leaf, torch.ones_like(x)), grads):
+        assert torch.equal(a[inside], b[inside]) and bool(a[~inside].isnan().all())
+    assert no_polls.dcarl_recurrence_status(dc._lib.stream_ptr()) == -3 and b"given up" in no_polls.dcarl_last_error()
+    no_polls.dcarl_debug_recurrence_polls(-1)
+    assert torch.equal(dc.episodes.gated_recurrence(x.detach(), gate.detach(), off), want)
+    dc.episodes.check_recurrence()
