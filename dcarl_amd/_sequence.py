@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import torch
 import torch.autograd.forward_ad as _forward
+import torch.fx._symbolic_trace as _fx
 
 from . import _lib
 
@@ -66,7 +67,11 @@ def like(t: torch.Tensor) -> torch.Tensor:
 
 
 def wants_gradient(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def number(name: str, v) -> float:
@@ -74,25 +79,21 @@ def number(name: str, v) -> float:
     if isinstance(v, torch.Tensor):
         if wants_gradient(v):
             raise ValueError(f"{name} has no gradient: detach it")
-        no_tangent(v)
+        recordable(False, v)
     return float(v)
 
 
-def no_tangent(*tensors) -> None:
-    """Refuses operands that carry a tangent: the operators have no forward-mode gradient, and a launch would drop it in silence."""
-    if getattr(_forward, "_current_level", 0) < 0:           # outside of every dual_level there are none
-        return
-    if any(isinstance(t, torch.Tensor) and _forward.unpack_dual(t).tangent is not None for t in tensors):
-        raise ValueError("the operator has no forward-mode gradient: an operand carries a tangent")
+_proxies, _tracing = torch._C._TorchDispatchModeKey.PROXY, torch._C._get_tracing_state
 
 
-_proxies = getattr(torch._C, "_TorchDispatchModeKey", None) and torch._C._TorchDispatchModeKey.PROXY
-
-
-def no_trace(launched: bool = True) -> None:
-    """Refuses to be traced: a launch through addresses leaves no node behind, so the record would hold the allocation of the result alone and
-    replay whatever lies there.  An autograd function (launched False) is a node of torch.jit's own and runs again on replay; to make_fx it is none."""
-    if _proxies is not None and torch._C._get_dispatch_mode(_proxies) is not None or launched and torch._C._get_tracing_state() is not None:
+def recordable(launched: bool, *tensors) -> None:
+    """Refuses calls of which a record or a derivative would lack the launch, which goes through addresses and leaves no node behind.
+    A tangent: the operators have no forward-mode gradient.  A trace: it would hold the allocation of the result alone and replay whatever lies there;
+    an autograd function (launched False) is a node of torch.jit's own and runs again on replay, to make_fx it is none."""
+    if _forward._current_level >= 0:                         # inside of a dual_level, the only place where there are tangents
+        if any(isinstance(t, torch.Tensor) and _forward.unpack_dual(t).tangent is not None for t in tensors):
+            raise ValueError("the operator has no forward-mode gradient: an operand carries a tangent")
+    if _fx._is_fx_tracing_flag and torch._C._get_dispatch_mode(_proxies) is not None or launched and _tracing() is not None:
         raise ValueError("the operator cannot be traced: the trace would not hold its launch (capture a graph instead)")
 
 
@@ -112,15 +113,8 @@ def rows_of(t: torch.Tensor, far: int = 1 << 62):
     return t, step
 
 
-def on_gpu(t):
-    """t where it lies on a GPU, else None: whole numbers may lie on the host too."""
-    return t if t is not None and t.is_cuda else None
-
-
 def from_host(name: str, t, device):
-    """Ids or offsets, moved to the call's device where they lie on the host."""
-    if t is None or t.device == device:
-        return t
+    """Ids or offsets that lie on the host, moved to the call's device."""
     if capturing():
         raise ValueError(f"{name} must lie on the GPU while a graph is captured")
     return t.to(device)
@@ -135,7 +129,7 @@ def whole_numbers(name: str, t) -> torch.Tensor:
         t = torch.as_tensor(t)
     if t.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be int32 or int64, not {t.dtype}")
-    return plain(t)
+    return t
 
 
 def offsets(name: str, off, n: int, segments, validate: bool) -> torch.Tensor:

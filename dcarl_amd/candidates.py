@@ -40,7 +40,7 @@ def _per_row(name, t, B, width, dtype):
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
     if tuple(t.shape) == (width,):
-        return _seq.plain(t).contiguous(), 0
+        return (_seq.plain(t) if dtype.is_floating_point else t).contiguous(), 0
     if tuple(t.shape) != (B, width):
         raise ValueError(f"{name} {tuple(t.shape)} is neither ({width},) nor ({B}, {width})")
     return _seq.rows_of(t)
@@ -95,8 +95,7 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
         raise ValueError(f"scores must be (B, V), not {tuple(scores.shape)}")
     if _seq.wants_gradient(scores, *(t for t in (repetition, frequency, presence, bias) if isinstance(t, torch.Tensor))):
         raise ValueError("adjust has no gradient: detach the scores, strengths and biases")
-    _seq.no_trace()
-    _seq.no_tangent(scores, repetition, frequency, presence, bias, out)
+    _seq.recordable(True, scores, repetition, frequency, presence, bias, out)
     B, V = scores.shape
     if (taken is None) != (taken_off is None):
         raise ValueError("taken and taken_off come together")
@@ -128,9 +127,12 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
                 raise ValueError(f"out lies over {name}")
         if bias is not None and (_half_over(bias, out) if bias.dim() == 2 and bias.dtype == out.dtype else _over(bias, out)):
             raise ValueError("out lies partly over bias: it is bias itself or apart from it")
-    dev = _seq.on_device(("scores", scores), ("taken", _seq.on_gpu(taken)), ("taken_off", _seq.on_gpu(off)), ("given", given), ("repetition", rep), ("frequency", freq),
+    dev = _seq.on_device(("scores", scores), ("taken", taken if taken is not None and taken.is_cuda else None), ("taken_off", off if off is not None and off.is_cuda else None), ("given", given), ("repetition", rep), ("frequency", freq),
                          ("presence", pres), ("bias", bias), ("allowed", allowed), ("out", out))
-    taken, off = _seq.from_host("taken", taken, dev), _seq.from_host("taken_off", off, dev)
+    if taken is not None and taken.device != dev:
+        taken = _seq.from_host("taken", taken, dev)
+    if off is not None and off.device != dev:
+        off = _seq.from_host("taken_off", off, dev)
     return _seq.run_on(dev, _adjust, scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias, ld_bias, allowed, ld_allowed, out)
 
 
@@ -139,7 +141,7 @@ def _adjust(scores, taken, off, given, rep, rep0, freq, freq0, pres, pres0, bias
     dev = scores.device
     s, ld = _seq.rows_of(scores)
     z = _seq.like(s) if out is None else out
-    given = None if given is None else _seq.plain(given).contiguous()
+    given = None if given is None else given.contiguous()
     at = _seq.at
     a = _lib.CScores(at(s), B, V, ld, at(taken), at(off), 0 if taken is None else taken.numel(), at(given), at(rep), at(freq), at(pres), at(bias),
                      ld_bias, at(allowed), ld_allowed, rep0 if rep is None else 1.0, freq0, pres0, _seq.TYPES[s.dtype],

@@ -141,8 +141,7 @@ class _Recurrence(torch.autograd.Function):
     def backward(ctx, dh, dlast=None):
         if not ctx.captured and _seq.capturing():
             raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
-        _seq.no_tangent(dh, dlast)
-        _seq.no_trace()
+        _seq.recordable(True, dh, dlast)
         x, gate, h0, ep_off, states = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dgate, dh0 = _seq.run_on(x.device, _recurrence_backward, x, gate, ep_off, h0, *ctx.rest, states, dh, dlast, need[:3])
@@ -183,7 +182,8 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
             raise ValueError(f"gate {tuple(gate.shape)} fits neither x {tuple(x.shape)} nor its {N} steps")
     else:
         value, gate = float(gate), None
-    _seq.no_tangent(x, gate, h0)
+    gradient = _seq.wants_gradient(x, gate, h0)
+    _seq.recordable(not gradient, x, gate, h0)
     E = None
     if h0 is not None:
         if _seq.type_code("h0", h0) != code:
@@ -192,14 +192,13 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
             raise ValueError(f"h0 {tuple(h0.shape)} does not hold a state like x {tuple(x.shape)} for every episode")
         E = h0.shape[0]
     off = _seq.offsets("ep_off", ep_off, N, E, validate)
-    dev = _seq.on_device(("x", x), ("gate", gate), ("h0", h0), ("ep_off", _seq.on_gpu(off)))
-    off = _seq.from_host("ep_off", off, dev)
+    dev = _seq.on_device(("x", x), ("gate", gate), ("h0", h0), ("ep_off", off if off.is_cuda else None))
+    if off.device != dev:
+        off = _seq.from_host("ep_off", off, dev)
     if flat:
         x, h0 = x.unsqueeze(1), None if h0 is None else h0.unsqueeze(1)
     if gate is not None and gate.dim() == 1 and x.shape[1] == 1:
         gate = gate.unsqueeze(1)                              # one channel: shared or not is the same
-    gradient = _seq.wants_gradient(x, gate, h0)
-    _seq.no_trace(not gradient)
     if gradient:
         out = _Recurrence.apply(x, gate, h0, off, value, bool(reverse), bool(want_last))
     else:

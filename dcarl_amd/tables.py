@@ -55,8 +55,7 @@ class _Lookup(torch.autograd.Function):
     def backward(ctx, dout):
         if not ctx.captured and _seq.capturing():
             raise ValueError("the forward pass ran outside of the graph that its backward pass is captured into")
-        _seq.no_tangent(dout)
-        _seq.no_trace()
+        _seq.recordable(True, dout)
         return _seq.run_on(dout.device, _gradient, dout, ctx.saved_tensors[0], *ctx.rest), None, None
 
 
@@ -72,13 +71,13 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
     _seq.type_code("table", table)
     if table.dim() != 2:
         raise ValueError(f"table must be (S, D), not {tuple(table.shape)}")
-    _seq.no_tangent(table)
+    gradient = _seq.wants_gradient(table)
+    _seq.recordable(not gradient, table)
     scale = _seq.number("scale", scale)
     ids = _check_ids(ids, table.shape[0], validate)
-    dev = _seq.on_device(("table", table), ("ids", _seq.on_gpu(ids)))
-    ids = _seq.from_host("ids", ids, dev)
-    gradient = _seq.wants_gradient(table)
-    _seq.no_trace(not gradient)
+    dev = _seq.on_device(("table", table), ("ids", ids if ids.is_cuda else None))
+    if ids.device != dev:
+        ids = _seq.from_host("ids", ids, dev)
     if gradient:
         return _Lookup.apply(table, ids, scale)
     return _seq.run_on(dev, _gather, table, ids, scale)
@@ -88,8 +87,7 @@ def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: boo
     """The gradient of ``lookup``'s table by itself: (n_rows, D) with row s = scale * the sum of ``dout`` (ids' shape, D) over ids == s.
     It has no gradient of its own: a dout that requires one is refused."""
     _seq.type_code("dout", dout)
-    _seq.no_tangent(dout)
-    _seq.no_trace()
+    _seq.recordable(True, dout)
     if _seq.wants_gradient(dout):
         raise ValueError("lookup_gradient has no gradient of its own: detach dout")
     scale = _seq.number("scale", scale)
@@ -99,6 +97,7 @@ def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: boo
     ids = _check_ids(ids, n_rows, validate)
     if dout.dim() < 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"dout {tuple(dout.shape)} has no row for each of the ids {tuple(ids.shape)}")
-    dev = _seq.on_device(("dout", dout), ("ids", _seq.on_gpu(ids)))
-    ids = _seq.from_host("ids", ids, dev)
+    dev = _seq.on_device(("dout", dout), ("ids", ids if ids.is_cuda else None))
+    if ids.device != dev:
+        ids = _seq.from_host("ids", ids, dev)
     return _seq.run_on(dev, _gradient, dout, ids, n_rows, scale)
