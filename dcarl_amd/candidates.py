@@ -25,7 +25,7 @@ def pack_allowed(allowed):
 def _strength(name, v, B):
     """A number, or a float32 tensor with one per row."""
     if isinstance(v, torch.Tensor):
-        if v.dtype != torch.float32 or tuple(v.shape) != (B,):
+        if v.dtype != torch.float32 or v.shape != (B,):
             raise ValueError(f"{name} must be a number or a float32 tensor ({B},), not {v.dtype} {tuple(v.shape)}")
         return _seq.plain(v).contiguous(), 0.0
     v = float(v)
@@ -39,9 +39,9 @@ def _per_row(name, t, B, width, dtype):
         return None, 0
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
-    if tuple(t.shape) == (width,):
+    if t.shape == (width,):
         return (_seq.plain(t) if dtype.is_floating_point else t).contiguous(), 0
-    if tuple(t.shape) != (B, width):
+    if t.shape != (B, width):
         raise ValueError(f"{name} {tuple(t.shape)} is neither ({width},) nor ({B}, {width})")
     return _seq.rows_of(t)
 
@@ -93,7 +93,7 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
         raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
     if scores.dim() != 2:
         raise ValueError(f"scores must be (B, V), not {tuple(scores.shape)}")
-    if _seq.wants_gradient(scores, *(t for t in (repetition, frequency, presence, bias) if isinstance(t, torch.Tensor))):
+    if _seq.wants_gradient(scores, *[t if isinstance(t, torch.Tensor) else None for t in (repetition, frequency, presence, bias)]):
         raise ValueError("adjust has no gradient: detach the scores, strengths and biases")
     _seq.recordable(True, scores, repetition, frequency, presence, bias, out)
     B, V = scores.shape
@@ -106,7 +106,7 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
             raise ValueError("taken must be one-dimensional")
         taken = taken.contiguous()
         off = _seq.offsets("taken_off", taken_off, taken.numel(), B, validate)
-    if given is not None and (not isinstance(given, torch.Tensor) or given.dtype != torch.int32 or tuple(given.shape) != (B,)):
+    if given is not None and (not isinstance(given, torch.Tensor) or given.dtype != torch.int32 or given.shape != (B,)):
         raise ValueError(f"given must be an int32 tensor ({B},)")
     (rep, rep0), (freq, freq0), (pres, pres0) = (_strength(n, v, B) for n, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence)))
     bias, ld_bias = _per_row("bias", bias, B, V, torch.float32)
