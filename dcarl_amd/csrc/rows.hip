@@ -2,6 +2,8 @@
 //   forward:  out[n] = scale * table[ids[n]], zeros where ids[n] is outside [0, S) (-1 = a visit the sampler dropped, DS:50-51)
 //   gradient: grad[s] = scale * sum of dout[n] over the n with ids[n] == s, in ascending n: the ids are sorted by a stable radix sort, a row's
 //             gradient is the sum over its run -- no atomics on values, run-to-run identical
+//             (sums of f32 in f64 would take 103 us where the skewed case below takes 97, for an error of 3e-8 of the gradient's norm in place of 1.3e-7: a caller
+//             who wants that hands over dout in f64)
 // DS = Simulation_testing/Simulation_Data_Collection/Data_Sampling/data_sampling.py
 // Bound by memory: rows in 16-byte pieces, each once; a thread sums a row's channels over its run in f32.  Runs are as uneven as the visits, so those of more than
 // RW_CHUNK places are summed in chunks by workgroups of their own, then joined.  16384 ids of 50000 rows of 1024 bf16: gather 14 us (4.8 TB/s), sort 18, where the

@@ -218,7 +218,8 @@ def check_recurrence(stream=None) -> None:
 def discounted_returns(rew, ep_off, gamma: float = 0.95, *, validate: bool = True):
     """``R[t] = rew[t] + gamma * R[t+1]`` to the end of each episode: the cumulative-reward column for a discount, where ``nstep_backup``
     has the field recorder's ten-step rule.  rew: (N,) (or (N, D): D streams side by side), a tensor of a type of ``gated_recurrence`` or anything
-    that becomes a float64 one; moved to the GPU where it lies elsewhere."""
+    that becomes a float64 one; moved to the GPU where it lies elsewhere.  For types below float64 gamma is rounded to f32 and states are held in f32: an error of
+    about 3e-8 / (1 - gamma) of a return.  Where that is too much, as for discounts near 1, hand over float64 rewards."""
     gamma = _seq.number("gamma", gamma)
     if not isinstance(rew, torch.Tensor):
         rew = _dev64(rew, _lib.require_gpu())

@@ -85,7 +85,7 @@ def lookup(table, ids, scale: float = 1.0, *, validate: bool = True):
 
 def lookup_gradient(dout, ids, n_rows: int, scale: float = 1.0, *, validate: bool = True):
     """The gradient of ``lookup``'s table by itself: (n_rows, D) with row s = scale * the sum of ``dout`` (ids' shape, D) over ids == s.
-    It has no gradient of its own: a dout that requires one is refused."""
+    Sums of f32 are held in f32: ``lookup_gradient(dout.double(), ...)`` holds them in f64.  It has no gradient of its own: a dout that requires one is refused."""
     _seq.type_code("dout", dout)
     _seq.recordable(True, dout)
     if _seq.wants_gradient(dout):
