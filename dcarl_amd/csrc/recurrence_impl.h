@@ -17,7 +17,7 @@
 // An episode's start is a flag, never a gate of zero: what lies before it is dropped, so a NaN there stays there.
 // All compositions happen in a fixed order, whoever comes first: run-to-run identical.
 // Bound by memory: x, g and h once each (dh, x, g, dx, dg backward), and 8 bytes per channel and tile between workgroups (1 %).  65536 steps of 2048 channels in two
-// episodes: bf16 forward 207 us (3.9 TB/s), backward 340 (3.9); 32768 steps in f32 171 (4.7) and 282 (4.8); a copy reaches 5.0 TB/s on the same GPU.  What the 16-bit
+// episodes: bf16 forward 209 us (3.9 TB/s), backward 356 (3.8); 32768 steps in f32 168 (4.8) and 293 (4.6); a copy reaches 5.0 TB/s on the same GPU.  What the 16-bit
 // types lack is bytes in flight: a load instruction carries half as many.  Composing the parts' maps in a launch of its own, which reads x and g twice, took
 // 322 and 448 us.
 #pragma once

@@ -6,8 +6,8 @@
 //             who wants that hands over dout in f64)
 // DS = Simulation_testing/Simulation_Data_Collection/Data_Sampling/data_sampling.py
 // Bound by memory: rows in 16-byte pieces, each once; a thread sums a row's channels over its run in f32.  Runs are as uneven as the visits, so those of more than
-// RW_CHUNK places are summed in chunks by workgroups of their own, then joined.  16384 ids of 50000 rows of 1024 bf16: gather 14 us (4.8 TB/s), sort 18, where the
-// runs begin 5, chunks 7, sums and zeros 22 (6.2 TB/s); 131071 f32 rows of 257, six tenths of one id: 32, 23, 6, 23, 15.
+// RW_CHUNK places are summed in chunks by workgroups of their own, then joined.  16384 ids of 50000 rows of 1024 bf16: gather 13 us (5.1 TB/s), sort 17, where the
+// runs begin 5, chunks 7, sums and zeros 21 (6.4 TB/s); 131071 f32 rows of 257, six tenths of one id: 32, 24, 6, 23, 15.
 #include <type_traits>
 #include "seq_common.h"
 

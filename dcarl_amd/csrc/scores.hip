@@ -2,14 +2,14 @@
 //   z = s;  taken before: z = z > 0 ? z / r : z * r;  z -= f * n + p * [n > 0];  z += bias;  not allowed: z = -inf
 // n counts the row's own choices (the entries of its history behind the first given[b]), "taken before" looks at the whole history.
 // Bound by memory: scores, biases and mask bits once in, scores once out.  A row's history is read by every tile of the row (from the caches) and counted in LDS, so
-// no counts go through memory; what it costs is the wait for it.  256 rows of 151643 f32 with biases and masks: 91 us (5.2 TB/s) without history, 98 with 1000
-// entries a row, 110 with 8000.
+// no counts go through memory; what it costs is the wait for it.  256 rows of 151643 f32 with biases and masks: 86 us (5.5 TB/s) without history, 105 with 1000
+// entries a row on average, 129 with 8000.
 #include <type_traits>
 #include "seq_common.h"
 
 namespace dcarl {
 
-constexpr int SC_EPT = 8;                      // candidates per thread: 16 and 32 take registers that waiting workgroups need (91 -> 100, 122 us without history)
+constexpr int SC_EPT = 8;                      // candidates per thread: 16 and 32 take registers that waiting workgroups need (10 and 34 % more time without history)
 constexpr uint32_t SC_SEEN = 0x80000000u;
 template <typename T> constexpr int SC_VEC = 16 / sizeof(T);
 
@@ -171,7 +171,7 @@ void launch_scores(const dcarl_scores_t& s, void* out, int64_t ld_out, hipStream
                 else hipLaunchKernelGGL((scores_kernel<T, int32_t, threads()>), grid, dim3(threads()), 0, st, (const T*)s.scores, (T*)out, a);
             };
             // Every tile reads the whole history of its row.  512 threads read it half as often, 256 leave more workgroups to wait side by side:
-            // 256 rows of 151643 f32, histories of 1000: 82 (256) and 85 us (512); of 2000: 91 and 88; of 8000: 121 and 111.
+            // 256 rows of 151643 f32, histories of 1000 on average: 105 (256) and 106 us (512); of 2000: 114 and 110; of 8000: 145 and 129.
             using std::integral_constant;
             if (s.taken_off && s.n_taken / s.B >= 1536) go(integral_constant<int, 512>{});
             else go(integral_constant<int, 256>{});

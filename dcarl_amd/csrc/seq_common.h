@@ -1,4 +1,4 @@
-// What the sequence operators share (recurrence.hip, rows.hip, scores.hip): the storage types of include/dcarl.h's dcarl_type_t, the
+// What the sequence operators share (recurrence.hip, rows.hip, scores.hip): the storage types of include/dcarl.h (DCARL_F64 ... DCARL_F16), the
 // type their sums are held in (f32; f64 for f64 storage), element conversions.  These units are compiled with NaNs honoured
 // (build.py SOURCE_FLAGS): a NaN is an ordinary input here.
 #pragma once
