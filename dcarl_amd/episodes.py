@@ -212,6 +212,8 @@ def gated_recurrence(x, gate, ep_off, h0=None, *, reverse: bool = False, want_la
 def check_recurrence(stream=None) -> None:
     """Waits for ``stream`` (a handle; default: the current one) and raises DcarlError if a recurrence on the current device gave up a wait between its
     workgroups since the last check: NaN stands behind it then.  No launch has been seen to; every wait ends by the order of the launch."""
+    if _seq.capturing():
+        raise ValueError("a stream cannot be waited for while a graph is captured: check after its replay")
     _lib.check(_lib.load().dcarl_recurrence_status(_lib.stream_ptr() if stream is None else C.c_void_p(stream)), "dcarl_recurrence_status")
 
 

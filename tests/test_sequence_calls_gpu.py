@@ -157,3 +157,19 @@ def test_waits_given_up_are_reported(dc, no_polls, D, tile, t):
     no_polls.dcarl_debug_recurrence_polls(-1)
     assert torch.equal(dc.episodes.gated_recurrence(x.detach(), gate.detach(), off), want)
     dc.episodes.check_recurrence()
+
+
+def test_waits_are_not_checked_while_a_graph_is_captured(dc):
+    x = torch.ones(5000, 3, device="cuda")
+    off = torch.tensor([0, 5000], device="cuda")
+    want = dc.episodes.gated_recurrence(x, 0.5, off)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = dc.episodes.gated_recurrence(x, 0.5, off, validate=False)
+        with pytest.raises(ValueError, match="captured"):
+            dc.episodes.check_recurrence()
+    for _ in range(3):
+        graph.replay()
+        dc.episodes.check_recurrence()
+        assert torch.equal(h, want)
