@@ -86,9 +86,8 @@ def adjust(scores, taken=None, taken_off=None, *, given=None, repetition=1.0, fr
     allowed: int32 words of ``pack_allowed``, (ceil(V/32),) or (B, ceil(V/32)); a row that allows nothing is -inf throughout.
     out: where the result goes; ``out=scores`` adjusts in place, and out lies over no other operand.  Autograd sees that write as it sees torch's own
     in-place ones: a gradient that needs what out held before raises.  validate: check taken_off's values (waits for them when they are on
-    the GPU); without it, and by default since
-    this call stands in an answer's path, offsets are held to the range of ``taken``.  No gradient flows through: scores that require one, or carry a tangent, are refused, and so is a
-    call under torch.jit.trace or make_fx, whose record would not hold it."""
+    the GPU); without it, which is the default since this call stands in an answer's path, offsets are held to the range of ``taken``.
+    No gradient flows through: scores that require one, or carry a tangent, are refused, and so is a call under torch.jit.trace or make_fx, whose record would not hold it."""
     if not isinstance(scores, torch.Tensor) or scores.dtype not in SCORE_TYPES:
         raise TypeError("scores must be a float32, bfloat16 or float16 tensor")
     if scores.dim() != 2:

@@ -14,6 +14,7 @@
  *     host memory of its own and no RESULT depends on an earlier call.  What it does keep between calls, all of it diagnostic:
  *       * one device word (static, not allocated): the fault word of the multi-wave online kernel, set by a hand-over that never
  *         arrives, read and cleared by dcarl_trace_status(); two more of the recurrence's waits, read and cleared by dcarl_recurrence_status();
+ *       * per process, the bound on polls that the test hook dcarl_debug_recurrence_polls() has set, if it has;
  *       * per thread, the text of the last error (dcarl_last_error) and the name of the last kernel launched (dcarl_last_kernel);
  *       * per process, a 64-entry memo {workspace address -> N, S, A, flags, element width} of the latest dcarl_ingest_group_* calls,
  *         consulted by dcarl_ingest_pack_* only to REFUSE a pack call whose arguments differ from its group call;
